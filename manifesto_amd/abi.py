@@ -39,6 +39,30 @@ class Operand(ctypes.Structure):
                 ("reserved", ctypes.c_uint8 * 6), ("period", ctypes.c_int64)]
 
 
+class KVCacheStruct(ctypes.Structure):
+    """mfh_kv_cache"""
+    _fields_ = [("dtype", ctypes.c_uint8), ("reserved", ctypes.c_uint8 * 3), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("pages", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+
+class RotaryShape(ctypes.Structure):
+    """mfh_rotary_shape"""
+    _fields_ = [("dtype", ctypes.c_uint8), ("interleaved", ctypes.c_uint8), ("inverse", ctypes.c_uint8),
+                ("reserved", ctypes.c_uint8), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("factor", ctypes.c_float),
+                *[(f"{t}_{of}_stride", ctypes.c_int64) for t in ("q", "q_out", "k", "k_out", "v") for of in ("token", "head")]]
+
+
+class AttentionShape(ctypes.Structure):
+    """mfh_attention_shape"""
+    _fields_ = [("dtype", ctypes.c_uint8), ("reserved", ctypes.c_uint8 * 3), ("q_heads", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int32),
+                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64)]
+
+
 _lib = None
 
 
@@ -62,7 +86,7 @@ def lib():
 
 def _declare(L):
     c = ctypes
-    vp, i64, i32, u8, f32 = c.c_void_p, c.c_int64, c.c_int32, c.c_uint8, c.c_float
+    vp, i64, i32, u8, f32, f64 = c.c_void_p, c.c_int64, c.c_int32, c.c_uint8, c.c_float, c.c_double
     sig = {
         "mfh_version": (c.c_int, []),
         "mfh_init": (c.c_int, [c.c_int]),
@@ -95,6 +119,19 @@ def _declare(L):
         "mfh_fusion_release": (c.c_int, [vp]),
         "mfh_fusion_cache_dir": (c.c_int, [c.c_char_p]),
         "mfh_fusion_cache_stats": (c.c_int, [c.POINTER(i64), c.POINTER(i64)]),
+        "mfh_page_plan": (c.c_int, [vp, vp, i32, i32, vp, i64, i32, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp]),
+        "mfh_rotary_frequencies": (c.c_int, [c.POINTER(f64), i32, f64, i32, f64, f64, f64, f64]),
+        "mfh_rotary": (c.c_int, [c.POINTER(RotaryShape), i64, vp, vp, vp, vp, vp, vp, vp]),
+        "mfh_rotary_append": (c.c_int, [c.POINTER(RotaryShape), c.POINTER(KVCacheStruct), i64, vp, vp, vp, vp, vp, vp, vp,
+                                        vp, vp, vp]),
+        "mfh_paged_decode": (c.c_int, [c.POINTER(AttentionShape), c.POINTER(KVCacheStruct), i32, vp, vp, vp, vp, i64, i32,
+                                       vp, i64, vp, vp, vp, vp, c.c_size_t, vp]),
+        "mfh_paged_decode_workspace": (c.c_int, [c.POINTER(AttentionShape), c.POINTER(KVCacheStruct), i32, i64,
+                                                 c.POINTER(c.c_size_t)]),
+        "mfh_paged_prefill": (c.c_int, [c.POINTER(AttentionShape), c.POINTER(KVCacheStruct), i32, i64, i64, vp, vp, vp, vp,
+                                        i64, i32, vp, vp, i64, vp, vp, vp, vp, vp, c.c_size_t, vp]),
+        "mfh_paged_prefill_workspace": (c.c_int, [c.POINTER(AttentionShape), c.POINTER(KVCacheStruct), i32, i64, i64, i64,
+                                                  c.POINTER(c.c_size_t)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -27,7 +27,7 @@ ARCH = "gfx950"
 
 SOURCES = ["runtime.cpp", "dequant.hip", "hostmath.hip", "scratch.hip", "fusion.cpp", "graph.cpp", "plan.cpp",
            "hostcopy.cpp",
-           "backend.cpp", "safetensors.cpp"]
+           "backend.cpp", "safetensors.cpp", "pages.hip", "rotary.hip", "decode.hip", "prefill.hip"]
 PRELUDE_PARTS = ["codec.hpp", "devmath.hpp", "fusion_io.hpp"]
 
 COMMON_FLAGS = [

@@ -1,0 +1,134 @@
+// paged.hpp — what the paged-cache kernels share: the cache's checks, exact
+// division by a launch's constants, 16-bit and FP8 pieces, matrix products.
+#ifndef MFH_PAGED_HPP
+#define MFH_PAGED_HPP
+
+#include "common.hpp"
+#include "launch.hpp"
+#include "../../include/mfh_attention.h"
+
+namespace mfh {
+
+int check_cache(const mfh_kv_cache* cache, const char* what);  // decode.hip
+int check_attention(const mfh_attention_shape* shape, const mfh_kv_cache* cache, const char* what);
+
+// Tokens of a request, and rows of a call, at most: sums and differences of two
+// positions and a window fit 32 bits.
+constexpr int kLongest = 1 << 30;
+
+// A descriptor's pair of strides, where two zeros stand for [tokens][heads][dim].
+struct Strides {
+    int64_t token, head;
+    Strides(int64_t t, int64_t h, int64_t heads, int64_t dim)
+        : token(t || h ? t : heads * dim), head(t || h ? h : dim)
+    {
+    }
+};
+
+// n / d for 32-bit n and a d known at launch: the high half of n * ceil(2^64 / d),
+// exact because the rounding adds n * d * 2^-64 < 1 / d at most.
+struct Divider {
+    mfh_u64 m;
+    mfh_u32 d;
+    Divider() = default;
+    explicit Divider(mfh_u32 by) : m(by > 1 ? ~mfh_u64(0) / by + 1 : 0), d(by) {}
+    __device__ mfh_u32 quotient(mfh_u32 n) const { return d == 1 ? n : (mfh_u32)__umul64hi(m, n); }
+    __device__ mfh_i64 quotient64(mfh_i64 n) const { return n >> 32 ? n / (mfh_i64)d : (mfh_i64)quotient((mfh_u32)n); }
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <int DT>
+MFH_DEV float dec16(mfh_u32 h)
+{
+    return DT == kBFloat16 ? mfh_bf16_to_f32(h) : mfh_f16_to_f32(h);
+}
+
+template <int DT>
+MFH_DEV mfh_u32 enc16x2(float lo, float hi)
+{
+    if constexpr (DT == kBFloat16) return mfh_bf16x2_rne(lo, hi);
+    else return mfh_f16x2_rne(lo, hi);
+}
+
+// Four E4M3 codes by the hardware's conversion (nearest, ties to even, into
+// subnormals too; the codec of mfh_convert keeps the reference's subnormal
+// rule instead), limited to the largest finite value first.  NaN stays NaN.
+MFH_DEV float e4m3_limit(float v) { return v > 448.0f ? 448.0f : v < -448.0f ? -448.0f : v; }
+
+MFH_DEV mfh_u32 e4m3x4(float v0, float v1, float v2, float v3)
+{
+    mfh_u32 w = (mfh_u32)__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_limit(v0), e4m3_limit(v1), 0, false);
+    return (mfh_u32)__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_limit(v2), e4m3_limit(v3), (int)w, true);
+}
+
+// Two of a dword's four E4M3 codes as bf16 or f16 (both hold every code exactly).
+template <int DT, bool HIGH>
+MFH_DEV mfh_u32 e4m3_pair(mfh_u32 codes)
+{
+    if constexpr (DT == kBFloat16)
+        return __builtin_bit_cast(mfh_u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, HIGH));
+    else return __builtin_bit_cast(mfh_u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, HIGH));
+}
+
+// c + a b with eight 16-bit values of a's row and of b's column per lane.
+// 16 x 16 x 32: row / column lane % 16, values 8 * (lane / 16) ..; c: column
+// lane % 16, rows 4 * (lane / 16) ...
+template <int DT>
+MFH_DEV f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c)
+{
+    if constexpr (DT == kBFloat16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// 32 x 32 x 16: row / column lane % 32, values 8 * (lane / 32) ..; c: column
+// lane % 32, element i is row 8 * (i / 4) + 4 * (lane / 32) + i % 4.
+template <int DT>
+MFH_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
+{
+    if constexpr (DT == kBFloat16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+MFH_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// cap * tanh(x / cap) * log2(e), from twice = 2 log2(e) / cap and scaled = cap log2(e):
+// tanh y = 1 - 2 / (1 + e^2y), which ends at -1 and 1 without a case of its own.
+MFH_DEV float capped(float x, float twice, float scaled)
+{
+    return scaled * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + exp2_fast(x * twice)));
+}
+
+// Pages a kernel reads: strides in bytes, of keys and of values alike.
+struct PageArgs {
+    const char* k;
+    const char* v;
+    const int32_t* table;
+    int64_t table_stride;
+    int64_t page_bytes, token_bytes, head_bytes;
+    int64_t pages;
+    Divider by_page;  // page size
+    mfh_u32 width;
+};
+
+// The part of a split sequence that each workgroup takes: `tiles` tiles in
+// parts of at least `least` tiles, at most `parts` of them.
+MFH_DEV mfh_u32 part_tiles(mfh_u32 tiles, mfh_u32 least, mfh_u32 parts)
+{
+    return max(least, (tiles + parts - 1) / parts);
+}
+
+}  // namespace mfh
+
+#endif  // MFH_PAGED_HPP
