@@ -85,20 +85,22 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kHeads = 16;   // query heads of a workgroup
 constexpr float kStep = 8.0f;  // the reference moves where a score passes it by 2^kStep
 
+// A row is a request's key-value head with up to 16 of its query heads.
 struct DecodeArgs {
     PageArgs pages;
     const char* q;
     char* out;
     float* lse;
-    float* part_out;   // [requests * q_heads][parts][head_dim]
-    float2* part_sum;  // [requests * q_heads][parts]: reference and sum
+    float* part_out;     // [slots][part_heads][head_dim]
+    float2* part_sum;    // [slots][part_heads]: reference and sum
     const int32_t* lengths;
     const float* slopes;
     int64_t q_t, q_h, out_t, out_h;  // elements
     float scale, cap_twice, cap_scaled, v_scale;
-    int32_t window, requests, kv_heads, q_heads, group, head_groups, dim;
-    mfh_u32 parts, least;  // of a request; tiles of a part at least
-    Divider by_parts, by_head_groups, by_kv_heads;
+    int32_t window, requests, kv_heads, q_heads, group, head_groups, dim, part_heads;
+    mfh_u32 request_rows;  // kv_heads * head_groups
+    mfh_u32 blocks;        // of the split form
+    Divider by_head_groups, by_request_rows, by_blocks, by_q_heads;
 };
 
 MFH_DEV mfh_u32 low_halves(mfh_u32 a, mfh_u32 b) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
@@ -117,111 +119,247 @@ struct Context {
     }
 };
 
+// The split form: all rows' tiles go to `blocks` workgroups, a piece each; a
+// row's pieces are its own, of equal size, so that there are `rows` workgroups
+// more at most.  Short rows end early and make room for the next workgroup.
+// The host takes this form only where the number of all tiles fits 31 bits.
+MFH_DEV mfh_u32 lane_tiles(const DecodeArgs& a, mfh_u32 r) { return r < (mfh_u32)a.requests ? Context(a, r).tiles : 0; }
+
+MFH_DEV mfh_u32 piece_of(const DecodeArgs& a, int lane)
+{
+    mfh_u32 sum = 0;
+    for (mfh_u32 base = 0; base < (mfh_u32)a.requests; base += 64) sum += lane_tiles(a, base + lane);
+    const mfh_u32 total = last_lane(lanes_upto(sum)) * a.request_rows;
+    return max(a.by_blocks.quotient(total + a.blocks - 1), (mfh_u32)kWaves);
+}
+
+MFH_DEV mfh_u32 parts_of(mfh_u32 tiles, mfh_u32 piece) { return (tiles + piece - 1) / piece; }
+
 // Where a tile's 32 tokens stand.  Where a page holds whole groups of 16 tokens
 // (FAST) the two halves have a uniform offset each and the lanes' own offsets
 // never change; else lane i % 32 looks token i up and the others ask for it.
+// The table is read a tile before its pages are.
 template <bool FAST>
 struct TileAt {
-    int64_t half[2];
-    int64_t mine;
+    mfh_i64 page[2];    // FAST: of each half, its page
+    mfh_u32 in_page[2]; // and its first row there, in bytes
+    mfh_i64 mine;
     mfh_u32 valid;  // bit i: token i is seen and has a page
 };
 
-MFH_DEV int64_t uniform64(int64_t v)
+// Bit i: whether first + i is in [from, to), for 16 i.
+MFH_DEV mfh_u32 range_bits(mfh_u32 first, mfh_u32 from, mfh_u32 to)
 {
-    const mfh_u32 lo = __builtin_amdgcn_readfirstlane((int)(mfh_u32)v);
-    const mfh_u32 hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-    return (int64_t)((mfh_u64)hi << 32 | lo);
-}
-
-MFH_DEV int64_t shuffle64(int64_t v, int lane)
-{
-    const mfh_u32 lo = __shfl((int)(mfh_u32)v, lane), hi = __shfl((int)(v >> 32), lane);
-    return (int64_t)((mfh_u64)hi << 32 | lo);
+    const mfh_u32 low = from > first ? min(from - first, 16u) : 0, high = to > first ? min(to - first, 16u) : 0;
+    return (1u << high) - 1 & ~((1u << low) - 1);
 }
 
 template <bool FAST>
-MFH_DEV TileAt<FAST> locate(const PageArgs& p, const int32_t* table, const Context& c, mfh_u32 t0, int lane)
-{
-    TileAt<FAST> at;
-    if constexpr (FAST) {
-        at.valid = 0;
+struct Pages {
+    int32_t page[2];
+    __device__ void ask(const PageArgs& p, const int32_t* table, const Context& c, mfh_u32 t0, int lane)
+    {
+        // past the length its last page again
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const mfh_u32 t = t0 + 16 * h;
-            const mfh_u32 row = p.by_page.quotient(t), in_page = t - row * p.by_page.d;
-            const int32_t page = __builtin_amdgcn_readfirstlane(t < c.length ? table[row] : -1);
-            const bool ok = page >= 0 && page < p.pages;
-            at.half[h] = (ok ? page : 0) * p.page_bytes + in_page * p.token_bytes;
-            if (ok) {
-                const mfh_u32 below = c.length - t;  // > 0
-                mfh_u32 bits = below >= 16 ? 0xffffu : (1u << below) - 1;
-                if (c.first > t) bits &= c.first - t >= 16 ? 0 : 0xffffu << (c.first - t);
-                at.valid |= (bits & 0xffffu) << (16 * h);
+        for (int h = 0; h < (FAST ? 2 : 1); h++)
+            page[h] = table[p.by_page.quotient(min(t0 + (FAST ? 16 * h : lane & 31), c.length - 1))];
+    }
+    // `real`: the tile is one of the wave's; else nothing of it is valid.
+    __device__ TileAt<FAST> place(const PageArgs& p, const Context& c, mfh_u32 t0, int lane, bool real) const
+    {
+        TileAt<FAST> at;
+        if constexpr (FAST) {
+            at.valid = 0;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const mfh_u32 t = t0 + 16 * h;
+                const mfh_u32 n = uniform((mfh_u32)page[h]);
+                const bool ok = real && t < c.length && n < p.pages;
+                at.page[h] = ok ? (mfh_i64)n : -1;
+                at.in_page[h] = (t - p.by_page.quotient(t) * p.by_page.d) * p.token_bytes;
+                if (ok) at.valid |= range_bits(t, c.first, c.length) << (16 * h);
             }
+        } else {
+            const mfh_u32 t = t0 + (lane & 31);
+            const bool ok = real && t < c.length && t >= c.first && (mfh_u32)page[0] < p.pages;
+            at.mine = ok ? (mfh_u32)page[0] * p.page_bytes + (t - p.by_page.quotient(t) * p.by_page.d) * p.token_bytes : 0;
+            at.valid = (mfh_u32)__ballot(ok);
         }
-    } else {
-        const mfh_u32 t = t0 + (lane & 31);
-        const mfh_u32 row = p.by_page.quotient(t), in_page = t - row * p.by_page.d;
-        const bool seen = t < c.length && t >= c.first;
-        const int32_t page = seen ? table[row] : -1;
-        const bool ok = page >= 0 && page < p.pages;
-        at.mine = (ok ? page : 0) * p.page_bytes + (ok ? in_page : 0) * p.token_bytes;
-        at.valid = (mfh_u32)__ballot(ok);
+        return at;
     }
-    return at;
+};
+
+// A page's rows of one head as a buffer; without a page one that has no bytes,
+// from which loads give zeros and move nothing.
+MFH_DEV __amdgpu_buffer_rsrc_t page_buffer(const char* base, mfh_i64 page, const PageArgs& p)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + max(page, (mfh_i64)0) * p.page_bytes), 0,
+                                             page < 0 ? 0 : (int)p.page_span, 0x00020000);
 }
 
-template <int DT, bool FP8>
-MFH_DEV u32x4 load_eight(const char* p)
+constexpr int kStreamed = 2;  // nt: keys and values are read once
+
+template <typename T>
+MFH_DEV T buffer_piece(__amdgpu_buffer_rsrc_t r, mfh_u32 lane_at, mfh_u32 at)
 {
-    if constexpr (FP8) {
-        const u32x2 w = load8<true>(p);
-        return u32x4{e4m3_pair<DT, false>(w[0]), e4m3_pair<DT, true>(w[0]), e4m3_pair<DT, false>(w[1]),
-                     e4m3_pair<DT, true>(w[1])};
-    } else {
-        return load16<true>(p);
-    }
+    if constexpr (sizeof(T) == 16) return __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane_at, (int)at, kStreamed);
+    else if constexpr (sizeof(T) == 8) return __builtin_amdgcn_raw_buffer_load_b64(r, (int)lane_at, (int)at, kStreamed);
+    else return __builtin_amdgcn_raw_buffer_load_b32(r, (int)lane_at, (int)at, kStreamed);
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.
-template <int DT, bool FP8, int DP, bool FAST>
-__global__ __launch_bounds__(kThreads) void k_decode(DecodeArgs a)
+// Eight codes as 16-bit values.
+template <int DT>
+MFH_DEV u32x4 widen(mfh_u32 lo, mfh_u32 hi)
 {
-    constexpr int kSteps = DP / 32;               // of the product with K
+    return u32x4{e4m3_pair<DT, false>(lo), e4m3_pair<DT, true>(lo), e4m3_pair<DT, false>(hi), e4m3_pair<DT, true>(hi)};
+}
+
+// What a lane loads of a token of V: 8 dims (4 where head_dim is at most 64).
+template <bool FP8, int DIMS> struct Piece { typedef u32x4 type; };
+template <> struct Piece<false, 4> { typedef u32x2 type; };
+template <> struct Piece<true, 8> { typedef u32x2 type; };
+template <> struct Piece<true, 4> { typedef mfh_u32 type; };
+
+template <typename T>
+MFH_DEV T load_piece(const char* p)
+{
+    if constexpr (sizeof(T) == 16) return load16<true>(p);
+    else if constexpr (sizeof(T) == 8) return load8<true>(p);
+    else return load4(p);
+}
+
+template <int DT, bool FP8, int DIMS>
+MFH_DEV u32x4 dims_of(typename Piece<FP8, DIMS>::type w)
+{
+    if constexpr (!FP8 && DIMS == 8) return w;
+    else if constexpr (!FP8) return u32x4{w[0], w[1], 0, 0};
+    else if constexpr (DIMS == 8) return widen<DT>(w[0], w[1]);
+    else return u32x4{e4m3_pair<DT, false>(w), e4m3_pair<DT, true>(w), 0, 0};
+}
+
+// DP: head_dim rounded up to 64, 128 or 256.  SPLIT: the line of all tiles in
+// equal pieces, joined by k_decode_join; else a workgroup takes one row.
+template <int DT, bool FP8, int DP, bool FAST, bool SPLIT>
+__global__ __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_decode(DecodeArgs a)
+{
+    constexpr int kSteps = DP / 32;                 // of the product with K
+    constexpr int kLoads = FP8 ? kSteps / 2 : kSteps;  // of 16 bytes of a token of K
     constexpr int kSets = DP == 64 ? 1 : DP / 128;  // of 16 lanes' dims in V
-    constexpr int kDims = DP == 64 ? 4 : 8;       // of a lane in a set
+    constexpr int kDims = DP == 64 ? 4 : 8;         // of a lane in a set
     constexpr int kBytes = FP8 ? 1 : 2;
     constexpr int kSetDims = 16 * kDims;
+    typedef typename Piece<FP8, kDims>::type VPiece;
+
+    __shared__ float s_ref[kWaves][kHeads], s_sum[kWaves][kHeads];
+    __shared__ float s_out[kWaves][kHeads][kSetDims + 4];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
-    mfh_u32 at = blockIdx.x;
-    mfh_u32 rest = a.by_parts.quotient(at);
-    const mfh_u32 part = at - rest * a.parts;
-    at = rest;
-    rest = a.by_head_groups.quotient(at);
-    const mfh_u32 head_group = at - rest * a.head_groups;
-    const mfh_u32 r = a.by_kv_heads.quotient(rest), kv = rest - r * a.kv_heads;
 
+    // This workgroup's row and its tiles.  Every wave finds them by itself.
+    mfh_u32 r, row_of, part = 0, parts = 1;
+    if constexpr (!SPLIT) {
+        r = a.by_request_rows.quotient(blockIdx.x);
+        row_of = blockIdx.x - r * a.request_rows;
+    } else {
+        const mfh_u32 piece = piece_of(a, lane);
+        mfh_u32 before = 0;
+        r = ~0u, row_of = 0;
+        for (mfh_u32 base = 0; base < (mfh_u32)a.requests; base += 64) {
+            const mfh_u32 its = parts_of(lane_tiles(a, base + lane), piece), upto = before + lanes_upto(its);
+            const mfh_u64 past = __ballot(upto * a.request_rows > blockIdx.x);
+            if (past) {  // the first request whose workgroups end past this one
+                const int at = __ffsll((unsigned long long)past) - 1;
+                parts = (mfh_u32)__builtin_amdgcn_readlane((int)its, at);
+                const mfh_u32 in_request = blockIdx.x - ((mfh_u32)__builtin_amdgcn_readlane((int)upto, at) - parts) * a.request_rows;
+                r = base + at;
+                row_of = in_request / parts;
+                part = in_request - row_of * parts;
+                break;
+            }
+            before = last_lane(upto);
+        }
+        if (r == ~0u) return;
+        // known to be uniform, the tables are read as scalars: their loads and
+        // those of the pages are then not waited for together
+        r = uniform(r), row_of = uniform(row_of), part = uniform(part), parts = uniform(parts);
+    }
     const Context c(a, r);
-    const mfh_u32 size = part_tiles(c.tiles, a.least, a.parts);
-    const mfh_u32 used = max(1u, (c.tiles + size - 1) / size);
-    if (part >= used) return;
-    const mfh_u32 begin = c.tile0 + part * size, end = min(begin + size, c.tile0 + c.tiles);
+    const mfh_u32 share = uniform((c.tiles + parts - 1) / parts);
+    const mfh_u32 begin = c.tile0 + min(part * share, c.tiles), end = c.tile0 + min((part + 1) * share, c.tiles);
 
+    const mfh_u32 token_bytes = a.pages.token_bytes;
+    // Lanes past head_dim read its last dims again, inside the row: their
+    // steps have zeros in Q (and, below, in K), their results are not written.
+    // A step of K takes eight dims of each quad; an 8-bit load holds two steps'.
+    auto dim_of = [&](int s) { return FP8 ? 64 * (s / 2) + 16 * quad + 8 * (s & 1) : 32 * s + 8 * quad; };
+    mfh_u32 k_lane[kLoads], v_lane[kSets];
+#pragma unroll
+    for (int s = 0; s < kLoads; s++)
+        k_lane[s] = (FAST ? col * token_bytes : 0) + (FP8 ? min(64 * s + 16 * quad, a.dim - 16) : min(32 * s + 8 * quad, a.dim - 8) * 2);
+#pragma unroll
+    for (int u = 0; u < kSets; u++)
+        v_lane[u] = (FAST ? 4 * quad * token_bytes : 0) + min(u * kSetDims + kDims * col, a.dim - kDims) * kBytes;
+    const bool ragged = a.dim != DP;
+
+    const mfh_u32 head_group = row_of % a.head_groups, kv = a.by_head_groups.quotient(row_of);
     const int heads = min(kHeads, a.group - (int)head_group * kHeads);
     const int head0 = kv * a.group + head_group * kHeads;
     const int32_t* table = a.pages.table + (int64_t)r * a.pages.table_stride;
     const char* k_base = a.pages.k + kv * a.pages.head_bytes;
     const char* v_base = a.pages.v + kv * a.pages.head_bytes;
-    const mfh_u32 token_bytes = (mfh_u32)a.pages.token_bytes;
 
-    // Q^T: head `col`, dims 32 s + 8 quad ..
+    Pages<FAST> pages;
+    auto load = [&](u32x4 (&k)[2][kLoads], VPiece (&v)[kSets][8], mfh_u32& valid, mfh_u32 tile) {
+        const TileAt<FAST> at = pages.place(a.pages, c, tile * kTile, lane, tile < end);
+        valid = at.valid;
+        if constexpr (FAST) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const __amdgpu_buffer_rsrc_t rows = page_buffer(k_base, at.page[h], a.pages);
+#pragma unroll
+                for (int s = 0; s < kLoads; s++) k[h][s] = buffer_piece<u32x4>(rows, k_lane[s], at.in_page[h]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const __amdgpu_buffer_rsrc_t rows = page_buffer(v_base, at.page[h], a.pages);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int u = 0; u < kSets; u++)
+                        v[u][4 * h + j] = buffer_piece<VPiece>(rows, v_lane[u], at.in_page[h] + j * token_bytes);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const char* row = k_base + shuffle64(at.mine, 16 * h + col);
+#pragma unroll
+                for (int s = 0; s < kLoads; s++) k[h][s] = load16<true>(row + k_lane[s]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const char* row = v_base + shuffle64(at.mine, 16 * (j >> 2) + 4 * quad + (j & 3));
+#pragma unroll
+                for (int u = 0; u < kSets; u++) v[u][j] = load_piece<VPiece>(row + v_lane[u]);
+            }
+        }
+    };
+    mfh_u32 tile = begin + wave;
+    // Two tiles' registers: one is on its way while the other is computed.
+    u32x4 k_a[2][kLoads], k_b[2][kLoads];
+    VPiece v_a[kSets][8], v_b[kSets][8];
+    mfh_u32 valid_a = 0, valid_b = 0;
+    if (tile < end) {
+        pages.ask(a.pages, table, c, tile * kTile, lane);
+        load(k_a, v_a, valid_a, tile);
+        pages.ask(a.pages, table, c, (tile + kWaves) * kTile, lane);
+    }
+
+    // Q^T: head `col`, the dims of each step
     u32x4 q[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; s++) {
-        const int d = 32 * s + 8 * quad;
+        const int d = dim_of(s);
         q[s] = u32x4{0, 0, 0, 0};
         if (col < heads && d < a.dim)
             q[s] = load16<false>(a.q + ((int64_t)r * a.q_t + (int64_t)(head0 + col) * a.q_h + d) * 2);
@@ -235,71 +373,26 @@ __global__ __launch_bounds__(kThreads) void k_decode(DecodeArgs a)
         for (int d = 0; d < kDims; d++) acc[u][d] = f32x4{0, 0, 0, 0};
     float ref = 0.0f, limit = -INFINITY, sum = 0.0f;
 
-    // Lanes past head_dim read its last dims again, inside the row: their
-    // steps have zeros in Q (and, below, in K), their results are not written.
-    mfh_u32 k_lane[kSteps], v_lane[kSets];
-#pragma unroll
-    for (int s = 0; s < kSteps; s++)
-        k_lane[s] = (FAST ? col * token_bytes : 0) + min(32 * s + 8 * quad, a.dim - 8) * kBytes;
-#pragma unroll
-    for (int u = 0; u < kSets; u++)
-        v_lane[u] = (FAST ? 4 * quad * token_bytes : 0) + min(u * kSetDims + kDims * col, a.dim - kDims) * kBytes;
-    const bool ragged = a.dim != DP;
-
-    u32x4 k[2][kSteps];
-    auto load_k = [&](const TileAt<FAST>& w) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const char* row;
-            if constexpr (FAST) row = k_base + w.half[h];
-            else row = k_base + shuffle64(w.mine, 16 * h + col);
-#pragma unroll
-            for (int s = 0; s < kSteps; s++) k[h][s] = load_eight<DT, FP8>(row + k_lane[s]);
-        }
-    };
-
-    mfh_u32 tile = begin + wave;
-    TileAt<FAST> now, next;
-    if (tile < end) {
-        now = locate<FAST>(a.pages, table, c, tile * kTile, lane);
-        load_k(now);
-    }
-    for (; tile < end; tile += kWaves) {
-        const bool more = tile + kWaves < end;
-        u32x4 v[kSets][8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const char* row;
-            if constexpr (FAST) row = v_base + (now.half[j >> 2] + (j & 3) * (int64_t)token_bytes);
-            else row = v_base + shuffle64(now.mine, 16 * (j >> 2) + 4 * quad + (j & 3));
-#pragma unroll
-            for (int u = 0; u < kSets; u++) {
-                if constexpr (kDims == 8) {
-                    v[u][j] = load_eight<DT, FP8>(row + v_lane[u]);
-                } else if constexpr (FP8) {
-                    const mfh_u32 w = load4(row + v_lane[u]);
-                    v[u][j] = u32x4{e4m3_pair<DT, false>(w), e4m3_pair<DT, true>(w), 0, 0};
-                } else {
-                    const u32x2 w = load8<true>(row + v_lane[u]);
-                    v[u][j] = u32x4{w[0], w[1], 0, 0};
-                }
-            }
-        }
-        if (ragged) {
-#pragma unroll
-            for (int s = 0; s < kSteps; s++)
-                if (32 * s + 8 * quad >= a.dim) k[0][s] = k[1][s] = u32x4{0, 0, 0, 0};
-        }
+    auto compute = [&](u32x4 (&k)[2][kLoads], VPiece (&v)[kSets][8], mfh_u32 valid) {
         f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+        auto product = [&](auto cut) {
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) {
-            s0 = mfma16<DT>(k[0][s], q[s], s0);
-            s1 = mfma16<DT>(k[1][s], q[s], s1);
-        }
-        if (more) {
-            next = locate<FAST>(a.pages, table, c, (tile + kWaves) * kTile, lane);
-            load_k(next);
-        }
+            for (int s = 0; s < kSteps; s++) {
+                u32x4 k0, k1;
+                if constexpr (FP8) {
+                    const int w = 2 * (s & 1);
+                    k0 = widen<DT>(k[0][s / 2][w], k[0][s / 2][w + 1]);
+                    k1 = widen<DT>(k[1][s / 2][w], k[1][s / 2][w + 1]);
+                } else {
+                    k0 = k[0][s], k1 = k[1][s];
+                }
+                if (cut.value && dim_of(s) >= a.dim) k0 = k1 = u32x4{0, 0, 0, 0};
+                s0 = mfma16<DT>(k0, q[s], s0);
+                s1 = mfma16<DT>(k1, q[s], s1);
+            }
+        };
+        if (ragged) product(std::true_type{});
+        else product(std::false_type{});
 
         float x[8];
 #pragma unroll
@@ -313,13 +406,13 @@ __global__ __launch_bounds__(kThreads) void k_decode(DecodeArgs a)
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] -= slope * (float)(back - (16 * (j >> 2) + (j & 3)));
         }
-        if (now.valid != 0xffffffffu) {
+        if (valid != 0xffffffffu) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                if (!(now.valid >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1)) {
+                if (!(valid >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1)) {
                     x[j] = -INFINITY;
 #pragma unroll
-                    for (int u = 0; u < kSets; u++) v[u][j] = u32x4{0, 0, 0, 0};  // 0 * NaN would be NaN
+                    for (int u = 0; u < kSets; u++) v[u][j] = VPiece{};  // 0 * NaN would be NaN
                 }
             }
         }
@@ -348,149 +441,191 @@ __global__ __launch_bounds__(kThreads) void k_decode(DecodeArgs a)
         sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
         for (int u = 0; u < kSets; u++) {
+            u32x4 t[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) t[j] = dims_of<DT, FP8, kDims>(v[u][j]);
 #pragma unroll
             for (int d = 0; d < kDims; d += 2) {
-                const int w = d / 2;
-                const u32x4 even = {low_halves(v[u][0][w], v[u][1][w]), low_halves(v[u][2][w], v[u][3][w]),
-                                    low_halves(v[u][4][w], v[u][5][w]), low_halves(v[u][6][w], v[u][7][w])};
-                const u32x4 odd = {high_halves(v[u][0][w], v[u][1][w]), high_halves(v[u][2][w], v[u][3][w]),
-                                   high_halves(v[u][4][w], v[u][5][w]), high_halves(v[u][6][w], v[u][7][w])};
+                const int i = d / 2;
+                const u32x4 even = {low_halves(t[0][i], t[1][i]), low_halves(t[2][i], t[3][i]),
+                                    low_halves(t[4][i], t[5][i]), low_halves(t[6][i], t[7][i])};
+                const u32x4 odd = {high_halves(t[0][i], t[1][i]), high_halves(t[2][i], t[3][i]),
+                                   high_halves(t[4][i], t[5][i]), high_halves(t[6][i], t[7][i])};
                 acc[u][d] = mfma16<DT>(even, p, acc[u][d]);
                 acc[u][d + 1] = mfma16<DT>(odd, p, acc[u][d + 1]);
             }
         }
-        now = next;
+    };
+    // Loads of a tile past the last one are made too, and move nothing:
+    // behind loads that only some iterations make, the compiler waits for
+    // all that are on their way.
+    while (tile < end) {
+        load(k_b, v_b, valid_b, tile + kWaves);
+        pages.ask(a.pages, table, c, (tile + 2 * kWaves) * kTile, lane);
+        compute(k_a, v_a, valid_a);
+        tile += kWaves;
+        if (tile >= end) break;
+        load(k_a, v_a, valid_a, tile + kWaves);
+        pages.ask(a.pages, table, c, (tile + 2 * kWaves) * kTile, lane);
+        compute(k_b, v_b, valid_b);
+        tile += kWaves;
     }
 
     // The waves' results meet: a common reference, then sums weighted by it.
-    __shared__ float s_ref[kWaves][kHeads], s_sum[kWaves][kHeads];
-    __shared__ float s_out[kWaves][kHeads][kSetDims + 4];
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
+    const float wave_ref = limit == -INFINITY ? -INFINITY : ref;
     if (quad == 0) {
-        s_ref[wave][col] = limit == -INFINITY ? -INFINITY : ref;
+        s_ref[wave][col] = wave_ref;
         s_sum[wave][col] = sum;
     }
+    __syncthreads();
+    float top = s_ref[0][col];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) top = fmaxf(top, s_ref[w][col]);
+    const float weight = wave_ref == -INFINITY ? 0.0f : exp2_fast(wave_ref - top);
+#pragma unroll
     for (int u = 0; u < kSets; u++) {
         if (u) __syncthreads();
 #pragma unroll
-        for (int uu = 0; uu < kSets; uu++) {
-            if (uu != u) continue;
+        for (int d = 0; d < kDims; d++)
 #pragma unroll
-            for (int d = 0; d < kDims; d++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) s_out[wave][col][kDims * (4 * quad + i) + d] = acc[uu][d][i];
-        }
+            for (int i = 0; i < 4; i++) s_out[wave][col][kDims * (4 * quad + i) + d] = weight * acc[u][d][i];
         __syncthreads();
-        const int pairs = min(kSetDims, a.dim - u * kSetDims) / 2;
+        const int dims = min(kSetDims, a.dim - u * kSetDims);
         for (int i = threadIdx.x; i < heads * (kSetDims / 2); i += kThreads) {
-            const int h = i / (kSetDims / 2), d = 2 * (i % (kSetDims / 2));
-            if (d >= 2 * pairs) continue;
-            float top = s_ref[0][h];
+            const int h = i / (kSetDims / 2), d = 2 * (i % (kSetDims / 2)), dim = u * kSetDims + d;
+            if (d >= dims) continue;
+            float all = s_ref[0][h], total = 0.0f, o0 = 0.0f, o1 = 0.0f;
 #pragma unroll
-            for (int w = 1; w < kWaves; w++) top = fmaxf(top, s_ref[w][h]);
-            float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+            for (int w = 1; w < kWaves; w++) all = fmaxf(all, s_ref[w][h]);
+#pragma unroll
+            for (int w = 0; w < kWaves; w++)
+                total += s_ref[w][h] == -INFINITY ? 0.0f : exp2_fast(s_ref[w][h] - all) * s_sum[w][h];
 #pragma unroll
             for (int w = 0; w < kWaves; w++) {
-                const float f = s_ref[w][h] == -INFINITY ? 0.0f : exp2_fast(s_ref[w][h] - top);
-                total += f * s_sum[w][h];
-                o0 += f * s_out[w][h][d];
-                o1 += f * s_out[w][h][d + 1];
+                o0 += s_out[w][h][d];
+                o1 += s_out[w][h][d + 1];
             }
-            const int64_t row = (int64_t)r * a.q_heads + head0 + h;
-            const int dim = u * kSetDims + d;
-            if (used > 1) {
-                const int64_t slot = row * a.parts + part;
-                float2* o = reinterpret_cast<float2*>(a.part_out + slot * a.dim + dim);
-                *o = make_float2(o0, o1);
-                if (dim == 0) a.part_sum[slot] = make_float2(top, total);
-            } else {
+            if (!SPLIT || parts == 1) {
                 const float f = total == 0.0f ? 0.0f : a.v_scale / total;
                 store4(a.out + ((int64_t)r * a.out_t + (int64_t)(head0 + h) * a.out_h + dim) * 2, enc16x2<DT>(o0 * f, o1 * f));
-                if (dim == 0 && a.lse) a.lse[row] = total == 0.0f ? -INFINITY : top * kLn2 + logf(total);
+                if (dim == 0 && a.lse)
+                    a.lse[(int64_t)r * a.q_heads + head0 + h] = total == 0.0f ? -INFINITY : all * kLn2 + logf(total);
+            } else {
+                const int64_t slot = (int64_t)blockIdx.x * a.part_heads + h;
+                *reinterpret_cast<float2*>(a.part_out + slot * a.dim + dim) = make_float2(o0, o1);
+                if (dim == 0) a.part_sum[slot] = make_float2(all, total);
             }
         }
     }
 }
 
-// Joins a request's parts, one wave per query head; lane l takes the dims
-// 2 l + 128 u.
+// Joins the parts of the rows that have several, and writes the rows of
+// requests without tokens.  A workgroup takes 128 dims of a query head, a
+// quarter of the parts in each wave; lanes take two dims each.
+constexpr int kJoinWaves = 4;
+
 template <int DT>
-__global__ __launch_bounds__(64) void k_decode_join(DecodeArgs a)
+__global__ __launch_bounds__(64 * kJoinWaves) void k_decode_join(DecodeArgs a)
 {
-    const mfh_u32 r = blockIdx.x / a.q_heads, h = blockIdx.x - r * a.q_heads;
+    __shared__ float s_all[kJoinWaves];
+    __shared__ float2 s_out[kJoinWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int chunks = (a.dim + 127) / 128;
+    const mfh_u32 head_row = blockIdx.x / chunks, chunk = blockIdx.x - head_row * chunks;
+    const mfh_u32 r = a.by_q_heads.quotient(head_row), head = head_row - r * a.q_heads;
+    const mfh_u32 kv = head / a.group, in_group = head - kv * a.group;
+    const mfh_u32 row_of = kv * a.head_groups + in_group / kHeads, h = in_group % kHeads;
     const Context c(a, r);
-    const mfh_u32 size = part_tiles(c.tiles, a.least, a.parts);
-    const mfh_u32 used = (c.tiles + size - 1) / size;
-    if (used <= 1) return;
-    const int lane = threadIdx.x;
-    const int64_t row = (int64_t)r * a.q_heads + h;
-    const float2* sums = a.part_sum + row * a.parts;
+    const mfh_u32 piece = piece_of(a, lane), parts = parts_of(c.tiles, piece);
+    if (parts == 1) return;  // one workgroup had it all
+    mfh_u32 before = 0;
+    for (mfh_u32 base = 0; base < r; base += 64)
+        if (base + lane < r) before += parts_of(lane_tiles(a, base + lane), piece);
+    const int64_t slot0 = (int64_t)last_lane(lanes_upto(before)) * a.request_rows + (mfh_u64)row_of * parts;
+    const int d = 128 * chunk + 2 * lane;
+    const float2* sums = a.part_sum + slot0 * a.part_heads + h;
+    const float* from = a.part_out + (slot0 * a.part_heads + h) * a.dim + min(d, a.dim - 2);
     float top = -INFINITY;
-    for (mfh_u32 i = lane; i < used; i += 64) top = fmaxf(top, sums[i].x);
+    for (mfh_u32 n = lane; n < parts; n += 64) top = fmaxf(top, sums[(int64_t)n * a.part_heads].x);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    float total = 0.0f, o[4] = {0, 0, 0, 0};
-    for (mfh_u32 i = 0; i < used; i++) {
-        const float2 s = sums[i];
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    float all = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 4
+    for (mfh_u32 n = wave; n < parts; n += kJoinWaves) {
+        const float2 s = sums[(int64_t)n * a.part_heads];
+        const float2 w = *reinterpret_cast<const float2*>(from + (int64_t)n * a.part_heads * a.dim);
         const float f = s.x == -INFINITY ? 0.0f : exp2_fast(s.x - top);
-        total += f * s.y;
-        const float* from = a.part_out + (row * a.parts + i) * a.dim;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int d = 128 * u + 2 * lane;
-            if (d < a.dim) {
-                const float2 w = *reinterpret_cast<const float2*>(from + d);
-                o[2 * u] += f * w.x;
-                o[2 * u + 1] += f * w.y;
-            }
-        }
+        all += f * s.y;
+        o0 += f * w.x;
+        o1 += f * w.y;
     }
-    const float f = total == 0.0f ? 0.0f : a.v_scale / total;
+    if (lane == 0) s_all[wave] = all;
+    s_out[wave][lane] = make_float2(o0, o1);
+    __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        const int d = 128 * u + 2 * lane;
-        if (d < a.dim)
-            store4(a.out + ((int64_t)r * a.out_t + (int64_t)h * a.out_h + d) * 2, enc16x2<DT>(o[2 * u] * f, o[2 * u + 1] * f));
+    for (int w = 1; w < kJoinWaves; w++) {
+        all += s_all[w];
+        o0 += s_out[w][lane].x;
+        o1 += s_out[w][lane].y;
     }
-    if (lane == 0 && a.lse) a.lse[row] = total == 0.0f ? -INFINITY : top * kLn2 + logf(total);
+    if (d >= a.dim) return;
+    const float f = all == 0.0f ? 0.0f : a.v_scale / all;
+    store4(a.out + ((int64_t)r * a.out_t + (int64_t)head * a.out_h + d) * 2, enc16x2<DT>(o0 * f, o1 * f));
+    if (d == 0 && a.lse) a.lse[(int64_t)r * a.q_heads + head] = all == 0.0f ? -INFINITY : top * kLn2 + logf(all);
 }
 
-template <int DT, bool FP8, int DP>
-void launch_pages(bool fast, unsigned grid, hipStream_t s, const DecodeArgs& a)
+// How a call is laid out, from what the host knows: the number of rows and the
+// lengths' upper bound.
+struct Layout {
+    bool split;
+    int64_t rows;
+    mfh_u32 blocks;
+    int part_heads;
+    size_t bytes;
+};
+
+// One workgroup a row where rows are short, and no second kernel: up to 16
+// tiles (8 rows of 512 tokens 10.7 us, split 12.8), and up to 32 where the rows
+// alone fill the card (256 rows of 1024 tokens 24.2 us, split 27.6).  Beyond,
+// and where lengths may differ much, the split wins: 8 rows of 2048 tokens 28.6
+// and 12.6 us, 512 rows of 1..4096 74 and 44.  The split aims at one workgroup
+// per CU: two come out slower at 256 dims (33.5 us, 39.7) and for 64 rows
+// (14.9, 15.8), and equal or 8% faster elsewhere.
+Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cache& c, int32_t requests, int64_t longest)
 {
-    if (fast) k_decode<DT, FP8, DP, true><<<grid, kThreads, 0, s>>>(a);
-    else k_decode<DT, FP8, DP, false><<<grid, kThreads, 0, s>>>(a);
+    Layout l{};
+    const int group = sh.q_heads / c.kv_heads;
+    l.rows = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads);
+    l.part_heads = std::min(group, kHeads);
+    const int64_t tiles = (std::min<int64_t>(std::max<int64_t>(longest, 1), kLongest) + kTile - 1) / kTile;
+    l.blocks = (mfh_u32)dev->compute_units;
+    l.split = tiles > (l.rows >= dev->compute_units ? 32 : 16);
+    l.bytes = l.split ? (size_t)(l.blocks + l.rows) * l.part_heads * (c.head_dim + 2) * sizeof(float) : 0;
+    return l;
+}
+
+template <int DT, bool FP8, int DP, bool FAST>
+void launch_form(const Layout& l, hipStream_t s, const DecodeArgs& a)
+{
+    if (l.split) k_decode<DT, FP8, DP, FAST, true><<<(unsigned)(l.blocks + l.rows), kThreads, 0, s>>>(a);
+    else k_decode<DT, FP8, DP, FAST, false><<<(unsigned)l.rows, kThreads, 0, s>>>(a);
 }
 
 template <int DT, bool FP8>
-void launch_dims(int dim, bool fast, unsigned grid, hipStream_t s, const DecodeArgs& a)
+void launch_dims(bool fast, const Layout& l, hipStream_t s, const DecodeArgs& a)
 {
-    if (dim <= 64) launch_pages<DT, FP8, 64>(fast, grid, s, a);
-    else if (dim <= 128) launch_pages<DT, FP8, 128>(fast, grid, s, a);
-    else launch_pages<DT, FP8, 256>(fast, grid, s, a);
-}
-
-// Parts of a request and tiles of a part at least.  The parts fill the card
-// four workgroups deep; below 128 tokens (a tile a wave) a part is not worth
-// its workgroup.
-constexpr int kDeep = 4;
-constexpr mfh_u32 kLeast = kWaves;
-
-void split(const Device* dev, int64_t rows, int64_t longest, mfh_u32* parts, mfh_u32* least)
-{
-    const int64_t tiles = std::min<int64_t>((std::max<int64_t>(longest, 1) + kTile - 1) / kTile, kLongest / kTile);
-    const int64_t wanted = std::max<int64_t>(1, (int64_t)dev->compute_units * kDeep / std::max<int64_t>(rows, 1));
-    const int64_t most = std::max<int64_t>(1, (tiles + kLeast - 1) / kLeast);
-    const int64_t n = std::min(wanted, most);
-    const int64_t size = ((tiles + n - 1) / n + kWaves - 1) / kWaves * kWaves;
-    *least = (mfh_u32)size;
-    *parts = (mfh_u32)((tiles + size - 1) / size);
-}
-
-size_t part_bytes(int64_t rows, mfh_u32 parts, int dim)
-{
-    return parts > 1 ? (size_t)rows * parts * (dim + 2) * sizeof(float) : 0;
+    if (fast) {
+        if (a.dim <= 64) launch_form<DT, FP8, 64, true>(l, s, a);
+        else if (a.dim <= 128) launch_form<DT, FP8, 128, true>(l, s, a);
+        else launch_form<DT, FP8, 256, true>(l, s, a);
+    } else {
+        if (a.dim <= 64) launch_form<DT, FP8, 64, false>(l, s, a);
+        else if (a.dim <= 128) launch_form<DT, FP8, 128, false>(l, s, a);
+        else launch_form<DT, FP8, 256, false>(l, s, a);
+    }
 }
 
 }  // namespace
@@ -509,10 +644,7 @@ int mfh_paged_decode_workspace(const mfh_attention_shape* shape, const mfh_kv_ca
     MFH_TRY(check_attention(shape, cache, what));
     if (requests < 0) return fail(MFH_ERR_INVALID_ARGUMENT, "%s: negative number of requests %d", what, requests);
     if (!bytes) return fail(MFH_ERR_INVALID_ARGUMENT, "%s: NULL result", what);
-    const int group = shape->q_heads / cache->kv_heads;
-    mfh_u32 parts, least;
-    split(dev, (int64_t)requests * cache->kv_heads * ((group + kHeads - 1) / kHeads), longest, &parts, &least);
-    *bytes = part_bytes((int64_t)requests * shape->q_heads, parts, cache->head_dim);
+    *bytes = layout(dev, *shape, *cache, requests, longest).bytes;
     return MFH_OK;
 }
 
@@ -534,11 +666,8 @@ int mfh_paged_decode(const mfh_attention_shape* shape, const mfh_kv_cache* cache
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: NULL buffer", what);
     if (workspace_bytes > 0 && (!workspace || (uintptr_t)workspace % 16))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: the workspace is NULL or not 16-byte aligned", what);
-    const int bytes = cache->dtype == kF8E4M3 ? 1 : 2;
     DecodeArgs a{};
-    a.pages = PageArgs{(const char*)k_cache, (const char*)v_cache, table, table_stride, cache->page_stride * bytes,
-                       cache->token_stride * bytes, cache->head_stride * bytes, cache->pages,
-                       Divider((mfh_u32)cache->page_size), (mfh_u32)table_width};
+    a.pages = PageArgs(*cache, k_cache, v_cache, table, table_stride, table_width);
     a.q = (const char*)q, a.out = (char*)out, a.lse = lse;
     a.lengths = lengths, a.slopes = slopes;
     const Strides qs(shape->q_token_stride, shape->q_head_stride, shape->q_heads, cache->head_dim);
@@ -556,35 +685,40 @@ int mfh_paged_decode(const mfh_attention_shape* shape, const mfh_kv_cache* cache
     a.group = shape->q_heads / cache->kv_heads;
     a.head_groups = (a.group + kHeads - 1) / kHeads;
     a.dim = cache->head_dim;
-    const int64_t rows = (int64_t)requests * cache->kv_heads * a.head_groups;
-    split(dev, rows, std::min<int64_t>(longest, (int64_t)table_width * cache->page_size), &a.parts, &a.least);
-    const int64_t heads = (int64_t)requests * shape->q_heads;
-    while (a.parts > 1 && part_bytes(heads, a.parts, a.dim) > workspace_bytes) {
-        a.least *= 2;
-        a.parts = (a.parts + 1) / 2;
-    }
-    const int64_t grid = rows * a.parts;
-    if (grid >= (int64_t(1) << 32) / kThreads || heads >= 0x7fffffff)
+    a.request_rows = (mfh_u32)(a.kv_heads * a.head_groups);
+    Layout l = layout(dev, *shape, *cache, requests, longest);
+    // all tiles, and the join's grid, in fewer than 31 bits
+    const int64_t most = std::min<int64_t>((int64_t)table_width * cache->page_size, kLongest) / kTile + 1;
+    if (l.bytes > workspace_bytes || l.rows * most > kLongest || (int64_t)requests * shape->q_heads > (1 << 22))
+        l.split = false;
+    if (l.rows + l.blocks >= (int64_t(1) << 32) / kThreads)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %d heads are too many for one call", what, requests,
                     shape->q_heads);
-    if (a.parts > 1) {
+    a.blocks = l.blocks;
+    a.part_heads = l.part_heads;
+    if (l.split) {
         a.part_out = (float*)workspace;
-        a.part_sum = (float2*)(a.part_out + heads * a.parts * a.dim);
+        a.part_sum = (float2*)(a.part_out + (l.blocks + l.rows) * l.part_heads * a.dim);
     }
-    a.by_parts = Divider(a.parts), a.by_head_groups = Divider((mfh_u32)a.head_groups), a.by_kv_heads = Divider((mfh_u32)a.kv_heads);
+    a.by_head_groups = Divider((mfh_u32)a.head_groups), a.by_request_rows = Divider(a.request_rows);
+    a.by_blocks = Divider(l.blocks), a.by_q_heads = Divider((mfh_u32)a.q_heads);
     hipStream_t s = (hipStream_t)stream;
-    const bool fast = cache->page_size % 16 == 0, fp8 = cache->dtype == kF8E4M3;
+    // whole groups of 16 tokens, and dwords for buffer loads
+    const bool fast = cache->page_size % 16 == 0 &&
+                      ((uintptr_t)k_cache | (uintptr_t)v_cache | a.pages.page_bytes | a.pages.head_bytes | a.pages.token_bytes) % 4 == 0;
+    const bool fp8 = cache->dtype == kF8E4M3;
     if (shape->dtype == kBFloat16) {
-        if (fp8) launch_dims<kBFloat16, true>(a.dim, fast, (unsigned)grid, s, a);
-        else launch_dims<kBFloat16, false>(a.dim, fast, (unsigned)grid, s, a);
+        if (fp8) launch_dims<kBFloat16, true>(fast, l, s, a);
+        else launch_dims<kBFloat16, false>(fast, l, s, a);
     } else {
-        if (fp8) launch_dims<kFloat16, true>(a.dim, fast, (unsigned)grid, s, a);
-        else launch_dims<kFloat16, false>(a.dim, fast, (unsigned)grid, s, a);
+        if (fp8) launch_dims<kFloat16, true>(fast, l, s, a);
+        else launch_dims<kFloat16, false>(fast, l, s, a);
     }
     MFH_TRY(launch_status("k_decode"));
-    if (a.parts > 1) {
-        if (shape->dtype == kBFloat16) k_decode_join<kBFloat16><<<(unsigned)heads, 64, 0, s>>>(a);
-        else k_decode_join<kFloat16><<<(unsigned)heads, 64, 0, s>>>(a);
+    if (l.split) {
+        const unsigned grid = (unsigned)((int64_t)requests * shape->q_heads * ((a.dim + 127) / 128));
+        if (shape->dtype == kBFloat16) k_decode_join<kBFloat16><<<grid, 64 * kJoinWaves, 0, s>>>(a);
+        else k_decode_join<kFloat16><<<grid, 64 * kJoinWaves, 0, s>>>(a);
         MFH_TRY(launch_status("k_decode_join"));
     }
     return MFH_OK;

@@ -25,15 +25,21 @@ struct Strides {
     }
 };
 
-// n / d for 32-bit n and a d known at launch: the high half of n * ceil(2^64 / d),
-// exact because the rounding adds n * d * 2^-64 < 1 / d at most.
+// n / d for n below 2^31 and a d known at launch: n * ceil(2^(31 + s) / d) >>
+// (31 + s) with 2^s >= d, where the rounding adds n * d * 2^-(31 + s) < 1 to
+// the quotient's numerator.
 struct Divider {
-    mfh_u64 m;
-    mfh_u32 d;
+    mfh_u32 m, shift, d;
     Divider() = default;
-    explicit Divider(mfh_u32 by) : m(by > 1 ? ~mfh_u64(0) / by + 1 : 0), d(by) {}
-    __device__ mfh_u32 quotient(mfh_u32 n) const { return d == 1 ? n : (mfh_u32)__umul64hi(m, n); }
-    __device__ mfh_i64 quotient64(mfh_i64 n) const { return n >> 32 ? n / (mfh_i64)d : (mfh_i64)quotient((mfh_u32)n); }
+    explicit Divider(mfh_u32 by) : d(by)
+    {
+        mfh_u32 s = 0;
+        while (((mfh_u64)1 << s) < by) s++;
+        shift = 31 + s;
+        m = (mfh_u32)((((mfh_u64)1 << shift) + by - 1) / by);
+    }
+    __device__ mfh_u32 quotient(mfh_u32 n) const { return (mfh_u32)((mfh_u64)n * m >> shift); }
+    __device__ mfh_i64 quotient64(mfh_i64 n) const { return n >> 31 ? n / (mfh_i64)d : (mfh_i64)quotient((mfh_u32)n); }
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -116,18 +122,50 @@ struct PageArgs {
     const char* v;
     const int32_t* table;
     int64_t table_stride;
-    int64_t page_bytes, token_bytes, head_bytes;
-    int64_t pages;
-    Divider by_page;  // page size
+    int64_t page_bytes, head_bytes;
+    mfh_u32 token_bytes;  // 0 where a page holds one token
+    mfh_u32 pages;
+    mfh_u32 page_span;    // bytes of a page from its first element of a head to the last one
+    Divider by_page;      // page size
     mfh_u32 width;
+    PageArgs() = default;
+    PageArgs(const mfh_kv_cache& c, const void* keys, const void* values, const int32_t* block_table, int64_t stride,
+             int32_t table_width)
+        : k((const char*)keys), v((const char*)values), table(block_table), table_stride(stride)
+    {
+        const int bytes = c.dtype == kF8E4M3 ? 1 : 2;
+        page_bytes = c.page_stride * bytes, head_bytes = c.head_stride * bytes;
+        token_bytes = c.page_size > 1 ? (mfh_u32)(c.token_stride * bytes) : 0;
+        pages = (mfh_u32)c.pages;
+        page_span = (mfh_u32)(c.page_size - 1) * token_bytes + (mfh_u32)(c.head_dim * bytes);
+        by_page = Divider((mfh_u32)c.page_size);
+        width = (mfh_u32)table_width;
+    }
 };
 
-// The part of a split sequence that each workgroup takes: `tiles` tiles in
-// parts of at least `least` tiles, at most `parts` of them.
-MFH_DEV mfh_u32 part_tiles(mfh_u32 tiles, mfh_u32 least, mfh_u32 parts)
+MFH_DEV mfh_i64 shuffle64(mfh_i64 v, int lane)
 {
-    return max(least, (tiles + parts - 1) / parts);
+    const mfh_u32 lo = __shfl((int)(mfh_u32)v, lane), hi = __shfl((int)(v >> 32), lane);
+    return (mfh_i64)((mfh_u64)hi << 32 | lo);
 }
+
+// A value that is the same in every lane, as the compiler may know it.
+MFH_DEV mfh_u32 uniform(mfh_u32 v) { return (mfh_u32)__builtin_amdgcn_readfirstlane((int)v); }
+
+// Sum of the lanes up to and with this one, by moves between lanes of a row of
+// 16 and then from the rows before.
+MFH_DEV mfh_u32 lanes_upto(mfh_u32 v)
+{
+    v += (mfh_u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+    v += (mfh_u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (mfh_u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (mfh_u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (mfh_u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    v += (mfh_u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+MFH_DEV mfh_u32 last_lane(mfh_u32 v) { return (mfh_u32)__builtin_amdgcn_readlane((int)v, 63); }
 
 }  // namespace mfh
 

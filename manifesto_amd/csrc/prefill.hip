@@ -54,12 +54,6 @@ MFH_DEV u32x2 read_column(const char* at)
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at)));
 }
 
-MFH_DEV int64_t shuffle64(int64_t v, int lane)
-{
-    const mfh_u32 lo = __shfl((int)(mfh_u32)v, lane), hi = __shfl((int)(v >> 32), lane);
-    return (int64_t)((mfh_u64)hi << 32 | lo);
-}
-
 // Whether a dword's halves are infinite or NaN.
 template <int DT>
 MFH_DEV bool not_finite(mfh_u32 pair)
@@ -175,7 +169,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
         const mfh_u32 t = (mfh_u32)(tile * kKeys + lane);
         const mfh_u32 in_table = a.pages.by_page.quotient(t), in_page = t - in_table * a.pages.by_page.d;
         const int32_t page = (int)t < length ? table[in_table] : -1;
-        const bool ok = page >= 0 && page < a.pages.pages;
+        const bool ok = (mfh_u32)page < a.pages.pages;
         at = ok ? page * a.pages.page_bytes + in_page * a.pages.token_bytes : 0;
         valid = __ballot(ok);
     };
@@ -420,11 +414,8 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: NULL buffer", what);
     if (workspace_bytes > 0 && (!workspace || (uintptr_t)workspace % 16))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: the workspace is NULL or not 16-byte aligned", what);
-    const int bytes = cache->dtype == kF8E4M3 ? 1 : 2;
     PrefillArgs a{};
-    a.pages = PageArgs{(const char*)k_cache, (const char*)v_cache, table, table_stride, cache->page_stride * bytes,
-                       cache->token_stride * bytes, cache->head_stride * bytes, cache->pages,
-                       Divider((mfh_u32)cache->page_size), (mfh_u32)table_width};
+    a.pages = PageArgs(*cache, k_cache, v_cache, table, table_stride, table_width);
     a.q = (const char*)q, a.out = (char*)out, a.lse = lse;
     a.starts = starts, a.lengths = lengths, a.prefix = prefix, a.slopes = slopes;
     const Strides qs(shape->q_token_stride, shape->q_head_stride, shape->q_heads, cache->head_dim);
