@@ -24,7 +24,6 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kRows = 32 * kWaves;  // of a workgroup
-constexpr int kKeys = 64;           // of a tile
 constexpr float kStep = 8.0f;       // the reference moves where a score passes it by 2^kStep
 
 struct PrefillArgs {
@@ -59,31 +58,17 @@ template <int DT>
 MFH_DEV bool not_finite(mfh_u32 pair)
 {
     constexpr mfh_u32 kExp = DT == kBFloat16 ? 0x7f80u : 0x7c00u;
-    return (pair & kExp) == kExp || (pair & kExp << 16) == kExp << 16;
+    return ((pair & kExp) == kExp) | ((pair & kExp << 16) == kExp << 16);
 }
 
-// Splits eight values into their finite part and a count of what is not:
-// 1 for inf, 128 for -inf, 16384 for NaN.  A tile's 64 keys leave the counts
-// apart, and they are exact in 16 bits and as f32 sums.
-template <int DT>
-MFH_DEV void split_values(u32x4 v, u32x4* finite, u32x4* count)
+// Where 16 bytes of a row stand among the row's pieces in LDS.  Rows have no
+// gaps (a load into LDS writes 64 lanes' pieces one after the other), so pieces
+// change places by row: 16 rows of one piece, as K is read, lie in 16 different
+// places, and four rows of four pieces, as V is, too.
+template <int PIECES>
+MFH_DEV int place(int row, int piece)
 {
-    constexpr mfh_u32 kExp = DT == kBFloat16 ? 0x7f80u : 0x7c00u;
-    constexpr mfh_u32 kMan = DT == kBFloat16 ? 0x007fu : 0x03ffu;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        mfh_u32 f = v[w];
-        float c[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const mfh_u32 x = v[w] >> (16 * h) & 0xffffu;
-            const bool out = (x & kExp) == kExp;
-            c[h] = !out ? 0.0f : x & kMan ? 16384.0f : x >> 15 ? 128.0f : 1.0f;
-            if (out) f &= 0xffff0000u >> (16 * h);
-        }
-        (*finite)[w] = f;
-        (*count)[w] = enc16x2<DT>(c[0], c[1]);
-    }
+    return piece ^ (((row & 3) << 2 | (row >> 2 & 3)) & (PIECES - 1));
 }
 
 // DP: head_dim rounded up to 64, 128 or 256.
@@ -93,14 +78,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
     constexpr int kBytes = FP8 ? 1 : 2;
     constexpr int kSteps = DP / 16;
     constexpr int kDimTiles = DP / 32;
-    // Pitches that put a read's rows into different banks: 16 bytes apart for
-    // K's 16-byte pieces, 64 for V's four rows of 64 bytes.
-    constexpr int kPitchK = 2 * DP + 16, kPitchV = 2 * DP + 64;
-    constexpr int kPieces = DP / 8;                       // of a key, eight values each
-    constexpr int kLoads = kKeys * kPieces / kThreads;    // of a thread
-    constexpr int kKeyStep = kThreads / kPieces;          // keys between a thread's pieces
-    __shared__ __align__(16) char s_k[kKeys * kPitchK];
-    __shared__ __align__(16) char s_v[kKeys * kPitchV];
+    constexpr int kKeys = DP <= 128 ? 64 : 32;           // of a tile
+    constexpr int kBlocks = kKeys / 32;
+    constexpr int kPitch = 2 * DP;
+    constexpr int kPieces = DP / 8;                      // of a key, eight values each
+    constexpr int kLoads = kKeys * kPieces / kThreads;   // of a thread
+    constexpr int kKeyStep = kThreads / kPieces;         // keys between a thread's pieces
+    __shared__ __align__(16) char s_tiles[2][2][kKeys * kPitch];  // K and V of two tiles
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
@@ -159,191 +143,266 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
         for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
     float ref = 0.0f, limit = -INFINITY, sum = 0.0f;
 
-    // Staging: lane l looks up key l of a tile; thread t takes piece t % kPieces
-    // of keys t / kPieces + i * kKeyStep.
-    const int piece = threadIdx.x % kPieces, key0 = threadIdx.x / kPieces;
-    const bool in_dim = piece * 8 < a.dim;
+    // Staging: lane l looks up key l of a tile; thread t takes the piece that
+    // belongs in place t % kPieces of keys t / kPieces + i * kKeyStep.
+    const int key0 = threadIdx.x / kPieces, slot = threadIdx.x % kPieces;
     int64_t at = 0;
-    mfh_u64 valid = 0;
+    mfh_u64 valid = 0;  // bit i: key i has a page
     auto locate = [&](int tile) {
-        const mfh_u32 t = (mfh_u32)(tile * kKeys + lane);
+        const mfh_u32 t = (mfh_u32)(tile * kKeys + (lane & (kKeys - 1)));
         const mfh_u32 in_table = a.pages.by_page.quotient(t), in_page = t - in_table * a.pages.by_page.d;
         const int32_t page = (int)t < length ? table[in_table] : -1;
         const bool ok = (mfh_u32)page < a.pages.pages;
-        at = ok ? page * a.pages.page_bytes + in_page * a.pages.token_bytes : 0;
-        valid = __ballot(ok);
+        at = ok ? (mfh_u32)page * a.pages.page_bytes + in_page * a.pages.token_bytes : 0;
+        valid = __ballot(ok) << (64 - kKeys);
     };
-    u32x4 k_next[kLoads], v_next[kLoads];
+    constexpr mfh_u64 kAll = ~mfh_u64(0) << (64 - kKeys);
+    auto is_valid = [&](mfh_u64 mask, int key) { return (mask >> (64 - kKeys + key) & 1) != 0; };
+    // whether every row of the workgroup sees every key
+    auto is_open = [&](int tile, mfh_u64 mask) {
+        const int key = tile * kKeys;
+        return mask == kAll && ((key + kKeys <= low_position + 1 && (a.window <= 0 || key > high_position - a.window)) || key + kKeys <= prefix);
+    };
+    auto piece_at = [&](int i, bool* in_dim) {  // of this thread's i-th piece
+        const int key = key0 + i * kKeyStep, piece = place<kPieces>(key, slot);
+        *in_dim = piece * 8 < a.dim;
+        return shuffle64(at, key) + (*in_dim ? piece * 8 * kBytes : 0);
+    };
+    // Eight-bit pieces wait in registers while the tile before is computed, and
+    // are widened on the way to LDS; so are those of tiles that a mask cuts.
+    u32x2 k_codes[kLoads], v_codes[kLoads];
     auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            const int key = key0 + i * kKeyStep;
-            const int64_t from = shuffle64(at, key) + (in_dim ? piece * 8 * kBytes : 0);
-            if constexpr (FP8) {
-                const u32x2 kw = load8<false>(k_base + from), vw = load8<false>(v_base + from);
-                k_next[i] = u32x4{kw[0], kw[1], 0, 0};
-                v_next[i] = u32x4{vw[0], vw[1], 0, 0};
-            } else {
-                k_next[i] = load16<false>(k_base + from);
-                v_next[i] = load16<false>(v_base + from);
-            }
+            bool in_dim;
+            const int64_t from = piece_at(i, &in_dim);
+            k_codes[i] = load8<false>(k_base + from);
+            v_codes[i] = load8<false>(v_base + from);
         }
     };
-    auto widen = [&](u32x4 w) {
-        if constexpr (!FP8) return w;
-        else return u32x4{e4m3_pair<DT, false>(w[0]), e4m3_pair<DT, true>(w[0]), e4m3_pair<DT, false>(w[1]), e4m3_pair<DT, true>(w[1])};
+    // True if a mask cuts the tile and this thread's part has values that are not finite.
+    auto put = [&](char* s_k, char* s_v, mfh_u64 mask, bool open, int i, u32x4 kw, u32x4 vw, bool in_dim) {
+        const int key = key0 + i * kKeyStep;
+        const u32x4 zero = {0, 0, 0, 0};
+        const bool keep = in_dim & is_valid(mask, key);
+        kw = keep ? kw : zero, vw = keep ? vw : zero;
+        *reinterpret_cast<u32x4*>(s_k + key * kPitch + slot * 16) = kw;
+        *reinterpret_cast<u32x4*>(s_v + key * kPitch + slot * 16) = vw;
+        return !open & (not_finite<DT>(vw[0]) | not_finite<DT>(vw[1]) | not_finite<DT>(vw[2]) | not_finite<DT>(vw[3]));
     };
-
-    int tile = next_tile(0);
-    if (tile < tile_end) {
-        locate(tile);
-        fetch();
-    }
-    while (tile < tile_end) {
-        const mfh_u64 tile_valid = valid;
-        const int key_first = tile * kKeys;
-        // whether every row of the workgroup sees every key
-        const bool open = tile_valid == ~mfh_u64(0) &&
-                          ((key_first + kKeys <= low_position + 1 && (a.window <= 0 || key_first > high_position - a.window)) ||
-                           key_first + kKeys <= prefix);
+    auto put_codes = [&](char* s_k, char* s_v, mfh_u64 mask, bool open) {
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
             const int key = key0 + i * kKeyStep;
-            const bool keep = in_dim && (tile_valid >> key & 1);
-            const u32x4 zero = {0, 0, 0, 0};
-            const u32x4 kw = keep ? widen(k_next[i]) : zero, vw = keep ? widen(v_next[i]) : zero;
-            *reinterpret_cast<u32x4*>(s_k + key * kPitchK + piece * 16) = kw;
-            *reinterpret_cast<u32x4*>(s_v + key * kPitchV + piece * 16) = vw;
-            if (!open)
-                odd |= not_finite<DT>(vw[0]) || not_finite<DT>(vw[1]) || not_finite<DT>(vw[2]) || not_finite<DT>(vw[3]);
+            const u32x2 k = k_codes[i], v = v_codes[i];
+            odd |= put(s_k, s_v, mask, open, i,
+                       u32x4{e4m3_pair<DT, false>(k[0]), e4m3_pair<DT, true>(k[0]), e4m3_pair<DT, false>(k[1]), e4m3_pair<DT, true>(k[1])},
+                       u32x4{e4m3_pair<DT, false>(v[0]), e4m3_pair<DT, true>(v[0]), e4m3_pair<DT, false>(v[1]), e4m3_pair<DT, true>(v[1])},
+                       place<kPieces>(key, slot) * 8 < a.dim);
         }
-        const int following = next_tile(tile + 1);
-        if (following < tile_end) {
-            locate(following);
-            fetch();
+        return odd;
+    };
+    // 16-bit pieces of a tile that is whole go to LDS directly.
+    auto stage = [&](char* s_k, char* s_v, mfh_u64 mask, bool open) {
+        bool odd = false;
+        if (open && a.dim == DP) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                bool in_dim;
+                const int64_t from = piece_at(i, &in_dim);
+                const int to = (i * kThreads + wave * 64) * 16;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(k_base + from),
+                                                 (__attribute__((address_space(3))) void*)(s_k + to), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(v_base + from),
+                                                 (__attribute__((address_space(3))) void*)(s_v + to), 16, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                bool in_dim;
+                const int64_t from = piece_at(i, &in_dim);
+                const u32x4 k = load16<false>(k_base + from), v = load16<false>(v_base + from);
+                odd |= put(s_k, s_v, mask, open, i, k, v, in_dim);
+            }
         }
-        // A masked weight of 0 times a value that is not finite would be NaN:
-        // such a tile, if a mask cuts it, takes the long way.
-        const bool any_odd = open ? (__syncthreads(), false) : __syncthreads_or(odd) != 0;
+        return odd;
+    };
 
+    // Score i of block b is of key 32 b + 4 half + 8 (i / 4) + i % 4; whether this lane's row sees it:
+    struct Seen {
+        mfh_u32 there;
+        int back, oldest, in_prefix;
+        __device__ bool operator()(int c) const  // (no short cuts: branches cost more than the comparisons)
+        {
+            return ((there >> c & 1) != 0) & (((c <= back) & (c > oldest)) | (c < in_prefix));
+        }
+    };
+    auto seen_from = [&](int key, mfh_u32 there) {
+        return Seen{there, position - key, a.window > 0 ? position - key - a.window : -kKeys, prefix - key};
+    };
+
+    // A masked weight of 0 times a value that is not finite would be NaN.  Where
+    // a mask cuts a tile that has such values, they are added to the rows that
+    // see them, and are zeros in the product.
+    auto add_odd = [&](const char* s_v, int tile, mfh_u64 mask) {
+        const Seen seen = seen_from(tile * kKeys, 0);
+        for (int key = 0; key < kKeys; key++) {
+            const bool see = is_valid(mask, key) & (((key <= seen.back) & (key > seen.oldest)) | (key < seen.in_prefix));
+#pragma unroll
+            for (int d = 0; d < kDimTiles; d++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int dim = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
+                    const mfh_u32 v = *reinterpret_cast<const mfh_u16*>(s_v + key * kPitch + place<kPieces>(key, dim / 8) * 16 + dim % 8 * 2);
+                    if (see & not_finite<DT>(v)) acc[d][i] += dec16<DT>(v);
+                }
+            }
+        }
+    };
+    auto clear_odd = [&](char* s_v) {
+        for (int i = 0; i < kLoads; i++) {
+            u32x4& w = *reinterpret_cast<u32x4*>(s_v + (key0 + i * kKeyStep) * kPitch + slot * 16);
+            u32x4 v = w;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] &= (not_finite<DT>(v[j] & 0xffffu) ? 0u : 0xffffu) | (not_finite<DT>(v[j] >> 16) ? 0u : 0xffff0000u);
+            w = v;
+        }
+    };
+
+    auto compute = [&](const char* s_k, const char* s_v, int tile, mfh_u64 mask) {
+        const int key_first = tile * kKeys;
         // Rows of this wave that see something here, and whether all of it.
         const bool some = key_first < max(wave_high + 1, prefix) &&
                           (a.window <= 0 || key_first < prefix || key_first + kKeys > wave_low - a.window + 1);
-        if (some) {
-            f32x16 s[2];
+        if (!some) return;
+        f32x16 s[kBlocks];
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < kBlocks; b++) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
+            for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
 #pragma unroll
-                for (int d = 0; d < kSteps; d++) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(s_k + (32 * b + col) * kPitchK + (16 * d + 8 * half) * 2);
-                    s[b] = mfma32<DT>(kf, q[d], s[b]);
-                }
+            for (int d = 0; d < kSteps; d++) {
+                const int key = 32 * b + col;
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(s_k + key * kPitch + place<kPieces>(key, 2 * d + half) * 16);
+                s[b] = mfma32<DT>(kf, q[d], s[b]);
             }
-            const bool all = tile_valid == ~mfh_u64(0) &&
-                             ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
-                              key_first + kKeys <= prefix);
-            mfh_u32 seen[2] = {0xffffu, 0xffffu};  // bit i: score i
-            float top = -INFINITY;
+        }
+        const bool all = mask == kAll && ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
+                                          key_first + kKeys <= prefix);
+        float scale = a.scale;  // what is left to multiply by
+        if (a.cap_scaled != 0.0f || a.slopes || !all || !(scale > 0.0f)) {
+            scale = 1.0f;
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < kBlocks; b++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[b][i] *= a.scale;
                 if (a.cap_scaled != 0.0f) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) s[b][i] = capped(s[b][i], a.cap_twice, a.cap_scaled);
                 }
-                const int key_b = key_first + 32 * b + 4 * half;
+                const Seen seen = seen_from(key_first + 32 * b + 4 * half, (mfh_u32)(mask >> (64 - kKeys + 32 * b)) >> (4 * half));
                 if (a.slopes) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        s[b][i] -= slope * fabsf((float)(position - (key_b + 8 * (i / 4) + i % 4)));
+                    for (int i = 0; i < 16; i++) s[b][i] -= slope * fabsf((float)(seen.back - (8 * (i / 4) + i % 4)));
                 }
                 if (!all) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int in_tile = 32 * b + 4 * half + 8 * (i / 4) + i % 4, key = key_first + in_tile;
-                        const bool see = (tile_valid >> in_tile & 1) &&
-                                         ((key <= position && (a.window <= 0 || key > position - a.window)) || key < prefix);
-                        if (!see) {
-                            s[b][i] = -INFINITY;
-                            seen[b] &= ~(1u << i);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) top = fmaxf(top, s[b][i]);
-            }
-            if (__any(top > limit)) {
-                top = fmaxf(top, __shfl_xor(top, 32));
-                if (top > limit) {
-                    const float alpha = limit == -INFINITY ? 0.0f : exp2_fast(ref - top);
-                    ref = top;
-                    limit = top + kStep;
-                    sum *= alpha;
-#pragma unroll
-                    for (int d = 0; d < kDimTiles; d++) acc[d] *= alpha;
-                }
-            }
-            u32x4 p[4];
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                float part = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    s[b][i] = exp2_fast(s[b][i] - ref);
-                    part += s[b][i];
-                }
-                sum += part;
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) p[2 * b + i / 8][i / 2 % 4] = enc16x2<DT>(s[b][i], s[b][i + 1]);
-            }
-            // V^T: in 16 lanes row lane % 16 / 4 of four keys, columns 4 (lane % 4) ..
-            const char* v_at = s_v + (4 * half + (lane & 15) / 4) * kPitchV + (16 * (lane >> 4 & 1) + 4 * (lane & 3)) * 2;
-            if (!any_odd) {
-#pragma unroll
-                for (int d = 0; d < kDimTiles; d++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const u32x2 lo = read_column(v_at + 16 * j * kPitchV + 64 * d);
-                        const u32x2 hi = read_column(v_at + (16 * j + 8) * kPitchV + 64 * d);
-                        acc[d] = mfma32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[j], acc[d]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int d = 0; d < kDimTiles; d++) {
-                    f32x16 count;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) count[i] = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const u32x2 lo = read_column(v_at + 16 * j * kPitchV + 64 * d);
-                        const u32x2 hi = read_column(v_at + (16 * j + 8) * kPitchV + 64 * d);
-                        u32x4 finite, code, sees;
-                        split_values<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, &finite, &code);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const mfh_u32 bits = seen[j >> 1] >> (8 * (j & 1) + 2 * i);
-                            sees[i] = enc16x2<DT>(bits & 1 ? 1.0f : 0.0f, bits & 2 ? 1.0f : 0.0f);
-                        }
-                        acc[d] = mfma32<DT>(finite, p[j], acc[d]);
-                        count = mfma32<DT>(code, sees, count);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const mfh_u32 n = (mfh_u32)count[i];
-                        if (n >> 14) acc[d][i] = NAN;
-                        if (n & 127) acc[d][i] += INFINITY;
-                        if (n >> 7 & 127) acc[d][i] -= INFINITY;
-                    }
+                    for (int i = 0; i < 16; i++) s[b][i] = seen(8 * (i / 4) + i % 4) ? s[b][i] : -INFINITY;
                 }
             }
         }
-        __syncthreads();
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[b][i]);
+        top *= scale;
+        if (__any(top > limit)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (top > limit) {
+                // (at first there is nothing to scale but what add_odd put there)
+                const float alpha = limit == -INFINITY ? 1.0f : exp2_fast(ref - top);
+                ref = top;
+                limit = top + kStep;
+                sum *= alpha;
+#pragma unroll
+                for (int d = 0; d < kDimTiles; d++) acc[d] *= alpha;
+            }
+        }
+        u32x4 p[2 * kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[b][i] = exp2_fast(__builtin_fmaf(s[b][i], scale, -ref));
+                part += s[b][i];
+            }
+            sum += part;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) p[2 * b + i / 8][i / 2 % 4] = enc16x2<DT>(s[b][i], s[b][i + 1]);
+        }
+        // V^T: in 16 lanes row lane % 16 / 4 of four keys, columns 4 (lane % 4) ..
+        auto column = [&](int key, int d) {
+            const int at_key = key + 4 * half + (lane & 15) / 4, piece = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
+            return read_column(s_v + at_key * kPitch + place<kPieces>(at_key, piece) * 16 + 8 * (lane & 1));
+        };
+#pragma unroll
+        for (int d = 0; d < kDimTiles; d++) {
+#pragma unroll
+            for (int j = 0; j < 2 * kBlocks; j++) {
+                const u32x2 lo = column(16 * j, d), hi = column(16 * j + 8, d);
+                acc[d] = mfma32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[j], acc[d]);
+            }
+        }
+    };
+
+    // One tile is computed while the next one is on its way to the other half
+    // of LDS.
+    int tile = next_tile(0), now = 0;
+    mfh_u64 mask = 0;
+    bool odd = false, open = true;
+    auto meet = [&]() {  // all of the staged tile is in LDS
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): loads into LDS are no one's registers
+        odd = open ? (__syncthreads(), false) : __syncthreads_or(odd) != 0;
+    };
+    if (tile < tile_end) {
+        locate(tile);
+        mask = valid, open = is_open(tile, mask);
+        if constexpr (FP8) {
+            fetch();
+            odd = put_codes(s_tiles[0][0], s_tiles[0][1], mask, open);
+        } else {
+            odd = stage(s_tiles[0][0], s_tiles[0][1], mask, open);
+        }
+        meet();
+    }
+    while (tile < tile_end) {
+        const char* s_k = s_tiles[now][0];
+        char* s_v = s_tiles[now][1];
+        const int following = next_tile(tile + 1);
+        const mfh_u64 mask_now = mask;
+        if (odd) {
+            add_odd(s_v, tile, mask);
+            __syncthreads();
+            clear_odd(s_v);
+            __syncthreads();
+            odd = false;
+        }
+        if (following < tile_end) {
+            locate(following);
+            mask = valid, open = is_open(following, mask);
+            if constexpr (FP8) fetch();
+            else odd = stage(s_tiles[now ^ 1][0], s_tiles[now ^ 1][1], mask, open);
+        }
+        compute(s_k, s_v, tile, mask_now);
         tile = following;
+        if (following < tile_end) {
+            if constexpr (FP8) odd = put_codes(s_tiles[now ^ 1][0], s_tiles[now ^ 1][1], mask, open);
+            meet();
+        }
+        now ^= 1;
     }
 
     sum += __shfl_xor(sum, 32);
