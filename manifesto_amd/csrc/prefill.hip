@@ -21,9 +21,9 @@
 namespace mfh {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;  // of a workgroup
+// Waves of a workgroup, 32 rows each: two a SIMD where their registers allow it.
+constexpr int waves_of(int dim) { return dim <= 128 ? 8 : 4; }
+constexpr int keys_of(int dim) { return dim <= 128 ? 64 : 32; }  // of a tile
 constexpr float kStep = 8.0f;       // the reference moves where a score passes it by 2^kStep
 
 struct PrefillArgs {
@@ -38,9 +38,13 @@ struct PrefillArgs {
     int64_t q_t, q_h, out_t, out_h;  // elements
     int64_t tokens, most_fresh;
     float scale, cap_twice, cap_scaled, v_scale;
+    float* part_out;   // [tokens * q_heads][parts][head_dim]
+    float2* part_sum;  // [tokens * q_heads][parts]: reference and sum
     int32_t window, kv_heads, q_heads, group, dim;
     mfh_u32 row_tiles;  // of a request and head at most
-    Divider by_group, by_kv_heads, by_row_tiles;
+    mfh_u32 parts;      // of a row's keys
+    mfh_u32 step_entries, step_bytes;  // a tile's keys in whole pages, and in bytes of a page
+    Divider by_group, by_kv_heads, by_row_tiles, by_parts;
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -73,23 +77,32 @@ MFH_DEV int place(int row, int piece)
 
 // DP: head_dim rounded up to 64, 128 or 256.
 template <int DT, bool FP8, int DP>
-__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(PrefillArgs a)
+__global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefill(PrefillArgs a)
 {
+    constexpr int kWaves = waves_of(DP), kThreads = 64 * kWaves, kRows = 32 * kWaves;
     constexpr int kBytes = FP8 ? 1 : 2;
     constexpr int kSteps = DP / 16;
     constexpr int kDimTiles = DP / 32;
-    constexpr int kKeys = DP <= 128 ? 64 : 32;           // of a tile
+    constexpr int kKeys = keys_of(DP);
     constexpr int kBlocks = kKeys / 32;
     constexpr int kPitch = 2 * DP;
     constexpr int kPieces = DP / 8;                      // of a key, eight values each
     constexpr int kLoads = kKeys * kPieces / kThreads;   // of a thread
     constexpr int kKeyStep = kThreads / kPieces;         // keys between a thread's pieces
-    __shared__ __align__(16) char s_tiles[2][2][kKeys * kPitch];  // K and V of two tiles
+    typedef typename std::conditional<FP8, u32x2, u32x4>::type Raw;
+    __shared__ __align__(16) char s_k[3][kKeys * kPitch], s_v[3][kKeys * kPitch];
+    __shared__ __align__(16) char s_raw[3][kKeys * kPitch];  // V as it was, where some of it is not finite
+    __shared__ int s_odd[3];                                 // the round whose V that is
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
-    mfh_u32 rest = a.by_kv_heads.quotient(blockIdx.x);
-    const mfh_u32 kv = blockIdx.x - rest * a.kv_heads;
+    const int group = wave / 4;  // of waves that multiply while the other one does the rest
+    mfh_u32 at_block = blockIdx.x;
+    mfh_u32 rest = a.by_parts.quotient(at_block);
+    const mfh_u32 part = at_block - rest * a.parts;
+    at_block = rest;
+    rest = a.by_kv_heads.quotient(at_block);
+    const mfh_u32 kv = at_block - rest * a.kv_heads;
     const mfh_u32 r = a.by_row_tiles.quotient(rest);
     const mfh_u32 row_tile = a.row_tiles - 1 - (rest - r * a.row_tiles);  // the longest rows first
 
@@ -111,18 +124,22 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
     const int high_position = first_position + (int)a.by_group.quotient(min(row0 + kRows, rows) - 1);
     const int key_end = min(max(high_position + 1, prefix), length);
     const int window_first = a.window > 0 ? max(low_position - a.window + 1, 0) : 0;  // below: the prefix only
-    const int tile_end = key_end > 0 ? (key_end + kKeys - 1) / kKeys : 0;
     // The next tile at or after `tile` that has a key for some row: between the
     // prefix and the window there is none.
     auto next_tile = [&](int tile) {
         return tile * kKeys >= prefix ? max(tile, window_first / kKeys) : tile;
     };
+    // this part's tiles
+    const int all_tiles = key_end > 0 ? (key_end + kKeys - 1) / kKeys : 0, first_tile = min(next_tile(0), all_tiles);
+    const int share = (int)a.by_parts.quotient((mfh_u32)(all_tiles - first_tile) + a.parts - 1);
+    const int tile_end = min(first_tile + (int)(part + 1) * share, all_tiles);
 
     // This lane's row, and its wave's.
     const mfh_u32 row = row0 + 32 * wave + col;
     const bool real = row < rows;
     const mfh_u32 token = a.by_group.quotient(min(row, rows - 1)), head = kv * a.group + (min(row, rows - 1) - token * a.group);
     const int position = first_position + (int)token;
+    const bool wave_real = row0 + 32 * wave < rows;
     const mfh_u32 wave_row0 = min(row0 + 32 * wave, rows - 1), wave_row1 = min(row0 + 32 * wave + 31, rows - 1);
     const int wave_low = first_position + (int)a.by_group.quotient(wave_row0);
     const int wave_high = first_position + (int)a.by_group.quotient(wave_row1);
@@ -134,7 +151,12 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
         q[s] = u32x4{0, 0, 0, 0};
         if (real && d < a.dim) q[s] = load16<false>(a.q + ((begin + token) * a.q_t + head * a.q_h + d) * 2);
     }
-    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    // Q is waited for here: in the loop the compiler would wait for all loads
+    // on its account, those into LDS among them.
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) asm volatile("" : "+v"(q[s]));
+    asm volatile("" : "+v"(slope));
 
     f32x16 acc[kDimTiles];
 #pragma unroll
@@ -143,92 +165,107 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
         for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
     float ref = 0.0f, limit = -INFINITY, sum = 0.0f;
 
-    // Staging: lane l looks up key l of a tile; thread t takes the piece that
-    // belongs in place t % kPieces of keys t / kPieces + i * kKeyStep.
+    // ---- staging: thread t takes the piece that belongs in place t % kPieces of
+    // keys t / kPieces + i * kKeyStep, and follows these keys from tile to tile:
+    // their places in the table and, in bytes, in their pages.
     const int key0 = threadIdx.x / kPieces, slot = threadIdx.x % kPieces;
-    int64_t at = 0;
-    mfh_u64 valid = 0;  // bit i: key i has a page
-    auto locate = [&](int tile) {
-        const mfh_u32 t = (mfh_u32)(tile * kKeys + (lane & (kKeys - 1)));
-        const mfh_u32 in_table = a.pages.by_page.quotient(t), in_page = t - in_table * a.pages.by_page.d;
-        const int32_t page = (int)t < length ? table[in_table] : -1;
-        const bool ok = (mfh_u32)page < a.pages.pages;
-        at = ok ? (mfh_u32)page * a.pages.page_bytes + in_page * a.pages.token_bytes : 0;
-        valid = __ballot(ok) << (64 - kKeys);
+    struct Tile {
+        int index;
+        bool open;   // every row of the workgroup sees every key
     };
-    constexpr mfh_u64 kAll = ~mfh_u64(0) << (64 - kKeys);
-    auto is_valid = [&](mfh_u64 mask, int key) { return (mask >> (64 - kKeys + key) & 1) != 0; };
-    // whether every row of the workgroup sees every key
-    auto is_open = [&](int tile, mfh_u64 mask) {
-        const int key = tile * kKeys;
-        return mask == kAll && ((key + kKeys <= low_position + 1 && (a.window <= 0 || key > high_position - a.window)) || key + kKeys <= prefix);
+    struct Keys {
+        mfh_u32 entry[kLoads], in_page[kLoads];
+        int32_t page[kLoads];
     };
-    auto piece_at = [&](int i, bool* in_dim) {  // of this thread's i-th piece
-        const int key = key0 + i * kKeyStep, piece = place<kPieces>(key, slot);
-        *in_dim = piece * 8 < a.dim;
-        return shuffle64(at, key) + (*in_dim ? piece * 8 * kBytes : 0);
+    const mfh_u32 last_entry = length > 0 ? a.pages.by_page.quotient((mfh_u32)length - 1) : 0;
+    const mfh_u32 page_size_bytes = a.pages.by_page.d * a.pages.token_bytes;
+    auto ask = [&](Keys& keys) {  // past the length its last page again
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) keys.page[i] = table[min(keys.entry[i], last_entry)];
     };
-    // Eight-bit pieces wait in registers while the tile before is computed, and
-    // are widened on the way to LDS; so are those of tiles that a mask cuts.
-    u32x2 k_codes[kLoads], v_codes[kLoads];
-    auto fetch = [&]() {
+    auto go_to = [&](Keys& keys, int tile) {
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            bool in_dim;
-            const int64_t from = piece_at(i, &in_dim);
-            k_codes[i] = load8<false>(k_base + from);
-            v_codes[i] = load8<false>(v_base + from);
+            const mfh_u32 t = (mfh_u32)(tile * kKeys) + key0 + i * kKeyStep;
+            keys.entry[i] = a.pages.by_page.quotient(t);
+            keys.in_page[i] = (t - keys.entry[i] * a.pages.by_page.d) * a.pages.token_bytes;
         }
     };
-    // True if a mask cuts the tile and this thread's part has values that are not finite.
-    auto put = [&](char* s_k, char* s_v, mfh_u64 mask, bool open, int i, u32x4 kw, u32x4 vw, bool in_dim) {
-        const int key = key0 + i * kKeyStep;
-        const u32x4 zero = {0, 0, 0, 0};
-        const bool keep = in_dim & is_valid(mask, key);
-        kw = keep ? kw : zero, vw = keep ? vw : zero;
-        *reinterpret_cast<u32x4*>(s_k + key * kPitch + slot * 16) = kw;
-        *reinterpret_cast<u32x4*>(s_v + key * kPitch + slot * 16) = vw;
-        return !open & (not_finite<DT>(vw[0]) | not_finite<DT>(vw[1]) | not_finite<DT>(vw[2]) | not_finite<DT>(vw[3]));
+    auto go_on = [&](Keys& keys) {  // by a tile
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const mfh_u32 in_page = keys.in_page[i] + a.step_bytes;
+            // (a page of one token has no bytes to go on by)
+            const bool over = a.pages.token_bytes > 0 && in_page >= page_size_bytes;
+            keys.in_page[i] = over ? in_page - page_size_bytes : in_page;
+            keys.entry[i] += a.step_entries + (over ? 1 : 0);
+        }
     };
-    auto put_codes = [&](char* s_k, char* s_v, mfh_u64 mask, bool open) {
+    // Whether a page of the request is not one of the cache's: its keys are
+    // masked then, and nothing takes the short ways.
+    bool bad = false;
+    for (mfh_u32 i = threadIdx.x; length > 0 && i <= last_entry; i += kThreads) bad |= (mfh_u32)table[i] >= a.pages.pages;
+    const bool clean = !__syncthreads_or(bad);
+    auto there = [&](int key) {
+        bool is = key < length;
+        if (!clean) is &= (mfh_u32)table[min(a.pages.by_page.quotient((mfh_u32)key), last_entry)] < a.pages.pages;
+        return is;
+    };
+    auto describe = [&](int tile) {
+        const int first = tile * kKeys;
+        return Tile{tile, clean && first + kKeys <= length && ((first + kKeys <= low_position + 1 && (a.window <= 0 || first > high_position - a.window)) ||
+                                                      first + kKeys <= prefix)};
+    };
+    // This thread's pieces of the tile.
+    auto locate = [&](const Keys& keys, int64_t (&from)[kLoads]) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const mfh_u32 page = (mfh_u32)keys.page[i] < a.pages.pages ? (mfh_u32)keys.page[i] : 0u;
+            const int piece = place<kPieces>(key0 + i * kKeyStep, slot);
+            from[i] = (int64_t)((mfh_u64)page * (mfh_u64)a.pages.page_bytes) + (keys.in_page[i] + (piece * 8 < a.dim ? piece * 8 * kBytes : 0));
+        }
+    };
+
+    // Pieces wait in registers while the vector units are busy with the scores,
+    // and go to LDS from there, 8-bit ones widened on the way.  (Loads straight
+    // into LDS took longer: a wave stands still for 200 cycles at each of them.)
+    auto fetch = [&](const int64_t (&from)[kLoads], const char* base, Raw (&raw)[kLoads]) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            if constexpr (FP8) raw[i] = load8<false>(base + from[i]);
+            else raw[i] = load16<false>(base + from[i]);
+        }
+    };
+    // A masked weight of 0 times a value that is not finite would be NaN.  Where
+    // a mask cuts a tile that has such values, they are zeros in the product
+    // and are kept aside for the rows that see them.
+    auto put = [&](const Tile& w, auto plain, char* to, char* aside, const Raw (&raw)[kLoads]) {
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
             const int key = key0 + i * kKeyStep;
-            const u32x2 k = k_codes[i], v = v_codes[i];
-            odd |= put(s_k, s_v, mask, open, i,
-                       u32x4{e4m3_pair<DT, false>(k[0]), e4m3_pair<DT, true>(k[0]), e4m3_pair<DT, false>(k[1]), e4m3_pair<DT, true>(k[1])},
-                       u32x4{e4m3_pair<DT, false>(v[0]), e4m3_pair<DT, true>(v[0]), e4m3_pair<DT, false>(v[1]), e4m3_pair<DT, true>(v[1])},
-                       place<kPieces>(key, slot) * 8 < a.dim);
+            u32x4 x;
+            if constexpr (FP8) x = u32x4{e4m3_pair<DT, false>(raw[i][0]), e4m3_pair<DT, true>(raw[i][0]), e4m3_pair<DT, false>(raw[i][1]), e4m3_pair<DT, true>(raw[i][1])};
+            else x = raw[i];
+            if (!plain.value && (!w.open || a.dim != DP)) {
+                const bool keep = (place<kPieces>(key, slot) * 8 < a.dim) & there(w.index * kKeys + key);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[j] &= keep ? ~0u : 0u;
+            }
+            if (!plain.value && aside && !w.open) {
+                *reinterpret_cast<u32x4*>(aside + key * kPitch + slot * 16) = x;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool lo = not_finite<DT>(x[j] & 0xffffu), hi = not_finite<DT>(x[j] >> 16);
+                    odd |= lo | hi;
+                    x[j] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                }
+            }
+            *reinterpret_cast<u32x4*>(to + key * kPitch + slot * 16) = x;
         }
         return odd;
     };
-    // 16-bit pieces of a tile that is whole go to LDS directly.
-    auto stage = [&](char* s_k, char* s_v, mfh_u64 mask, bool open) {
-        bool odd = false;
-        if (open && a.dim == DP) {
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) {
-                bool in_dim;
-                const int64_t from = piece_at(i, &in_dim);
-                const int to = (i * kThreads + wave * 64) * 16;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(k_base + from),
-                                                 (__attribute__((address_space(3))) void*)(s_k + to), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(v_base + from),
-                                                 (__attribute__((address_space(3))) void*)(s_v + to), 16, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) {
-                bool in_dim;
-                const int64_t from = piece_at(i, &in_dim);
-                const u32x4 k = load16<false>(k_base + from), v = load16<false>(v_base + from);
-                odd |= put(s_k, s_v, mask, open, i, k, v, in_dim);
-            }
-        }
-        return odd;
-    };
-
+    // ---- what a row sees
     // Score i of block b is of key 32 b + 4 half + 8 (i / 4) + i % 4; whether this lane's row sees it:
     struct Seen {
         mfh_u32 there;
@@ -241,57 +278,76 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
     auto seen_from = [&](int key, mfh_u32 there) {
         return Seen{there, position - key, a.window > 0 ? position - key - a.window : -kKeys, prefix - key};
     };
-
-    // A masked weight of 0 times a value that is not finite would be NaN.  Where
-    // a mask cuts a tile that has such values, they are added to the rows that
-    // see them, and are zeros in the product.
-    auto add_odd = [&](const char* s_v, int tile, mfh_u64 mask) {
-        const Seen seen = seen_from(tile * kKeys, 0);
+    auto add_odd = [&](const char* aside, const Tile& w) {
+        const Seen seen = seen_from(w.index * kKeys, 0);
         for (int key = 0; key < kKeys; key++) {
-            const bool see = is_valid(mask, key) & (((key <= seen.back) & (key > seen.oldest)) | (key < seen.in_prefix));
+            const bool see = there(w.index * kKeys + key) & (((key <= seen.back) & (key > seen.oldest)) | (key < seen.in_prefix));
 #pragma unroll
             for (int d = 0; d < kDimTiles; d++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int dim = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-                    const mfh_u32 v = *reinterpret_cast<const mfh_u16*>(s_v + key * kPitch + place<kPieces>(key, dim / 8) * 16 + dim % 8 * 2);
+                    const mfh_u32 v = *reinterpret_cast<const mfh_u16*>(aside + key * kPitch + place<kPieces>(key, dim / 8) * 16 + dim % 8 * 2);
                     if (see & not_finite<DT>(v)) acc[d][i] += dec16<DT>(v);
                 }
             }
         }
     };
-    auto clear_odd = [&](char* s_v) {
-        for (int i = 0; i < kLoads; i++) {
-            u32x4& w = *reinterpret_cast<u32x4*>(s_v + (key0 + i * kKeyStep) * kPitch + slot * 16);
-            u32x4 v = w;
+
+    // ---- the products and what lies between them
+    f32x16 s[kBlocks];
+    u32x4 p[2 * kBlocks];
+    // K of step d (16 dims) for the tile's blocks of 32 keys, and V^T of 16 keys
+    // and 32 dims: in 16 lanes row lane % 16 / 4 of four keys, columns 4 (lane % 4) ..
+    auto k_piece = [&](const char* k_from, int d, int b) {
+        const int key = 32 * b + col;
+        return *reinterpret_cast<const u32x4*>(k_from + key * kPitch + place<kPieces>(key, 2 * d + half) * 16);
+    };
+    auto v_piece = [&](const char* v_from, int n) {
+        const int j = n / kDimTiles, d = n % kDimTiles;
+        auto column = [&](int key) {
+            const int at_key = key + 4 * half + (lane & 15) / 4, piece = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
+            return read_column(v_from + at_key * kPitch + place<kPieces>(at_key, piece) * 16 + 8 * (lane & 1));
+        };
+        const u32x2 lo = column(16 * j), hi = column(16 * j + 8);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    // Scores of a tile and the weights of the one before times its V.  Reads of
+    // LDS run kAhead products ahead of their use, in this order: left to itself
+    // the compiler reads right ahead of each product and waits there.
+    constexpr int kScores = kSteps * kBlocks, kWeights = kDimTiles * 2 * kBlocks, kAhead = 6;
+    auto products = [&](const char* __restrict__ k_from, const char* __restrict__ v_from, auto with_scores) {
+        constexpr int kFirst = with_scores.value ? 0 : kScores;
+        u32x4 piece[kScores + kWeights];
+        auto read = [&](int n) {
+            if (n < kScores) piece[n] = k_piece(k_from, n / kBlocks, n % kBlocks);
+            else if (n < kScores + kWeights) piece[n] = v_piece(v_from, n - kScores);
+        };
+        if constexpr (with_scores.value) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] &= (not_finite<DT>(v[j] & 0xffffu) ? 0u : 0xffffu) | (not_finite<DT>(v[j] >> 16) ? 0u : 0xffff0000u);
-            w = v;
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
+        }
+#pragma unroll
+        for (int n = kFirst; n < kFirst + kAhead; n++) read(n);
+#pragma unroll
+        for (int n = kFirst; n < kScores + kWeights; n++) {
+            read(n + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+            if (n < kScores) s[n % kBlocks] = mfma32<DT>(piece[n], q[n / kBlocks], s[n % kBlocks]);
+            else acc[(n - kScores) % kDimTiles] = mfma32<DT>(piece[n], p[(n - kScores) / kDimTiles], acc[(n - kScores) % kDimTiles]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-
-    auto compute = [&](const char* s_k, const char* s_v, int tile, mfh_u64 mask) {
-        const int key_first = tile * kKeys;
-        // Rows of this wave that see something here, and whether all of it.
-        const bool some = key_first < max(wave_high + 1, prefix) &&
-                          (a.window <= 0 || key_first < prefix || key_first + kKeys > wave_low - a.window + 1);
-        if (!some) return;
-        f32x16 s[kBlocks];
-#pragma unroll
-        for (int b = 0; b < kBlocks; b++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < kSteps; d++) {
-                const int key = 32 * b + col;
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(s_k + key * kPitch + place<kPieces>(key, 2 * d + half) * 16);
-                s[b] = mfma32<DT>(kf, q[d], s[b]);
-            }
-        }
-        const bool all = mask == kAll && ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
-                                          key_first + kKeys <= prefix);
+    auto soften = [&](const Tile& w, auto plain) {
+        const int key_first = w.index * kKeys;
+        const bool all = w.open || clean && key_first + kKeys <= length && ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
+                                             key_first + kKeys <= prefix);
         float scale = a.scale;  // what is left to multiply by
-        if (a.cap_scaled != 0.0f || a.slopes || !all || !(scale > 0.0f)) {
+        if constexpr (!plain.value) {
+            mfh_u64 mask = 0;   // bit i: key i is there
+            if (!all) mask = __ballot(there(key_first + lane));
             scale = 1.0f;
 #pragma unroll
             for (int b = 0; b < kBlocks; b++) {
@@ -301,7 +357,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
 #pragma unroll
                     for (int i = 0; i < 16; i++) s[b][i] = capped(s[b][i], a.cap_twice, a.cap_scaled);
                 }
-                const Seen seen = seen_from(key_first + 32 * b + 4 * half, (mfh_u32)(mask >> (64 - kKeys + 32 * b)) >> (4 * half));
+                const Seen seen = seen_from(key_first + 32 * b + 4 * half, (mfh_u32)(mask >> (32 * b)) >> (4 * half));
                 if (a.slopes) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) s[b][i] -= slope * fabsf((float)(seen.back - (8 * (i / 4) + i % 4)));
@@ -330,83 +386,138 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
                 for (int d = 0; d < kDimTiles; d++) acc[d] *= alpha;
             }
         }
-        u32x4 p[2 * kBlocks];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++) {
-            float part = 0.0f;
+            float part_sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 s[b][i] = exp2_fast(__builtin_fmaf(s[b][i], scale, -ref));
-                part += s[b][i];
+                part_sum += s[b][i];
             }
-            sum += part;
+            sum += part_sum;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) p[2 * b + i / 8][i / 2 % 4] = enc16x2<DT>(s[b][i], s[b][i + 1]);
         }
-        // V^T: in 16 lanes row lane % 16 / 4 of four keys, columns 4 (lane % 4) ..
-        auto column = [&](int key, int d) {
-            const int at_key = key + 4 * half + (lane & 15) / 4, piece = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
-            return read_column(s_v + at_key * kPitch + place<kPieces>(at_key, piece) * 16 + 8 * (lane & 1));
-        };
-#pragma unroll
-        for (int d = 0; d < kDimTiles; d++) {
-#pragma unroll
-            for (int j = 0; j < 2 * kBlocks; j++) {
-                const u32x2 lo = column(16 * j, d), hi = column(16 * j + 8, d);
-                acc[d] = mfma32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[j], acc[d]);
-            }
-        }
+    };
+    auto barrier = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     };
 
-    // One tile is computed while the next one is on its way to the other half
-    // of LDS.
-    int tile = next_tile(0), now = 0;
-    mfh_u64 mask = 0;
-    bool odd = false, open = true;
-    auto meet = [&]() {  // all of the staged tile is in LDS
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): loads into LDS are no one's registers
-        odd = open ? (__syncthreads(), false) : __syncthreads_or(odd) != 0;
-    };
-    if (tile < tile_end) {
-        locate(tile);
-        mask = valid, open = is_open(tile, mask);
-        if constexpr (FP8) {
-            fetch();
-            odd = put_codes(s_tiles[0][0], s_tiles[0][1], mask, open);
-        } else {
-            odd = stage(s_tiles[0][0], s_tiles[0][1], mask, open);
+    // Round i of a wave multiplies tile i with Q and the weights of tile i - 1
+    // with V, and then softens the scores of tile i, each between two barriers.
+    // The second four waves run one barrier behind the first four: of the two
+    // waves of a SIMD one has the matrix units while the other one has the vector
+    // units.  Tiles are three deep in LDS: K of tile i + 2 and V of tile i + 1 are
+    // loaded ahead of the softening and put into LDS behind it, where every wave
+    // has left round i - 1's products.
+    const int tile0 = next_tile(first_tile + (int)part * share);
+    if (tile0 < tile_end) {
+        Raw k_raw[kLoads], v_raw[kLoads];
+        Keys keys;  // of the next tile whose K sets out
+        int64_t k_from[kLoads], v_from[kLoads];
+        auto follow = [&](int tile) { return tile < tile_end ? next_tile(tile + 1) : tile; };
+        auto move = [&](int from, int to) {
+            if (to == from + 1) go_on(keys);
+            else go_to(keys, to);
+            ask(keys);
+        };
+        Tile now = describe(tile0), next = describe(follow(tile0)), after = describe(follow(next.index)), before = now;
+        go_to(keys, tile0);
+        ask(keys);
+        locate(keys, k_from);
+        fetch(k_from, k_base, k_raw);
+        fetch(k_from, v_base, v_raw);
+        if (threadIdx.x < 3) s_odd[threadIdx.x] = -1;
+        for (int i = threadIdx.x * 16; i < kKeys * kPitch; i += kThreads * 16) *reinterpret_cast<u32x4*>(s_v[2] + i) = u32x4{0, 0, 0, 0};
+        move(tile0, next.index);
+        put(now, std::false_type{}, s_k[0], nullptr, k_raw);
+        const bool odd0 = put(now, std::false_type{}, s_v[0], s_raw[0], v_raw);
+        locate(keys, v_from);
+        if (next.index < tile_end) {
+            fetch(v_from, k_base, k_raw);
+            put(next, std::false_type{}, s_k[1], nullptr, k_raw);
         }
-        meet();
-    }
-    while (tile < tile_end) {
-        const char* s_k = s_tiles[now][0];
-        char* s_v = s_tiles[now][1];
-        const int following = next_tile(tile + 1);
-        const mfh_u64 mask_now = mask;
-        if (odd) {
-            add_odd(s_v, tile, mask);
-            __syncthreads();
-            clear_odd(s_v);
-            __syncthreads();
-            odd = false;
+        move(next.index, after.index);
+#pragma unroll
+        for (int j = 0; j < 2 * kBlocks; j++) p[j] = u32x4{0, 0, 0, 0};
+        int third = 0, round = 0;  // third of LDS of tile i
+        __syncthreads();
+        if (odd0) s_odd[0] = 0;
+        __syncthreads();
+        if (group == 1) barrier();
+        // Rounds whose tiles follow one another, are seen whole and need no more
+        // than the scale go without the questions that the others have to ask:
+        // their branches took as long as the products.
+        const int plain_begin = a.window > 0 ? max(high_position - a.window + kKeys, 0) / kKeys : 0;
+        const int plain_end = clean && a.dim == DP && a.cap_scaled == 0.0f && !a.slopes && a.scale > 0.0f
+                                  ? min(min(length, low_position + 1) / kKeys, tile_end) : 0;
+        auto turn = [&](auto plain) {
+            const int ahead = third == 2 ? 0 : third + 1, behind = third == 0 ? 2 : third - 1;
+            if (!plain.value && round > 0 && !before.open && s_odd[behind] == round - 1) add_odd(s_raw[behind], before);
+            __builtin_amdgcn_s_setprio(1);
+            products(s_k[third], s_v[behind], std::true_type{});
+            __builtin_amdgcn_s_setprio(0);
+            barrier();
+            const bool put_v = plain.value || next.index < tile_end, put_k = plain.value || after.index < tile_end;
+            if (put_k) {
+                locate(keys, k_from);
+                fetch(k_from, k_base, k_raw);
+            }
+            if (put_v) fetch(v_from, v_base, v_raw);
+            before = now, now = next, next = after;
+            if constexpr (plain.value) {
+                after.index++;
+                go_on(keys);
+                ask(keys);
+            } else {
+                after = describe(follow(after.index));
+                move(next.index, after.index);
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) v_from[i] = k_from[i];
+            soften(before, plain);
+#pragma unroll
+            for (int j = 0; j < 2 * kBlocks; j++) asm volatile("" : "+v"(p[j]));  // here, not behind the barrier
+            asm volatile("" : "+v"(sum));
+            if (put_k) put(next, plain, s_k[behind], nullptr, k_raw);
+            if (put_v && put(now, plain, s_v[ahead], s_raw[ahead], v_raw)) s_odd[ahead] = round + 1;
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): it is in LDS
+            barrier();
+            third = ahead;
+            round++;
+        };
+        while (now.index < tile_end) {
+            // the tile before is whole too, or there is none
+            while (now.index > plain_begin && after.index + 1 < plain_end) turn(std::true_type{});
+            turn(std::false_type{});
         }
-        if (following < tile_end) {
-            locate(following);
-            mask = valid, open = is_open(following, mask);
-            if constexpr (FP8) fetch();
-            else odd = stage(s_tiles[now ^ 1][0], s_tiles[now ^ 1][1], mask, open);
-        }
-        compute(s_k, s_v, tile, mask_now);
-        tile = following;
-        if (following < tile_end) {
-            if constexpr (FP8) odd = put_codes(s_tiles[now ^ 1][0], s_tiles[now ^ 1][1], mask, open);
-            meet();
-        }
-        now ^= 1;
+        if (group == 0) barrier();
+        const int behind = third == 0 ? 2 : third - 1;
+        if (!before.open && s_odd[behind] == round - 1) add_odd(s_raw[behind], before);
+        products(s_k[0], s_v[behind], std::false_type{});
     }
 
     sum += __shfl_xor(sum, 32);
     if (!real) return;
+    const int64_t out_row = (begin + token) * a.q_heads + head;
+    if (a.parts > 1) {
+        const int64_t at_part = out_row * a.parts + part;
+#pragma unroll
+        for (int d = 0; d < kDimTiles; d++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int dim = 32 * d + 8 * i + 4 * half;
+                if (dim < a.dim)
+                    *reinterpret_cast<f32x4*>(a.part_out + at_part * a.dim + dim) = f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+            }
+        }
+        if (half == 0) a.part_sum[at_part] = make_float2(limit == -INFINITY ? -INFINITY : ref, sum);
+        return;
+    }
     const float f = sum == 0.0f ? 0.0f : a.v_scale / sum;
     char* to = a.out + ((begin + token) * a.out_t + head * a.out_h) * 2;
 #pragma unroll
@@ -419,16 +530,15 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void k_prefill(Prefill
                                            enc16x2<DT>(acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f)});
         }
     }
-    if (half == 0 && a.lse)
-        a.lse[(begin + token) * a.q_heads + head] = sum == 0.0f ? -INFINITY : ref * kLn2 + logf(sum);
+    if (half == 0 && a.lse) a.lse[out_row] = sum == 0.0f ? -INFINITY : ref * kLn2 + logf(sum);
 }
 
 template <int DT, bool FP8>
 void launch_dims(int dim, unsigned grid, hipStream_t s, const PrefillArgs& a)
 {
-    if (dim <= 64) k_prefill<DT, FP8, 64><<<grid, kThreads, 0, s>>>(a);
-    else if (dim <= 128) k_prefill<DT, FP8, 128><<<grid, kThreads, 0, s>>>(a);
-    else k_prefill<DT, FP8, 256><<<grid, kThreads, 0, s>>>(a);
+    if (dim <= 64) k_prefill<DT, FP8, 64><<<grid, 64 * waves_of(64), 0, s>>>(a);
+    else if (dim <= 128) k_prefill<DT, FP8, 128><<<grid, 64 * waves_of(128), 0, s>>>(a);
+    else k_prefill<DT, FP8, 256><<<grid, 64 * waves_of(256), 0, s>>>(a);
 }
 
 }  // namespace
@@ -492,12 +602,16 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     a.window = shape->window < kLongest ? shape->window : 0, a.kv_heads = cache->kv_heads, a.q_heads = shape->q_heads;
     a.group = shape->q_heads / cache->kv_heads;
     a.dim = cache->head_dim;
+    const int kRows = 32 * waves_of(a.dim), kThreads = 2 * kRows;
     const int64_t row_tiles = (a.most_fresh * a.group + kRows - 1) / kRows;
     const __int128 grid = (__int128)row_tiles * cache->kv_heads * requests;
     if (a.most_fresh * a.group > 0x7fffffff || grid >= ((int64_t)1 << 32) / kThreads)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %lld tokens and %d heads are too many for one call",
                     what, requests, (long long)a.most_fresh, shape->q_heads);
     a.row_tiles = (mfh_u32)row_tiles;
+    a.parts = 1, a.by_parts = Divider(1);
+    const int keys = keys_of(a.dim);
+    a.step_entries = (mfh_u32)(keys / cache->page_size), a.step_bytes = (mfh_u32)(keys % cache->page_size) * a.pages.token_bytes;
     a.by_group = Divider((mfh_u32)a.group), a.by_kv_heads = Divider((mfh_u32)a.kv_heads), a.by_row_tiles = Divider(a.row_tiles);
     hipStream_t s = (hipStream_t)stream;
     const bool fp8 = cache->dtype == kF8E4M3;
