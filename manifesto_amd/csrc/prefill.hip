@@ -44,7 +44,7 @@ struct PrefillArgs {
     mfh_u32 row_tiles;  // of a request and head at most
     mfh_u32 parts;      // of a row's keys
     mfh_u32 step_entries, step_bytes;  // a tile's keys in whole pages, and in bytes of a page
-    Divider by_group, by_kv_heads, by_row_tiles, by_parts;
+    Divider by_group, by_kv_heads, by_row_tiles, by_parts, by_q_heads;
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -201,11 +201,7 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
             keys.entry[i] += a.step_entries + (over ? 1 : 0);
         }
     };
-    // Whether a page of the request is not one of the cache's: its keys are
-    // masked then, and nothing takes the short ways.
-    bool bad = false;
-    for (mfh_u32 i = threadIdx.x; length > 0 && i <= last_entry; i += kThreads) bad |= (mfh_u32)table[i] >= a.pages.pages;
-    const bool clean = !__syncthreads_or(bad);
+    bool clean = true;  // every page of the request is one of the cache's
     auto there = [&](int key) {
         bool is = key < length;
         if (!clean) is &= (mfh_u32)table[min(a.pages.by_page.quotient((mfh_u32)key), last_entry)] < a.pages.pages;
@@ -315,7 +311,7 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
     // Scores of a tile and the weights of the one before times its V.  Reads of
     // LDS run kAhead products ahead of their use, in this order: left to itself
     // the compiler reads right ahead of each product and waits there.
-    constexpr int kScores = kSteps * kBlocks, kWeights = kDimTiles * 2 * kBlocks, kAhead = 6;
+    constexpr int kScores = kSteps * kBlocks, kWeights = kDimTiles * 2 * kBlocks, kAhead = 5;
     auto products = [&](const char* __restrict__ k_from, const char* __restrict__ v_from, auto with_scores) {
         constexpr int kFirst = with_scores.value ? 0 : kScores;
         u32x4 piece[kScores + kWeights];
@@ -340,14 +336,17 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    const bool optional = a.cap_scaled != 0.0f || a.slopes || !(a.scale > 0.0f);
     auto soften = [&](const Tile& w, auto plain) {
         const int key_first = w.index * kKeys;
         const bool all = w.open || clean && key_first + kKeys <= length && ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
                                              key_first + kKeys <= prefix);
         float scale = a.scale;  // what is left to multiply by
-        if constexpr (!plain.value) {
+        if (!plain.value || optional) {
+            // a row's position is below the length
+            const bool only_causal = clean && a.window <= 0 && prefix == 0;
             mfh_u64 mask = 0;   // bit i: key i is there
-            if (!all) mask = __ballot(there(key_first + lane));
+            if (!plain.value && !all && !only_causal) mask = __ballot(there(key_first + lane));
             scale = 1.0f;
 #pragma unroll
             for (int b = 0; b < kBlocks; b++) {
@@ -359,21 +358,27 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
                 }
                 const Seen seen = seen_from(key_first + 32 * b + 4 * half, (mfh_u32)(mask >> (32 * b)) >> (4 * half));
                 if (a.slopes) {
+                    const float back = (float)seen.back;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) s[b][i] -= slope * fabsf((float)(seen.back - (8 * (i / 4) + i % 4)));
+                    for (int i = 0; i < 16; i++) s[b][i] = __builtin_fmaf(-slope, fabsf(back - (float)(8 * (i / 4) + i % 4)), s[b][i]);
                 }
-                if (!all) {
+                if (!plain.value && !all) {
+                    if (only_causal) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) s[b][i] = seen(8 * (i / 4) + i % 4) ? s[b][i] : -INFINITY;
+                        for (int i = 0; i < 16; i++) s[b][i] = 8 * (i / 4) + i % 4 <= seen.back ? s[b][i] : -INFINITY;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) s[b][i] = seen(8 * (i / 4) + i % 4) ? s[b][i] : -INFINITY;
+                    }
                 }
             }
         }
-        float top = -INFINITY;
+        float tops[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};  // (four chains, here and for the sum)
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, s[b][i]);
-        top *= scale;
+            for (int i = 0; i < 16; i++) tops[i / 4] = fmaxf(tops[i / 4], s[b][i]);
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
         if (__any(top > limit)) {
             top = fmaxf(top, __shfl_xor(top, 32));
             if (top > limit) {
@@ -386,18 +391,18 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
                 for (int d = 0; d < kDimTiles; d++) acc[d] *= alpha;
             }
         }
+        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < kBlocks; b++) {
-            float part_sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 s[b][i] = exp2_fast(__builtin_fmaf(s[b][i], scale, -ref));
-                part_sum += s[b][i];
+                sums[i % 4] += s[b][i];
             }
-            sum += part_sum;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) p[2 * b + i / 8][i / 2 % 4] = enc16x2<DT>(s[b][i], s[b][i + 1]);
         }
+        sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
     };
     auto barrier = [&]() {
         __builtin_amdgcn_sched_barrier(0);
@@ -418,27 +423,32 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
     if (tile0 < tile_end) {
         Raw k_raw[kLoads], v_raw[kLoads];
         Keys keys;  // of the next tile whose K sets out
-        int64_t k_from[kLoads], v_from[kLoads];
+        int64_t from[kLoads];  // of the last tile whose K set out
         auto follow = [&](int tile) { return tile < tile_end ? next_tile(tile + 1) : tile; };
         auto move = [&](int from, int to) {
             if (to == from + 1) go_on(keys);
             else go_to(keys, to);
             ask(keys);
         };
-        Tile now = describe(tile0), next = describe(follow(tile0)), after = describe(follow(next.index)), before = now;
         go_to(keys, tile0);
         ask(keys);
-        locate(keys, k_from);
-        fetch(k_from, k_base, k_raw);
-        fetch(k_from, v_base, v_raw);
+        locate(keys, from);
+        fetch(from, k_base, k_raw);
+        fetch(from, v_base, v_raw);
+        // Keys of a page that is not one of the cache's are masked, and nothing
+        // takes the short ways then.
+        bool bad = false;
+        for (mfh_u32 i = threadIdx.x; i <= last_entry; i += kThreads) bad |= (mfh_u32)table[i] >= a.pages.pages;
+        clean = !__syncthreads_or(bad);
+        Tile now = describe(tile0), next = describe(follow(tile0)), after = describe(follow(next.index)), before = now;
         if (threadIdx.x < 3) s_odd[threadIdx.x] = -1;
         for (int i = threadIdx.x * 16; i < kKeys * kPitch; i += kThreads * 16) *reinterpret_cast<u32x4*>(s_v[2] + i) = u32x4{0, 0, 0, 0};
         move(tile0, next.index);
         put(now, std::false_type{}, s_k[0], nullptr, k_raw);
         const bool odd0 = put(now, std::false_type{}, s_v[0], s_raw[0], v_raw);
-        locate(keys, v_from);
+        locate(keys, from);
         if (next.index < tile_end) {
-            fetch(v_from, k_base, k_raw);
+            fetch(from, k_base, k_raw);
             put(next, std::false_type{}, s_k[1], nullptr, k_raw);
         }
         move(next.index, after.index);
@@ -449,12 +459,11 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
         if (odd0) s_odd[0] = 0;
         __syncthreads();
         if (group == 1) barrier();
-        // Rounds whose tiles follow one another, are seen whole and need no more
-        // than the scale go without the questions that the others have to ask:
-        // their branches took as long as the products.
+        // Rounds whose tiles follow one another and are seen whole go without the
+        // questions that the others have to ask: their branches took as long as
+        // the products.
         const int plain_begin = a.window > 0 ? max(high_position - a.window + kKeys, 0) / kKeys : 0;
-        const int plain_end = clean && a.dim == DP && a.cap_scaled == 0.0f && !a.slopes && a.scale > 0.0f
-                                  ? min(min(length, low_position + 1) / kKeys, tile_end) : 0;
+        const int plain_end = clean && a.dim == DP ? min(min(length, low_position + 1) / kKeys, tile_end) : 0;
         auto turn = [&](auto plain) {
             const int ahead = third == 2 ? 0 : third + 1, behind = third == 0 ? 2 : third - 1;
             if (!plain.value && round > 0 && !before.open && s_odd[behind] == round - 1) add_odd(s_raw[behind], before);
@@ -463,11 +472,11 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
             __builtin_amdgcn_s_setprio(0);
             barrier();
             const bool put_v = plain.value || next.index < tile_end, put_k = plain.value || after.index < tile_end;
+            if (put_v) fetch(from, v_base, v_raw);
             if (put_k) {
-                locate(keys, k_from);
-                fetch(k_from, k_base, k_raw);
+                locate(keys, from);
+                fetch(from, k_base, k_raw);
             }
-            if (put_v) fetch(v_from, v_base, v_raw);
             before = now, now = next, next = after;
             if constexpr (plain.value) {
                 after.index++;
@@ -477,8 +486,6 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
                 after = describe(follow(after.index));
                 move(next.index, after.index);
             }
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) v_from[i] = k_from[i];
             soften(before, plain);
 #pragma unroll
             for (int j = 0; j < 2 * kBlocks; j++) asm volatile("" : "+v"(p[j]));  // here, not behind the barrier
@@ -502,10 +509,15 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
     }
 
     sum += __shfl_xor(sum, 32);
-    if (!real) return;
-    const int64_t out_row = (begin + token) * a.q_heads + head;
+    // the row's place anew: kept through the loop it costs registers there
+    mfh_u32 out_at = row0 + 32 * wave + col;
+    asm volatile("" : "+v"(out_at));
+    if (out_at >= rows) return;
+    const mfh_u32 out_token = a.by_group.quotient(out_at), out_head = kv * a.group + (out_at - out_token * a.group);
+    const int64_t out_row = (begin + out_token) * a.q_heads + out_head;
     if (a.parts > 1) {
         const int64_t at_part = out_row * a.parts + part;
+        if (tile0 < tile_end)
 #pragma unroll
         for (int d = 0; d < kDimTiles; d++) {
 #pragma unroll
@@ -519,7 +531,7 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
         return;
     }
     const float f = sum == 0.0f ? 0.0f : a.v_scale / sum;
-    char* to = a.out + ((begin + token) * a.out_t + head * a.out_h) * 2;
+    char* to = a.out + ((begin + out_token) * a.out_t + out_head * a.out_h) * 2;
 #pragma unroll
     for (int d = 0; d < kDimTiles; d++) {
 #pragma unroll
@@ -531,6 +543,69 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
         }
     }
     if (half == 0 && a.lse) a.lse[out_row] = sum == 0.0f ? -INFINITY : ref * kLn2 + logf(sum);
+}
+
+// Joins the parts of the rows that were computed.  A row takes the lanes that
+// its dims need, four dims each, and the wave as many rows as fit.
+template <int DT, int LANES>
+__global__ __launch_bounds__(256) void k_prefill_join(PrefillArgs a, int requests)
+{
+    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;  // token * q_heads + head
+    const int dim = 4 * (threadIdx.x % LANES);
+    if (row >= a.tokens * a.q_heads) return;
+    const mfh_u32 token = a.by_q_heads.quotient((mfh_u32)row);
+    // the last request that starts at or before the token
+    int lo = 0, hi = requests;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.starts[mid] <= (int64_t)token) lo = mid;
+        else hi = mid;
+    }
+    const int64_t begin = min(max((int64_t)a.starts[lo], (int64_t)0), a.tokens), end = min(max((int64_t)a.starts[lo + 1], begin), a.tokens);
+    if (token < begin || token >= end || token - begin >= a.most_fresh || dim >= a.dim) return;
+    const float2* sums = a.part_sum + row * a.parts;
+    float top = -INFINITY;
+    for (mfh_u32 n = 0; n < a.parts; n++) top = fmaxf(top, sums[n].x);
+    float all = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (mfh_u32 n = 0; n < a.parts; n++) {
+        const float2 s = sums[n];
+        if (s.x == -INFINITY && s.y == 0.0f) continue;  // a part that saw nothing has written nothing else
+        const float f = s.x == -INFINITY ? 1.0f : exp2_fast(s.x - top);
+        all += f * s.y;
+        o += f * *reinterpret_cast<const f32x4*>(a.part_out + (row * a.parts + n) * a.dim + dim);
+    }
+    const float f = all == 0.0f ? 0.0f : a.v_scale / all;
+    char* to = a.out + ((int64_t)token * a.out_t + (row - (int64_t)token * a.q_heads) * a.out_h + dim) * 2;
+    store8(to, u32x2{enc16x2<DT>(o[0] * f, o[1] * f), enc16x2<DT>(o[2] * f, o[3] * f)});
+    if (dim == 0 && a.lse) a.lse[row] = all == 0.0f ? -INFINITY : top * kLn2 + logf(all);
+}
+
+// Workgroups of a call at most, and the parts that a row's keys are split into:
+// where the rows do not fill the card, as many as do, of eight tiles at least.
+// (256 workgroups for 256 CUs: 302 us whole, 340 us in two parts.)
+struct Layout {
+    int64_t row_tiles;
+    __int128 blocks;  // of one part
+    mfh_u32 parts;
+    size_t bytes;
+};
+
+Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cache& c, int32_t requests, int64_t tokens,
+              int64_t most_fresh, int64_t longest)
+{
+    Layout l{};
+    const int rows = 32 * waves_of(c.head_dim), group = sh.q_heads / c.kv_heads;
+    most_fresh = std::min(most_fresh, tokens);
+    l.row_tiles = (most_fresh * group + rows - 1) / rows;
+    l.blocks = (__int128)l.row_tiles * c.kv_heads * requests;
+    const int64_t tiles = std::min<int64_t>(std::max<int64_t>(longest, 1), kLongest) / keys_of(c.head_dim);
+    // those that find rows, whatever the requests' sizes
+    const __int128 busy = std::min<__int128>(l.blocks, ((__int128)tokens * group / rows + requests) * c.kv_heads);
+    const int64_t wanted = busy > 0 ? (int64_t)(3 * dev->compute_units / (2 * busy)) : 1;
+    l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / 8, 64}));
+    l.bytes = l.parts > 1 ? (size_t)tokens * sh.q_heads * l.parts * (c.head_dim + 2) * sizeof(float) : 0;
+    return l;
 }
 
 template <int DT, bool FP8>
@@ -558,7 +633,7 @@ int mfh_paged_prefill_workspace(const mfh_attention_shape* shape, const mfh_kv_c
     if (requests < 0 || tokens < 0 || most_fresh < 0)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: negative number of requests or tokens", what);
     if (!bytes) return fail(MFH_ERR_INVALID_ARGUMENT, "%s: NULL result", what);
-    *bytes = 0;
+    *bytes = layout(dev, *shape, *cache, requests, tokens, most_fresh, longest).bytes;
     return MFH_OK;
 }
 
@@ -602,14 +677,18 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     a.window = shape->window < kLongest ? shape->window : 0, a.kv_heads = cache->kv_heads, a.q_heads = shape->q_heads;
     a.group = shape->q_heads / cache->kv_heads;
     a.dim = cache->head_dim;
-    const int kRows = 32 * waves_of(a.dim), kThreads = 2 * kRows;
-    const int64_t row_tiles = (a.most_fresh * a.group + kRows - 1) / kRows;
-    const __int128 grid = (__int128)row_tiles * cache->kv_heads * requests;
-    if (a.most_fresh * a.group > 0x7fffffff || grid >= ((int64_t)1 << 32) / kThreads)
+    Layout l = layout(dev, *shape, *cache, requests, tokens, most_fresh, std::min<int64_t>(longest, (int64_t)table_width * cache->page_size));
+    if (l.bytes > workspace_bytes || tokens * shape->q_heads > kLongest) l.parts = 1;
+    const __int128 grid = l.blocks * l.parts;
+    if (a.most_fresh * a.group > kLongest || grid >= ((int64_t)1 << 32) / (64 * waves_of(a.dim)))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %lld tokens and %d heads are too many for one call",
                     what, requests, (long long)a.most_fresh, shape->q_heads);
-    a.row_tiles = (mfh_u32)row_tiles;
-    a.parts = 1, a.by_parts = Divider(1);
+    a.row_tiles = (mfh_u32)l.row_tiles;
+    a.parts = l.parts, a.by_parts = Divider(l.parts), a.by_q_heads = Divider((mfh_u32)a.q_heads);
+    if (l.parts > 1) {
+        a.part_out = (float*)workspace;
+        a.part_sum = (float2*)(a.part_out + tokens * shape->q_heads * l.parts * a.dim);
+    }
     const int keys = keys_of(a.dim);
     a.step_entries = (mfh_u32)(keys / cache->page_size), a.step_bytes = (mfh_u32)(keys % cache->page_size) * a.pages.token_bytes;
     a.by_group = Divider((mfh_u32)a.group), a.by_kv_heads = Divider((mfh_u32)a.kv_heads), a.by_row_tiles = Divider(a.row_tiles);
@@ -622,7 +701,17 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
         if (fp8) launch_dims<kFloat16, true>(a.dim, (unsigned)grid, s, a);
         else launch_dims<kFloat16, false>(a.dim, (unsigned)grid, s, a);
     }
-    return launch_status("k_prefill");
+    MFH_TRY(launch_status("k_prefill"));
+    if (l.parts > 1) {
+        const int lanes = a.dim <= 64 ? 16 : a.dim <= 128 ? 32 : 64;
+        const unsigned blocks = (unsigned)((tokens * shape->q_heads * lanes + 255) / 256);
+        const bool bf16 = shape->dtype == kBFloat16;
+        if (lanes == 16) bf16 ? k_prefill_join<kBFloat16, 16><<<blocks, 256, 0, s>>>(a, requests) : k_prefill_join<kFloat16, 16><<<blocks, 256, 0, s>>>(a, requests);
+        else if (lanes == 32) bf16 ? k_prefill_join<kBFloat16, 32><<<blocks, 256, 0, s>>>(a, requests) : k_prefill_join<kFloat16, 32><<<blocks, 256, 0, s>>>(a, requests);
+        else bf16 ? k_prefill_join<kBFloat16, 64><<<blocks, 256, 0, s>>>(a, requests) : k_prefill_join<kFloat16, 64><<<blocks, 256, 0, s>>>(a, requests);
+        MFH_TRY(launch_status("k_prefill_join"));
+    }
+    return MFH_OK;
 }
 
 }  // extern "C"
