@@ -2,12 +2,12 @@
 // (mfh_paged_prefill): causal, with an optional window, prefix, cap and bias.
 //
 // 4 * pairs * q_heads * head_dim operations over keys and values that stay in
-// the caches near the cores: the matrix cores bound it.  The rows of one
-// key-value head are its query heads of all new tokens (row = token * group +
-// head of the group), so that heads which share keys share a workgroup's key
-// tiles too.  A workgroup is four waves of 32 rows each and walks over tiles of
-// 64 keys, staged through LDS: the next tile's pieces are loaded into registers
-// while the present one is computed, and 8-bit caches become 16-bit on the way.
+// the caches near the cores: the matrix units bound it, and beside them the
+// exponentials and what else is done to each score.  The rows of one key-value
+// head are its query heads of all new tokens (row = token * group + head of the
+// group), so that heads which share keys share a workgroup's key tiles too.  A
+// wave has 32 rows and walks over tiles of 64 keys (32 for heads wider than
+// 128) in LDS:
 //
 //   scores^T [keys][rows] = K Q^T      Q stays in registers, K as it stands in LDS
 //   out^T [dims][rows] += V^T P^T      V^T by LDS reads that transpose
@@ -16,12 +16,20 @@
 // + i % 4; eight of them, in that order, are the second product's P^T operand,
 // so weights never leave their lane, and a row's maximum is one exchange between
 // two lanes.  The running reference is decode.hip's.
+//
+// A workgroup has eight waves in two groups of four, one of each group on a
+// SIMD, a barrier apart: while one wave multiplies, the other one turns its
+// scores into weights and puts the next tile into LDS.  The tile's pieces wait
+// in registers meanwhile, and 8-bit caches become 16-bit on the way.
+//
+// One prompt of 8192 tokens, 32 heads over 8 of 128, bf16: 640 us, 860 TFLOP/s of
+// the 1360 that a large matrix product reaches; by workgroups of four waves 890.
 #include "paged.hpp"
 
 namespace mfh {
 namespace {
 
-// Waves of a workgroup, 32 rows each: two a SIMD where their registers allow it.
+// Waves of a workgroup, 32 rows each, where rows fill the card: two a SIMD if their registers allow it.
 constexpr int waves_of(int dim) { return dim <= 128 ? 8 : 4; }
 constexpr int keys_of(int dim) { return dim <= 128 ? 64 : 32; }  // of a tile
 constexpr float kStep = 8.0f;       // the reference moves where a score passes it by 2^kStep
@@ -75,11 +83,11 @@ MFH_DEV int place(int row, int piece)
     return piece ^ (((row & 3) << 2 | (row >> 2 & 3)) & (PIECES - 1));
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.
-template <int DT, bool FP8, int DP>
-__global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefill(PrefillArgs a)
+// DP: head_dim rounded up to 64, 128 or 256.  WAVES: 4 (one group) or 8.
+template <int DT, bool FP8, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a)
 {
-    constexpr int kWaves = waves_of(DP), kThreads = 64 * kWaves, kRows = 32 * kWaves;
+    constexpr int kWaves = WAVES, kThreads = 64 * kWaves, kRows = 32 * kWaves;
     constexpr int kBytes = FP8 ? 1 : 2;
     constexpr int kSteps = DP / 16;
     constexpr int kDimTiles = DP / 32;
@@ -139,7 +147,6 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
     const bool real = row < rows;
     const mfh_u32 token = a.by_group.quotient(min(row, rows - 1)), head = kv * a.group + (min(row, rows - 1) - token * a.group);
     const int position = first_position + (int)token;
-    const bool wave_real = row0 + 32 * wave < rows;
     const mfh_u32 wave_row0 = min(row0 + 32 * wave, rows - 1), wave_row1 = min(row0 + 32 * wave + 31, rows - 1);
     const int wave_low = first_position + (int)a.by_group.quotient(wave_row0);
     const int wave_high = first_position + (int)a.by_group.quotient(wave_row1);
@@ -339,8 +346,8 @@ __global__ __launch_bounds__(64 * waves_of(DP), DP <= 128 ? 2 : 1) void k_prefil
     const bool optional = a.cap_scaled != 0.0f || a.slopes || !(a.scale > 0.0f);
     auto soften = [&](const Tile& w, auto plain) {
         const int key_first = w.index * kKeys;
-        const bool all = w.open || clean && key_first + kKeys <= length && ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
-                                             key_first + kKeys <= prefix);
+        const bool all = w.open || (clean && key_first + kKeys <= length && ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
+                                             key_first + kKeys <= prefix));
         float scale = a.scale;  // what is left to multiply by
         if (!plain.value || optional) {
             // a row's position is below the length
@@ -581,10 +588,23 @@ __global__ __launch_bounds__(256) void k_prefill_join(PrefillArgs a, int request
     if (dim == 0 && a.lse) a.lse[row] = all == 0.0f ? -INFINITY : top * kLn2 + logf(all);
 }
 
-// Workgroups of a call at most, and the parts that a row's keys are split into:
-// where the rows do not fill the card, as many as do, of eight tiles at least.
-// (256 workgroups for 256 CUs: 302 us whole, 340 us in two parts.)
+// Workgroups of a call at most, their waves, and the parts that a row's keys are
+// split into: where the rows do not fill the card, as many as do, of eight tiles
+// at least.  (256 workgroups for 256 CUs: 302 us whole, 340 us in two parts.)
+//
+// Workgroups of four waves have no second group to work beside them, load every
+// tile for half the rows, and are more in number.  Heads of 128, 8 of them, bf16,
+// four waves and eight:
+//   rows of a request's head that four waves hold    8 requests, 16 tokens over 2000     35 us  39 us
+//   a few tiles, most of it the beginning and end    64 requests of 128 tokens          153    164
+//   under 25 tiles and no eight waves for every CU   1 request of 1500 tokens            59     69
+//   under 49 tiles and the fours fill most CUs       2 requests, 512 tokens over 2000    81     96
+// and where none of this holds                       1 request of 2048 tokens            88     76
+//                                                    2 requests of 1500 tokens          117     81
+//                                                    8 requests, 40 tokens over 2000     65     45
+//                                                    2 requests, 512 tokens over 16000  420    371
 struct Layout {
+    int waves;
     int64_t row_tiles;
     __int128 blocks;  // of one part
     mfh_u32 parts;
@@ -595,25 +615,37 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
               int64_t most_fresh, int64_t longest)
 {
     Layout l{};
-    const int rows = 32 * waves_of(c.head_dim), group = sh.q_heads / c.kv_heads;
+    const int group = sh.q_heads / c.kv_heads;
     most_fresh = std::min(most_fresh, tokens);
-    l.row_tiles = (most_fresh * group + rows - 1) / rows;
-    l.blocks = (__int128)l.row_tiles * c.kv_heads * requests;
-    const int64_t tiles = std::min<int64_t>(std::max<int64_t>(longest, 1), kLongest) / keys_of(c.head_dim);
+    auto with_waves = [&](int waves) {
+        l.waves = waves;
+        l.row_tiles = (most_fresh * group + 32 * waves - 1) / (32 * waves);
+        l.blocks = (__int128)l.row_tiles * c.kv_heads * requests;
+    };
     // those that find rows, whatever the requests' sizes
-    const __int128 busy = std::min<__int128>(l.blocks, ((__int128)tokens * group / rows + requests) * c.kv_heads);
-    const int64_t wanted = busy > 0 ? (int64_t)(3 * dev->compute_units / (2 * busy)) : 1;
+    auto busy = [&]() {
+        return std::min<__int128>(l.blocks, ((__int128)tokens * group / (32 * l.waves) + requests) * c.kv_heads);
+    };
+    const int64_t tiles = std::min<int64_t>(std::max<int64_t>(longest, 1), kLongest) / keys_of(c.head_dim);
+    with_waves(waves_of(c.head_dim));
+    const int cus = dev->compute_units;
+    if (most_fresh * group <= 128 || tiles <= 4 || (tiles <= 24 && busy() < cus) ||
+        (tiles <= 48 && busy() > cus / 4 && busy() <= cus / 2))
+        with_waves(4);
+    const int64_t wanted = busy() > 0 ? (int64_t)(3 * cus / (2 * busy())) : 1;
     l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / 8, 64}));
     l.bytes = l.parts > 1 ? (size_t)tokens * sh.q_heads * l.parts * (c.head_dim + 2) * sizeof(float) : 0;
     return l;
 }
 
 template <int DT, bool FP8>
-void launch_dims(int dim, unsigned grid, hipStream_t s, const PrefillArgs& a)
+void launch_dims(int dim, int waves, unsigned grid, hipStream_t s, const PrefillArgs& a)
 {
-    if (dim <= 64) k_prefill<DT, FP8, 64><<<grid, 64 * waves_of(64), 0, s>>>(a);
-    else if (dim <= 128) k_prefill<DT, FP8, 128><<<grid, 64 * waves_of(128), 0, s>>>(a);
-    else k_prefill<DT, FP8, 256><<<grid, 64 * waves_of(256), 0, s>>>(a);
+    if (dim > 128) k_prefill<DT, FP8, 256, 4><<<grid, 256, 0, s>>>(a);
+    else if (waves == 4 && dim <= 64) k_prefill<DT, FP8, 64, 4><<<grid, 256, 0, s>>>(a);
+    else if (waves == 4) k_prefill<DT, FP8, 128, 4><<<grid, 256, 0, s>>>(a);
+    else if (dim <= 64) k_prefill<DT, FP8, 64, 8><<<grid, 512, 0, s>>>(a);
+    else k_prefill<DT, FP8, 128, 8><<<grid, 512, 0, s>>>(a);
 }
 
 }  // namespace
@@ -630,8 +662,9 @@ int mfh_paged_prefill_workspace(const mfh_attention_shape* shape, const mfh_kv_c
     const Device* dev;
     MFH_TRY(bind_device(&dev));
     MFH_TRY(check_attention(shape, cache, what));
-    if (requests < 0 || tokens < 0 || most_fresh < 0)
-        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: negative number of requests or tokens", what);
+    if (requests < 0 || tokens < 0 || most_fresh < 0 || tokens > kLongest)
+        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests, %lld tokens, %lld of one at most", what, requests,
+                    (long long)tokens, (long long)most_fresh);
     if (!bytes) return fail(MFH_ERR_INVALID_ARGUMENT, "%s: NULL result", what);
     *bytes = layout(dev, *shape, *cache, requests, tokens, most_fresh, longest).bytes;
     return MFH_OK;
@@ -680,7 +713,7 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     Layout l = layout(dev, *shape, *cache, requests, tokens, most_fresh, std::min<int64_t>(longest, (int64_t)table_width * cache->page_size));
     if (l.bytes > workspace_bytes || tokens * shape->q_heads > kLongest) l.parts = 1;
     const __int128 grid = l.blocks * l.parts;
-    if (a.most_fresh * a.group > kLongest || grid >= ((int64_t)1 << 32) / (64 * waves_of(a.dim)))
+    if (a.most_fresh * a.group > kLongest || grid >= ((int64_t)1 << 32) / (64 * l.waves))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %lld tokens and %d heads are too many for one call",
                     what, requests, (long long)a.most_fresh, shape->q_heads);
     a.row_tiles = (mfh_u32)l.row_tiles;
@@ -695,11 +728,11 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     hipStream_t s = (hipStream_t)stream;
     const bool fp8 = cache->dtype == kF8E4M3;
     if (shape->dtype == kBFloat16) {
-        if (fp8) launch_dims<kBFloat16, true>(a.dim, (unsigned)grid, s, a);
-        else launch_dims<kBFloat16, false>(a.dim, (unsigned)grid, s, a);
+        if (fp8) launch_dims<kBFloat16, true>(a.dim, l.waves, (unsigned)grid, s, a);
+        else launch_dims<kBFloat16, false>(a.dim, l.waves, (unsigned)grid, s, a);
     } else {
-        if (fp8) launch_dims<kFloat16, true>(a.dim, (unsigned)grid, s, a);
-        else launch_dims<kFloat16, false>(a.dim, (unsigned)grid, s, a);
+        if (fp8) launch_dims<kFloat16, true>(a.dim, l.waves, (unsigned)grid, s, a);
+        else launch_dims<kFloat16, false>(a.dim, l.waves, (unsigned)grid, s, a);
     }
     MFH_TRY(launch_status("k_prefill"));
     if (l.parts > 1) {

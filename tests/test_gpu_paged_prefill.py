@@ -186,6 +186,57 @@ def test_few_rows_over_a_long_context(hq, hk, dim):
     assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+# A large bound of the lengths: workgroups of eight waves, whole and in parts.
+@pytest.mark.parametrize("dtype, cache", [(BF16, BF16), (F16, F16), (BF16, FP8), (F16, FP8)])
+@pytest.mark.parametrize("hq, hk, dim, page, order", [(4, 1, 128, 16, "head"), (3, 1, 64, 1, "token"), (6, 2, 80, 7, "head"), (2, 1, 112, 256, "token")])
+def test_a_large_bound_of_the_lengths(dtype, cache, hq, hk, dim, page, order):
+    c = Chunk(dtype, cache, MIXED + [(900, 40)], hq, hk, dim, page, order, seed=dim + page, q_std=2.0)
+    for workspace in (False, True):
+        c.check(*c.run(longest=10 ** 9, workspace=workspace))
+
+
+@pytest.mark.parametrize("option", [dict(window=1), dict(window=70), dict(slopes=True), dict(prefix=PREFIX), dict(prefix=PREFIX, window=66, slopes=True, softcap=8.0),
+                                    dict(scale=-0.3)])
+@pytest.mark.parametrize("page, dim", [(16, 128), (10, 64)])
+def test_masks_cap_and_bias_under_a_large_bound(option, page, dim):
+    c = Chunk(BF16, BF16, MIXED, 4, 2, dim, page, seed=5, q_std=3.0, **dict(option))
+    for workspace in (False, True):
+        c.check(*c.run(longest=10 ** 9, workspace=workspace))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_masked_places_under_a_large_bound(dim):
+    def chunk():
+        return Chunk(F16, F16, [(300, 180)], 2, 1, dim, 16, seed=4)
+
+    c = chunk()
+    clean, lse_clean = c.run(longest=10 ** 9)
+    c.check(clean, lse_clean)
+    for t, value in ((330, math.inf), (400, math.nan), (470, -math.inf)):
+        c.cache.views[1][int(c.table[0, t // 16]), t % 16, 0, 7] = value
+    for workspace in (False, True):
+        out, lse = c.run(longest=10 ** 9, workspace=workspace)
+        others = torch.arange(dim) != 7
+        check_attention(out[:, :, others], lse, [x[:, :, others] if x.ndim == 3 else x for x in c.oracle()], F16, dim)
+        assert torch.isfinite(out[:30, :, 7]).all() and (out[30:100, :, 7] == math.inf).all() and torch.isnan(out[100:, :, 7]).all()
+    c = chunk()
+    c.cache.views[0][int(c.table[0, 25]), 2, 0, 9] = math.nan  # a key: token 402
+    out, lse = c.run(longest=10 ** 9)
+    assert torch.equal(out[:102], clean[:102]) and torch.equal(lse[:102], lse_clean[:102]) and torch.isnan(out[102:]).all()
+
+
+def test_a_page_outside_the_cache_under_a_large_bound():
+    c = Chunk(BF16, BF16, [(0, 200)], 1, 1, 64, 16, seed=9)
+    c.table[0, 1], c.table[0, 10] = 10 ** 6, -1
+    k, v = c.kv[0]
+    keep = torch.cat([torch.arange(16), torch.arange(32, 160), torch.arange(176, 200)])
+    for workspace in (False, True):
+        out, lse = c.run(longest=10 ** 9, workspace=workspace)
+        for i in (0, 15, 16, 31, 32, 127, 128, 159, 160, 175, 176, 199):
+            seen = keep[keep <= i]
+            check_attention(out[i: i + 1], lse[i: i + 1], attention_oracle(c.q[i: i + 1].double(), k[seen], v[seen], [10 ** 6], c.scale), BF16, 64)
+
+
 def test_large_scores_and_the_moving_reference():
     c = Chunk(F16, F16, [(0, 300)], 2, 1, 64, 16, seed=3, slopes=True)
     c.slopes = torch.tensor([3.0, -3.0])
