@@ -589,20 +589,27 @@ __global__ __launch_bounds__(256) void k_prefill_join(PrefillArgs a, int request
 }
 
 // Workgroups of a call at most, their waves, and the parts that a row's keys are
-// split into: where the rows do not fill the card, as many as do, of eight tiles
-// at least.  (256 workgroups for 256 CUs: 302 us whole, 340 us in two parts.)
+// split into.
+//
+// A CU holds one workgroup (of heads of 64 two).  Rows that do not fill the card
+// are split into as many parts as fit it at once, of eight tiles at least: 4
+// tokens over 32000 keys, 8 heads of 128 with 4 queries each, 32 parts 62 us, 48
+// parts 93 us, for half of them have to wait; 3 requests of 512 tokens over 2000
+// (192 workgroups) whole 103 us, in two parts 131.  Where workgroups differ in
+// their work, for requests differ in their new tokens or a request's first rows
+// see much less than its last, half as many parts again even it out: 4 requests
+// of up to 512 tokens over up to 7000 in two parts 171 us, whole 280; a prompt of
+// 3000, 4 heads of 64, 60 and 74.
 //
 // Workgroups of four waves have no second group to work beside them, load every
-// tile for half the rows, and are more in number.  Heads of 128, 8 of them, bf16,
-// four waves and eight:
-//   rows of a request's head that four waves hold    8 requests, 16 tokens over 2000     35 us  39 us
-//   a few tiles, most of it the beginning and end    64 requests of 128 tokens          153    164
-//   under 25 tiles and no eight waves for every CU   1 request of 1500 tokens            59     69
-//   under 49 tiles and the fours fill most CUs       2 requests, 512 tokens over 2000    81     96
-// and where none of this holds                       1 request of 2048 tokens            88     76
-//                                                    2 requests of 1500 tokens          117     81
-//                                                    8 requests, 40 tokens over 2000     65     45
-//                                                    2 requests, 512 tokens over 16000  420    371
+// tile for half the rows, and are more in number.  8 heads of 128, 4 queries
+// each, bf16, four waves and eight:
+//   rows of a request's head that four waves hold   8 requests, 16 tokens over 2000      36 us  39 us
+//   a few tiles, most of it beginning and end       64 requests of 128 tokens           154    163
+//   under 25 tiles and no eight waves for every CU  1 request of 512 tokens              26     31
+// and where none of this holds                      1 request of 2048 tokens             92     81
+//                                                   2 requests of 1500 tokens           117     81
+//                                                   2 requests, 512 tokens over 16000   413    331
 struct Layout {
     int waves;
     int64_t row_tiles;
@@ -629,10 +636,9 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     const int64_t tiles = std::min<int64_t>(std::max<int64_t>(longest, 1), kLongest) / keys_of(c.head_dim);
     with_waves(waves_of(c.head_dim));
     const int cus = dev->compute_units;
-    if (most_fresh * group <= 128 || tiles <= 4 || (tiles <= 24 && busy() < cus) ||
-        (tiles <= 48 && busy() > cus / 4 && busy() <= cus / 2))
-        with_waves(4);
-    const int64_t wanted = busy() > 0 ? (int64_t)(3 * cus / (2 * busy())) : 1;
+    if (most_fresh * group <= 128 || tiles <= 4 || (tiles <= 24 && busy() < cus)) with_waves(4);
+    const bool uneven = 4 * (__int128)tokens < 3 * (__int128)most_fresh * requests || most_fresh > longest / 2;
+    const int64_t wanted = busy() > 0 ? (int64_t)((uneven ? 3 * cus : 2 * cus) / (2 * busy())) : 1;
     l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / 8, 64}));
     l.bytes = l.parts > 1 ? (size_t)tokens * sh.q_heads * l.parts * (c.head_dim + 2) * sizeof(float) : 0;
     return l;
