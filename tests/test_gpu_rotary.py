@@ -86,6 +86,20 @@ def test_in_place_and_strided_slices_of_a_fused_projection(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype, hq, hk, dim, rot", [(BF16, 40, 9, 256, 192), (F32, 33, 1, 96, 96), (F16, 71, 8, 34, 10)])
+def test_more_heads_than_a_workgroup_turns_at_once(dtype, hq, hk, dim, rot, interleaved):
+    M.init(0)
+    gen = torch.Generator().manual_seed(hq)
+    q, k = (torch.randn(3, h, dim, generator=gen).to(TORCH[dtype]) for h in (hq, hk))
+    positions, freqs = torch.tensor([0, 77, 40000], dtype=torch.int32), A.rotary_frequencies(rot)
+    qd, kd, pd, f = q.cuda(), k.cuda(), positions.cuda(), torch.tensor(freqs, dtype=torch.float64).cuda()
+    A.rotary(A.Rotary(dtype, hq, hk, dim, rot, interleaved=interleaved), 3, ptr(qd), ptr(qd), ptr(kd), ptr(kd), ptr(pd), ptr(f), stream=stream())
+    for got, x in ((qd, q), (kd, k)):
+        near(got, *turned(x.double(), positions, freqs, rot, interleaved), dtype)
+
+
+@gpu
 def test_the_inverse_is_the_gradient():
     # <g, d turn(x) / dx> by differences of the turn itself (it is linear: exact but for rounding), and turn(inverse(x)) = x
     M.init(0)
