@@ -99,8 +99,8 @@ struct DecodeArgs {
     float scale, cap_twice, cap_scaled, v_scale;
     int32_t window, requests, kv_heads, q_heads, group, head_groups, dim, part_heads;
     mfh_u32 request_rows;  // kv_heads * head_groups
-    mfh_u32 blocks;        // of the split form
-    Divider by_head_groups, by_request_rows, by_blocks, by_q_heads;
+    mfh_u32 blocks, uneven;  // of the split form, where requests are alike and where not
+    Divider by_head_groups, by_request_rows, by_blocks, by_uneven, by_q_heads;
 };
 
 MFH_DEV mfh_u32 low_halves(mfh_u32 a, mfh_u32 b) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
@@ -119,7 +119,7 @@ struct Context {
     }
 };
 
-// The split form: all rows' tiles go to `blocks` workgroups, a piece each; a
+// The split form: all rows' tiles go to `blocks` (or `uneven`) workgroups, a piece each; a
 // row's pieces are its own, of equal size, so that there are `rows` workgroups
 // more at most.  Short rows end early and make room for the next workgroup.
 // The host takes this form only where the number of all tiles fits 31 bits.
@@ -127,10 +127,15 @@ MFH_DEV mfh_u32 lane_tiles(const DecodeArgs& a, mfh_u32 r) { return r < (mfh_u32
 
 MFH_DEV mfh_u32 piece_of(const DecodeArgs& a, int lane)
 {
-    mfh_u32 sum = 0;
-    for (mfh_u32 base = 0; base < (mfh_u32)a.requests; base += 64) sum += lane_tiles(a, base + lane);
-    const mfh_u32 total = last_lane(lanes_upto(sum)) * a.request_rows;
-    return max(a.by_blocks.quotient(total + a.blocks - 1), (mfh_u32)kWaves);
+    mfh_u32 sum = 0, most = 0;
+    for (mfh_u32 base = 0; base < (mfh_u32)a.requests; base += 64) {
+        const mfh_u32 tiles = lane_tiles(a, base + lane);
+        sum += tiles, most = max(most, tiles);
+    }
+    const mfh_u32 all = last_lane(lanes_upto(sum)), total = all * a.request_rows;
+    const bool uneven = __any((mfh_u64)most * (mfh_u32)a.requests * 4 > (mfh_u64)all * 5);
+    const mfh_u32 piece = uneven ? a.by_uneven.quotient(total + a.uneven - 1) : a.by_blocks.quotient(total + a.blocks - 1);
+    return max(piece, (mfh_u32)kWaves);
 }
 
 MFH_DEV mfh_u32 parts_of(mfh_u32 tiles, mfh_u32 piece) { return (tiles + piece - 1) / piece; }
@@ -582,7 +587,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_decode_join(DecodeArgs a)
 struct Layout {
     bool split;
     int64_t rows;
-    mfh_u32 blocks;
+    mfh_u32 blocks, uneven;  // workgroups aimed at
     int part_heads;
     size_t bytes;
 };
@@ -593,7 +598,11 @@ struct Layout {
 // and where lengths may differ much, the split wins: 8 rows of 2048 tokens 28.6
 // and 12.6 us, 512 rows of 1..4096 74 and 44.  The split aims at one workgroup
 // per CU: two come out slower at 256 dims (33.5 us, 39.7) and for 64 rows
-// (14.9, 15.8), and equal or 8% faster elsewhere.
+// (14.9, 15.8), and equal or 8% faster elsewhere.  Where requests differ in length
+// by so much that the longest is a quarter over the mean, which only the device
+// knows, a row's last cut leaves much uneven, and half as many workgroups again
+// even it out: 48 rows of 1..16384, e4m3, 33.5 us and 38, the same in bf16 47 and
+// 57; 128 rows of 1..3000 73.6 and 76.8 (rows of 256 dims 19.1 and 18.6).
 Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cache& c, int32_t requests, int64_t longest)
 {
     Layout l{};
@@ -601,16 +610,16 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     l.rows = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads);
     l.part_heads = std::min(group, kHeads);
     const int64_t tiles = (std::min<int64_t>(std::max<int64_t>(longest, 1), kLongest) + kTile - 1) / kTile;
-    l.blocks = (mfh_u32)dev->compute_units;
+    l.blocks = (mfh_u32)dev->compute_units, l.uneven = l.blocks + l.blocks / 2;
     l.split = tiles > (l.rows >= dev->compute_units ? 32 : 16);
-    l.bytes = l.split ? (size_t)(l.blocks + l.rows) * l.part_heads * (c.head_dim + 2) * sizeof(float) : 0;
+    l.bytes = l.split ? (size_t)(l.uneven + l.rows) * l.part_heads * (c.head_dim + 2) * sizeof(float) : 0;
     return l;
 }
 
 template <int DT, bool FP8, int DP, bool FAST>
 void launch_form(const Layout& l, hipStream_t s, const DecodeArgs& a)
 {
-    if (l.split) k_decode<DT, FP8, DP, FAST, true><<<(unsigned)(l.blocks + l.rows), kThreads, 0, s>>>(a);
+    if (l.split) k_decode<DT, FP8, DP, FAST, true><<<(unsigned)(l.uneven + l.rows), kThreads, 0, s>>>(a);
     else k_decode<DT, FP8, DP, FAST, false><<<(unsigned)l.rows, kThreads, 0, s>>>(a);
 }
 
@@ -691,17 +700,17 @@ int mfh_paged_decode(const mfh_attention_shape* shape, const mfh_kv_cache* cache
     const int64_t most = std::min<int64_t>((int64_t)table_width * cache->page_size, kLongest) / kTile + 1;
     if (l.bytes > workspace_bytes || l.rows * most > kLongest || (int64_t)requests * shape->q_heads > (1 << 22))
         l.split = false;
-    if (l.rows + l.blocks >= (int64_t(1) << 32) / kThreads)
+    if (l.rows + l.uneven >= (int64_t(1) << 32) / kThreads)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %d heads are too many for one call", what, requests,
                     shape->q_heads);
-    a.blocks = l.blocks;
+    a.blocks = l.blocks, a.uneven = l.uneven;
     a.part_heads = l.part_heads;
     if (l.split) {
         a.part_out = (float*)workspace;
-        a.part_sum = (float2*)(a.part_out + (l.blocks + l.rows) * l.part_heads * a.dim);
+        a.part_sum = (float2*)(a.part_out + (l.uneven + l.rows) * l.part_heads * a.dim);
     }
     a.by_head_groups = Divider((mfh_u32)a.head_groups), a.by_request_rows = Divider(a.request_rows);
-    a.by_blocks = Divider(l.blocks), a.by_q_heads = Divider((mfh_u32)a.q_heads);
+    a.by_blocks = Divider(l.blocks), a.by_uneven = Divider(l.uneven), a.by_q_heads = Divider((mfh_u32)a.q_heads);
     hipStream_t s = (hipStream_t)stream;
     // whole groups of 16 tokens, and dwords for buffer loads
     const bool fast = cache->page_size % 16 == 0 &&

@@ -85,6 +85,13 @@ def test_window_cap_and_bias(option, page):
     s.check(*s.run())
 
 
+@pytest.mark.parametrize("cache", [F16, FP8])
+@pytest.mark.parametrize("lengths", [[2000] * 3, [1500, 1499, 1600, 1501], [1, 3000, 40, 600, 0, 90], [4000], [0] * 70 + [2500], [700] * 65])
+def test_requests_alike_and_not(lengths, cache):
+    s = Step(F16, cache, lengths, 4, 2, 64, 16, seed=len(lengths))
+    s.check(*s.run())
+
+
 @pytest.mark.parametrize("page", [16, 9])
 def test_parts_do_not_change_what_is_computed(page):
     # one request split as far as it goes, with any hint of the lengths, with little workspace and with none
