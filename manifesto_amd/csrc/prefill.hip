@@ -66,12 +66,13 @@ MFH_DEV u32x2 read_column(const char* at)
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at)));
 }
 
-// Whether a dword's halves are infinite or NaN.
+// The top bits of those halves of a dword that are infinite or NaN: an exponent
+// of ones carries into them.
 template <int DT>
-MFH_DEV bool not_finite(mfh_u32 pair)
+MFH_DEV mfh_u32 not_finite(mfh_u32 pair)
 {
-    constexpr mfh_u32 kExp = DT == kBFloat16 ? 0x7f80u : 0x7c00u;
-    return ((pair & kExp) == kExp) | ((pair & kExp << 16) == kExp << 16);
+    constexpr mfh_u32 kExponents = DT == kBFloat16 ? 0x7f807f80u : 0x7c007c00u, kOnes = DT == kBFloat16 ? 0x00800080u : 0x04000400u;
+    return ((pair & kExponents) + kOnes) & 0x80008000u;
 }
 
 // Where 16 bytes of a row stand among the row's pieces in LDS.  Rows have no
@@ -258,11 +259,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             }
             if (!plain.value && aside && !w.open) {
                 *reinterpret_cast<u32x4*>(aside + key * kPitch + slot * 16) = x;
+                mfh_u32 tops[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const bool lo = not_finite<DT>(x[j] & 0xffffu), hi = not_finite<DT>(x[j] >> 16);
-                    odd |= lo | hi;
-                    x[j] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                for (int j = 0; j < 4; j++) tops[j] = not_finite<DT>(x[j]);
+                if ((tops[0] | tops[1] | tops[2] | tops[3]) != 0) {
+                    odd = true;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[j] &= ~(tops[j] | (tops[j] - (tops[j] >> 15)));  // whole halves
                 }
             }
             *reinterpret_cast<u32x4*>(to + key * kPitch + slot * 16) = x;
@@ -292,7 +295,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
                 for (int i = 0; i < 16; i++) {
                     const int dim = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
                     const mfh_u32 v = *reinterpret_cast<const mfh_u16*>(aside + key * kPitch + place<kPieces>(key, dim / 8) * 16 + dim % 8 * 2);
-                    if (see & not_finite<DT>(v)) acc[d][i] += dec16<DT>(v);
+                    if (see & (not_finite<DT>(v) != 0)) acc[d][i] += dec16<DT>(v);
                 }
             }
         }
