@@ -22,8 +22,8 @@
 // scores into weights and puts the next tile into LDS.  The tile's pieces wait
 // in registers meanwhile, and 8-bit caches become 16-bit on the way.
 //
-// One prompt of 8192 tokens, 32 heads over 8 of 128, bf16: 590 to 650 us from card
-// to card, 850 to 930 TFLOP/s of the 1360 that a large matrix product reaches; by
+// One prompt of 8192 tokens, 32 heads over 8 of 128, bf16: 575 to 650 us from card
+// to card, 850 to 956 TFLOP/s of the 1360 that a large matrix product reaches; by
 // workgroups of four waves 890 us.
 #include "paged.hpp"
 
