@@ -456,27 +456,30 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             else go_to(keys, to);
             ask(keys);
         };
-        go_to(keys, tile0);
+        // (the second tile's K sets out with the first tile)
+        const int second = follow(tile0);
+        Raw second_raw[kLoads];
+        Keys first_keys;
+        go_to(first_keys, tile0);
+        go_to(keys, second);
+        ask(first_keys);
         ask(keys);
-        locate(keys, from);
+        locate(first_keys, from);
         fetch(from, k_base, k_raw);
         fetch(from, v_base, v_raw);
+        locate(keys, from);
+        if (second < tile_end) fetch(from, k_base, second_raw);
         // Keys of a page that is not one of the cache's are masked, and nothing
         // takes the short ways then.
         bool bad = false;
         for (mfh_u32 i = threadIdx.x; i <= last_entry; i += kThreads) bad |= (mfh_u32)table[i] >= a.pages.pages;
         clean = !__syncthreads_or(bad);
-        Tile now = describe(tile0), next = describe(follow(tile0)), after = describe(follow(next.index)), before = now;
+        Tile now = describe(tile0), next = describe(second), after = describe(follow(next.index)), before = now;
         if (threadIdx.x < 3) s_odd[threadIdx.x] = -1;
         for (int i = threadIdx.x * 16; i < kKeys * kPitch; i += kThreads * 16) *reinterpret_cast<u32x4*>(s_v[2] + i) = u32x4{0, 0, 0, 0};
-        move(tile0, next.index);
         put(now, std::false_type{}, s_k[0], nullptr, k_raw);
         const bool odd0 = put(now, std::false_type{}, s_v[0], s_raw[0], v_raw);
-        locate(keys, from);
-        if (next.index < tile_end) {
-            fetch(from, k_base, k_raw);
-            put(next, std::false_type{}, s_k[1], nullptr, k_raw);
-        }
+        if (second < tile_end) put(next, std::false_type{}, s_k[1], nullptr, second_raw);
         move(next.index, after.index);
 #pragma unroll
         for (int j = 0; j < 2 * kBlocks; j++) p[j] = u32x4{0, 0, 0, 0};

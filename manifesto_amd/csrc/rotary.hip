@@ -8,9 +8,9 @@
 // parts allow it): E pairs of one head, or elements that are only copied (the
 // head behind rotary_dim, and values).  While these are on their way they
 // compute the tokens' cosines and sines, each once for all heads, into LDS.
-// 8192 tokens of 32 + 8 + 8 heads of 128, bf16 into a cache of e4m3: 62 us,
-// 5.9 TB/s; with the two pieces of whole pairs side by side, so that a load of
-// the wave has gaps, and the loads behind the angles, 83 us.
+// 16381 tokens of 32 + 8 + 8 heads of 128, half of each turned, bf16 into a cache
+// of e4m3: 62 us, 5.9 TB/s; with the two pieces of whole pairs side by side, so
+// that a load of the wave has gaps, and the loads behind the angles, 83 us.
 //
 // The phase position * frequency is reduced to one turn in f64: at position
 // 2^24 its error is below 2^-28 of a turn, under the step of the f32 phase that
@@ -304,8 +304,8 @@ int launch(const mfh_rotary_shape& sh, RotaryArgs a, int cache, hipStream_t s)
     a.k_units = a.q_units + (a.k ? (mfh_u32)sh.kv_heads * a.units_per_head : 0);
     a.units = a.k_units + (a.v ? (mfh_u32)sh.kv_heads * a.units_per_head : 0);
     if (a.units == 0) return MFH_OK;
-    // One unit a thread, or one token where that is more: 62 us for 8192 tokens of 32 + 8 + 8
-    // heads of 128, bf16 into a cache of e4m3; with 2, 3 or 4 units in flight 66.
+    // One unit a thread, or one token where that is more: 62 us for 16381 tokens of
+    // 32 + 8 + 8 heads of 128, bf16 into a cache of e4m3; with 2, 3 or 4 units in flight 66.
     int64_t per = std::max<int64_t>(1, kThreads / a.units);
     if (half) per = std::min<int64_t>(per, kMaxPairs / half);
     a.tokens_per_block = (int32_t)std::max<int64_t>(1, per);
