@@ -614,14 +614,17 @@ __global__ __launch_bounds__(256) void k_prefill_join(PrefillArgs a, int request
 // split into.
 //
 // A CU holds one workgroup (of heads of 64 two).  Rows that do not fill the card
-// are split into as many parts as fit it at once, of eight tiles at least: 4
-// tokens over 32000 keys, 8 heads of 128 with 4 queries each, 32 parts 62 us, 48
-// parts 93 us, for half of them have to wait; 3 requests of 512 tokens over 2000
-// (192 workgroups) whole 103 us, in two parts 131.  Where workgroups differ in
-// their work, for requests differ in their new tokens or a request's first rows
-// see much less than its last, half as many parts again even it out: 4 requests
-// of up to 512 tokens over up to 7000 in two parts 171 us, whole 280; a prompt of
-// 3000, 4 heads of 64, 60 and 74.
+// are split into as many parts as fit it at once: 4 tokens over 32000 keys, 8
+// heads of 128 with 4 queries each, 32 parts 62 us, 48 parts 93 us, for half of
+// them have to wait.  A part has eight tiles at least, or four where the join has
+// little to do, at most 48 rows a CU: 8 requests, 4 tokens over 1000, whole 36.6
+// us, in three parts 25.9; a prompt of 512, which is 64 rows a CU, whole 25.3 us,
+// in two parts 29.4.  Rows that nearly fill the card stay whole: 3 requests of 512
+// tokens over 2000 (192 workgroups) 103 us, in two parts 131.  Where workgroups
+// differ in their work, for requests differ in their new tokens or a request's
+// first rows see much less than its last, half as many parts again even it out: 4
+// requests of up to 512 tokens over up to 7000 in two parts 171 us, whole 280; a
+// prompt of 3000, 4 heads of 64, 60 and 74.
 //
 // Workgroups of four waves have no second group to work beside them, load every
 // tile for half the rows, and are more in number.  8 heads of 128, 4 queries
@@ -661,7 +664,7 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     if (most_fresh * group <= 128 || tiles <= 4 || (tiles <= 24 && busy() < cus)) with_waves(4);
     const bool uneven = 4 * (__int128)tokens < 3 * (__int128)most_fresh * requests || most_fresh > longest / 2;
     const int64_t wanted = busy() > 0 ? (int64_t)((uneven ? 3 * cus : 2 * cus) / (2 * busy())) : 1;
-    l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / 8, 64}));
+    l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / (tokens * sh.q_heads <= 48 * cus ? 4 : 8), 64}));
     l.bytes = l.parts > 1 ? (size_t)tokens * sh.q_heads * l.parts * (c.head_dim + 2) * sizeof(float) : 0;
     return l;
 }
