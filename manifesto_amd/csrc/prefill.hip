@@ -742,7 +742,11 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     a.group = shape->q_heads / cache->kv_heads;
     a.dim = cache->head_dim;
     Layout l = layout(dev, *shape, *cache, requests, tokens, most_fresh, std::min<int64_t>(longest, (int64_t)table_width * cache->page_size));
-    if (l.bytes > workspace_bytes || tokens * shape->q_heads > kLongest) l.parts = 1;
+    if (tokens * shape->q_heads > kLongest) l.parts = 1;
+    if (l.parts > 1) {  // as many as there is room for
+        const size_t room = workspace_bytes / (l.bytes / l.parts);
+        l.parts = (mfh_u32)std::max<size_t>(1, std::min<size_t>(l.parts, room));
+    }
     const __int128 grid = l.blocks * l.parts;
     if (a.most_fresh * a.group > kLongest || grid >= ((int64_t)1 << 32) / (64 * l.waves))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %lld tokens and %d heads are too many for one call",

@@ -33,7 +33,7 @@ class Chunk:
         self.scale = option.pop("scale", dim ** -0.5)
         self.slopes = torch.rand(hq, generator=self.cache.gen) * 0.3 if option.pop("slopes", False) else None
 
-    def run(self, tokens=None, most=None, longest=None, workspace=True, shape=None, q=None, out=None, on=None):
+    def run(self, tokens=None, most=None, longest=None, workspace=True, share=1.0, shape=None, q=None, out=None, on=None):
         n, width = len(self.requests), self.table.shape[1] - 1
         shape = shape or A.Attention(self.dtype, self.hq, self.scale, **self.option)
         tokens = self.starts[-1] if tokens is None else tokens
@@ -46,6 +46,7 @@ class Chunk:
         out = torch.full((self.starts[-1], self.hq, self.dim), math.nan, dtype=TORCH[self.dtype], device="cuda") if out is None else out
         lse = torch.full((self.starts[-1], self.hq), math.nan, device="cuda")
         need = A.paged_prefill_workspace(shape, self.cache.desc, n, tokens, most, longest) if workspace else 0
+        need = int(need * share)
         ws = torch.full((max(need, 16),), 255, dtype=torch.uint8, device="cuda")
         torch.cuda.synchronize()
         A.paged_prefill(shape, self.cache.desc, n, tokens, most, ptr(q_), ptr(self.cache.buffers[0]), ptr(self.cache.buffers[1]), ptr(table), width,
@@ -235,6 +236,13 @@ def test_a_page_outside_the_cache_under_a_large_bound():
         for i in (0, 15, 16, 31, 32, 127, 128, 159, 160, 175, 176, 199):
             seen = keep[keep <= i]
             check_attention(out[i: i + 1], lse[i: i + 1], attention_oracle(c.q[i: i + 1].double(), k[seen], v[seen], [10 ** 6], c.scale), BF16, 64)
+
+
+@pytest.mark.parametrize("share", [0.03, 0.3, 0.5, 0.999])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_less_workspace_than_is_asked_for(share, dim):
+    c = Chunk(F16, F16, [(3000, 9), (700, 5)], 4, 2, dim, 16, seed=17)
+    c.check(*c.run(share=share))
 
 
 def test_large_scores_and_the_moving_reference():
