@@ -71,7 +71,8 @@ MFH_DEV u32x2 read_column(const char* at)
 template <int DT>
 MFH_DEV mfh_u32 not_finite(mfh_u32 pair)
 {
-    constexpr mfh_u32 kExponents = DT == kBFloat16 ? 0x7f807f80u : 0x7c007c00u, kOnes = DT == kBFloat16 ? 0x00800080u : 0x04000400u;
+    constexpr mfh_u32 kExponents = DT == kBFloat16 ? 0x7f807f80u : 0x7c007c00u;
+    constexpr mfh_u32 kOnes = DT == kBFloat16 ? 0x00800080u : 0x04000400u;
     return ((pair & kExponents) + kOnes) & 0x80008000u;
 }
 
@@ -121,7 +122,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     const mfh_u32 fresh = (mfh_u32)(end - begin), computed = (mfh_u32)min((int64_t)fresh, a.most_fresh);
     const mfh_u32 rows = computed * a.group, row0 = row_tile * kRows;
     if (row0 >= rows) return;
-    const int length = (int)min((mfh_u64)max(a.lengths[r], 0), min((mfh_u64)a.pages.width * a.pages.by_page.d, (mfh_u64)kLongest));
+    const mfh_u64 most = min((mfh_u64)a.pages.width * a.pages.by_page.d, (mfh_u64)kLongest);
+    const int length = (int)min((mfh_u64)max(a.lengths[r], 0), most);
     const int prefix = a.prefix ? min(max(a.prefix[r], 0), length) : 0;
     const int first_position = length - (int)fresh;  // of the request's new tokens; may be negative
 
@@ -147,7 +149,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     // This lane's row, and its wave's.
     const mfh_u32 row = row0 + 32 * wave + col;
     const bool real = row < rows;
-    const mfh_u32 token = a.by_group.quotient(min(row, rows - 1)), head = kv * a.group + (min(row, rows - 1) - token * a.group);
+    const mfh_u32 token = a.by_group.quotient(min(row, rows - 1));
+    const mfh_u32 head = kv * a.group + (min(row, rows - 1) - token * a.group);
     const int position = first_position + (int)token;
     const mfh_u32 wave_row0 = min(row0 + 32 * wave, rows - 1), wave_row1 = min(row0 + 32 * wave + 31, rows - 1);
     const int wave_low = first_position + (int)a.by_group.quotient(wave_row0);
@@ -218,8 +221,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     };
     auto describe = [&](int tile) {
         const int first = tile * kKeys;
-        return Tile{tile, clean && first + kKeys <= length && ((first + kKeys <= low_position + 1 && (a.window <= 0 || first > high_position - a.window)) ||
-                                                      first + kKeys <= prefix)};
+        const bool past = first + kKeys <= low_position + 1 && (a.window <= 0 || first > high_position - a.window);
+        return Tile{tile, clean && first + kKeys <= length && (past || first + kKeys <= prefix)};
     };
     // This thread's pieces of the tile.
     auto locate = [&](const Keys& keys, int64_t (&from)[kLoads]) {
@@ -227,7 +230,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         for (int i = 0; i < kLoads; i++) {
             const mfh_u32 page = (mfh_u32)keys.page[i] < a.pages.pages ? (mfh_u32)keys.page[i] : 0u;
             const int piece = place<kPieces>(key0 + i * kKeyStep, slot);
-            from[i] = (int64_t)((mfh_u64)page * (mfh_u64)a.pages.page_bytes) + (keys.in_page[i] + (piece * 8 < a.dim ? piece * 8 * kBytes : 0));
+            from[i] = (int64_t)((mfh_u64)page * (mfh_u64)a.pages.page_bytes) +
+                      (keys.in_page[i] + (piece * 8 < a.dim ? piece * 8 * kBytes : 0));
         }
     };
 
@@ -250,7 +254,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         for (int i = 0; i < kLoads; i++) {
             const int key = key0 + i * kKeyStep;
             u32x4 x;
-            if constexpr (FP8) x = u32x4{e4m3_pair<DT, false>(raw[i][0]), e4m3_pair<DT, true>(raw[i][0]), e4m3_pair<DT, false>(raw[i][1]), e4m3_pair<DT, true>(raw[i][1])};
+            if constexpr (FP8)
+                x = u32x4{e4m3_pair<DT, false>(raw[i][0]), e4m3_pair<DT, true>(raw[i][0]),
+                          e4m3_pair<DT, false>(raw[i][1]), e4m3_pair<DT, true>(raw[i][1])};
             else x = raw[i];
             if (!plain.value && (!w.open || a.dim != DP)) {
                 const bool keep = (place<kPieces>(key, slot) * 8 < a.dim) & there(w.index * kKeys + key);
@@ -288,13 +294,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     auto add_odd = [&](const char* aside, const Tile& w) {
         const Seen seen = seen_from(w.index * kKeys, 0);
         for (int key = 0; key < kKeys; key++) {
-            const bool see = there(w.index * kKeys + key) & (((key <= seen.back) & (key > seen.oldest)) | (key < seen.in_prefix));
+            const bool see = there(w.index * kKeys + key) &
+                             (((key <= seen.back) & (key > seen.oldest)) | (key < seen.in_prefix));
 #pragma unroll
             for (int d = 0; d < kDimTiles; d++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int dim = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-                    const mfh_u32 v = *reinterpret_cast<const mfh_u16*>(aside + key * kPitch + place<kPieces>(key, dim / 8) * 16 + dim % 8 * 2);
+                    const mfh_u32 v = *reinterpret_cast<const mfh_u16*>(
+                        aside + key * kPitch + place<kPieces>(key, dim / 8) * 16 + dim % 8 * 2);
                     if (see & (not_finite<DT>(v) != 0)) acc[d][i] += dec16<DT>(v);
                 }
             }
@@ -343,15 +351,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             read(n + kAhead);
             __builtin_amdgcn_sched_barrier(0);
             if (n < kScores) s[n % kBlocks] = mfma32<DT>(piece[n], q[n / kBlocks], s[n % kBlocks]);
-            else acc[(n - kScores) % kDimTiles] = mfma32<DT>(piece[n], p[(n - kScores) / kDimTiles], acc[(n - kScores) % kDimTiles]);
+            else acc[(n - kScores) % kDimTiles] =
+                mfma32<DT>(piece[n], p[(n - kScores) / kDimTiles], acc[(n - kScores) % kDimTiles]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     const bool whole = a.slopes || !(a.scale > 0.0f), optional = a.cap_scaled != 0.0f || whole;
     auto soften = [&](const Tile& w, auto plain) {
         const int key_first = w.index * kKeys;
-        const bool all = w.open || (clean && key_first + kKeys <= length && ((key_first + kKeys <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window)) ||
-                                             key_first + kKeys <= prefix));
+        const int key_behind = key_first + kKeys;
+        const bool past = key_behind <= wave_low + 1 && (a.window <= 0 || key_first > wave_high - a.window);
+        const bool all = w.open || (clean && key_behind <= length && (past || key_behind <= prefix));
         // What makes the scores of what s holds: s * scale + offset.  With a cap, s
         // becomes -1 / (1 + e^2y), whose double and 1 are tanh y: two operations for a
         // score fewer than tanh and the scale one after the other (a prompt of 8192,
@@ -368,7 +378,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) s[b][i] = -__builtin_amdgcn_rcpf(1.0f + exp2_fast(s[b][i] * a.cap_twice));
+                    for (int i = 0; i < 16; i++)
+                        s[b][i] = -__builtin_amdgcn_rcpf(1.0f + exp2_fast(s[b][i] * a.cap_twice));
                 scale = 2.0f * a.cap_scaled, offset = a.cap_scaled;
             }
             if (whole) {
@@ -384,12 +395,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
                 if (a.slopes) {
                     const float back = (float)seen.back;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) s[b][i] = __builtin_fmaf(-slope, fabsf(back - (float)(8 * (i / 4) + i % 4)), s[b][i]);
+                    for (int i = 0; i < 16; i++)
+                        s[b][i] = __builtin_fmaf(-slope, fabsf(back - (float)(8 * (i / 4) + i % 4)), s[b][i]);
                 }
                 if (!plain.value && !all) {
                     if (band) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) s[b][i] = (mfh_u32)(seen.back - (8 * (i / 4) + i % 4)) < width ? s[b][i] : -INFINITY;
+                        for (int i = 0; i < 16; i++) {
+                            const mfh_u32 distance = (mfh_u32)(seen.back - (8 * (i / 4) + i % 4));
+                            s[b][i] = distance < width ? s[b][i] : -INFINITY;
+                        }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; i++) s[b][i] = seen(8 * (i / 4) + i % 4) ? s[b][i] : -INFINITY;
@@ -476,7 +491,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         clean = !__syncthreads_or(bad);
         Tile now = describe(tile0), next = describe(second), after = describe(follow(next.index)), before = now;
         if (threadIdx.x < 3) s_odd[threadIdx.x] = -1;
-        for (int i = threadIdx.x * 16; i < kKeys * kPitch; i += kThreads * 16) *reinterpret_cast<u32x4*>(s_v[2] + i) = u32x4{0, 0, 0, 0};
+        for (int i = threadIdx.x * 16; i < kKeys * kPitch; i += kThreads * 16)
+            *reinterpret_cast<u32x4*>(s_v[2] + i) = u32x4{0, 0, 0, 0};
         put(now, std::false_type{}, s_k[0], nullptr, k_raw);
         const bool odd0 = put(now, std::false_type{}, s_v[0], s_raw[0], v_raw);
         if (second < tile_end) put(next, std::false_type{}, s_k[1], nullptr, second_raw);
@@ -553,7 +569,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             for (int i = 0; i < 4; i++) {
                 const int dim = 32 * d + 8 * i + 4 * half;
                 if (dim < a.dim)
-                    *reinterpret_cast<f32x4*>(a.part_out + at_part * a.dim + dim) = f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                    *reinterpret_cast<f32x4*>(a.part_out + at_part * a.dim + dim) =
+                        f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
             }
         }
         if (half == 0) a.part_sum[at_part] = make_float2(limit == -INFINITY ? -INFINITY : ref, sum);
@@ -590,7 +607,8 @@ __global__ __launch_bounds__(256) void k_prefill_join(PrefillArgs a, int request
         if (a.starts[mid] <= (int64_t)token) lo = mid;
         else hi = mid;
     }
-    const int64_t begin = min(max((int64_t)a.starts[lo], (int64_t)0), a.tokens), end = min(max((int64_t)a.starts[lo + 1], begin), a.tokens);
+    const int64_t begin = min(max((int64_t)a.starts[lo], (int64_t)0), a.tokens);
+    const int64_t end = min(max((int64_t)a.starts[lo + 1], begin), a.tokens);
     if (token < begin || token >= end || token - begin >= a.most_fresh || dim >= a.dim) return;
     const float2* sums = a.part_sum + row * a.parts;
     float top = -INFINITY;
@@ -664,7 +682,8 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     if (most_fresh * group <= 128 || tiles <= 4 || (tiles <= 24 && busy() < cus)) with_waves(4);
     const bool uneven = 4 * (__int128)tokens < 3 * (__int128)most_fresh * requests || most_fresh > longest / 2;
     const int64_t wanted = busy() > 0 ? (int64_t)((uneven ? 3 * cus : 2 * cus) / (2 * busy())) : 1;
-    l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / (tokens * sh.q_heads <= 48 * cus ? 4 : 8), 64}));
+    const int64_t least = tokens * sh.q_heads <= 48 * cus ? 4 : 8;  // tiles of a part
+    l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / least, 64}));
     l.bytes = l.parts > 1 ? (size_t)tokens * sh.q_heads * l.parts * (c.head_dim + 2) * sizeof(float) : 0;
     return l;
 }
@@ -677,6 +696,16 @@ void launch_dims(int dim, int waves, unsigned grid, hipStream_t s, const Prefill
     else if (waves == 4) k_prefill<DT, FP8, 128, 4><<<grid, 256, 0, s>>>(a);
     else if (dim <= 64) k_prefill<DT, FP8, 64, 8><<<grid, 512, 0, s>>>(a);
     else k_prefill<DT, FP8, 128, 8><<<grid, 512, 0, s>>>(a);
+}
+
+template <int DT>
+void launch_join(const PrefillArgs& a, int requests, hipStream_t s)
+{
+    const int lanes = a.dim <= 64 ? 16 : a.dim <= 128 ? 32 : 64;
+    const unsigned blocks = (unsigned)((a.tokens * a.q_heads * lanes + 255) / 256);
+    if (lanes == 16) k_prefill_join<DT, 16><<<blocks, 256, 0, s>>>(a, requests);
+    else if (lanes == 32) k_prefill_join<DT, 32><<<blocks, 256, 0, s>>>(a, requests);
+    else k_prefill_join<DT, 64><<<blocks, 256, 0, s>>>(a, requests);
 }
 
 }  // namespace
@@ -741,7 +770,8 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     a.window = shape->window < kLongest ? shape->window : 0, a.kv_heads = cache->kv_heads, a.q_heads = shape->q_heads;
     a.group = shape->q_heads / cache->kv_heads;
     a.dim = cache->head_dim;
-    Layout l = layout(dev, *shape, *cache, requests, tokens, most_fresh, std::min<int64_t>(longest, (int64_t)table_width * cache->page_size));
+    Layout l = layout(dev, *shape, *cache, requests, tokens, most_fresh,
+                      std::min<int64_t>(longest, (int64_t)table_width * cache->page_size));
     if (tokens * shape->q_heads > kLongest) l.parts = 1;
     if (l.parts > 1) {  // as many as there is room for
         const size_t room = workspace_bytes / (l.bytes / l.parts);
@@ -758,8 +788,10 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
         a.part_sum = (float2*)(a.part_out + tokens * shape->q_heads * l.parts * a.dim);
     }
     const int keys = keys_of(a.dim);
-    a.step_entries = (mfh_u32)(keys / cache->page_size), a.step_bytes = (mfh_u32)(keys % cache->page_size) * a.pages.token_bytes;
-    a.by_group = Divider((mfh_u32)a.group), a.by_kv_heads = Divider((mfh_u32)a.kv_heads), a.by_row_tiles = Divider(a.row_tiles);
+    a.step_entries = (mfh_u32)(keys / cache->page_size);
+    a.step_bytes = (mfh_u32)(keys % cache->page_size) * a.pages.token_bytes;
+    a.by_group = Divider((mfh_u32)a.group), a.by_kv_heads = Divider((mfh_u32)a.kv_heads);
+    a.by_row_tiles = Divider(a.row_tiles);
     hipStream_t s = (hipStream_t)stream;
     const bool fp8 = cache->dtype == kF8E4M3;
     if (shape->dtype == kBFloat16) {
@@ -771,12 +803,8 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     }
     MFH_TRY(launch_status("k_prefill"));
     if (l.parts > 1) {
-        const int lanes = a.dim <= 64 ? 16 : a.dim <= 128 ? 32 : 64;
-        const unsigned blocks = (unsigned)((tokens * shape->q_heads * lanes + 255) / 256);
-        const bool bf16 = shape->dtype == kBFloat16;
-        if (lanes == 16) bf16 ? k_prefill_join<kBFloat16, 16><<<blocks, 256, 0, s>>>(a, requests) : k_prefill_join<kFloat16, 16><<<blocks, 256, 0, s>>>(a, requests);
-        else if (lanes == 32) bf16 ? k_prefill_join<kBFloat16, 32><<<blocks, 256, 0, s>>>(a, requests) : k_prefill_join<kFloat16, 32><<<blocks, 256, 0, s>>>(a, requests);
-        else bf16 ? k_prefill_join<kBFloat16, 64><<<blocks, 256, 0, s>>>(a, requests) : k_prefill_join<kFloat16, 64><<<blocks, 256, 0, s>>>(a, requests);
+        if (shape->dtype == kBFloat16) launch_join<kBFloat16>(a, requests, s);
+        else launch_join<kFloat16>(a, requests, s);
         MFH_TRY(launch_status("k_prefill_join"));
     }
     return MFH_OK;
