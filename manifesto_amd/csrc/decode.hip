@@ -476,7 +476,9 @@ __global__ __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_
         tile += kWaves;
     }
 
-    // The waves' results meet: a common reference, then sums weighted by it.
+    // The waves' results meet: a common reference, then sums weighted by it.  A
+    // wave without a reference has seen nothing, and its sum is 0, or nothing but
+    // NaN, and its sum is NaN: it is added as it stands, for the row is NaN then.
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
     const float wave_ref = limit == -INFINITY ? -INFINITY : ref;
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_
             for (int w = 1; w < kWaves; w++) all = fmaxf(all, s_ref[w][h]);
 #pragma unroll
             for (int w = 0; w < kWaves; w++)
-                total += s_ref[w][h] == -INFINITY ? 0.0f : exp2_fast(s_ref[w][h] - all) * s_sum[w][h];
+                total += s_ref[w][h] == -INFINITY ? s_sum[w][h] : exp2_fast(s_ref[w][h] - all) * s_sum[w][h];  // 0, or NaN
 #pragma unroll
             for (int w = 0; w < kWaves; w++) {
                 o0 += s_out[w][h][d];
@@ -562,7 +564,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_decode_join(DecodeArgs a)
         const float2 s = sums[(int64_t)n * a.part_heads];
         const float2 w = *reinterpret_cast<const float2*>(from + (int64_t)n * a.part_heads * a.dim);
         const float f = s.x == -INFINITY ? 0.0f : exp2_fast(s.x - top);
-        all += f * s.y;
+        all += s.x == -INFINITY ? s.y : f * s.y;  // without a reference 0, or NaN
         o0 += f * w.x;
         o1 += f * w.y;
     }

@@ -247,3 +247,29 @@ def test_refused_arguments():
     call(requests=0, q=0)
     with pytest.raises(M.MFHError, match="requests"):
         A.paged_decode_workspace(A.Attention(BF16, 4, 1.0), A.KVCache(BF16, 16, 2, 64, 4), -1, 5)
+
+
+@pytest.mark.parametrize("workspace", [True, False])  # with a workspace the long request is in parts
+@pytest.mark.parametrize("page", [16, 10])
+def test_rows_whose_scores_are_all_nan(page, workspace):
+    # NaN is not -inf: lse is NaN beside a result of NaN, also where one wave or one part has nothing else
+    def step():
+        return Step(BF16, BF16, [5000, 1, 33, 200, 0, 3000], 4, 2, 64, page, seed=21)
+
+    def key(s, request, first, last):
+        for t in range(first, last):
+            s.cache.views[0][int(s.table[request, t // page]), t % page, 1, 3] = math.nan  # of key-value head 1: query heads 2 and 3
+
+    s = step()
+    clean, lse_clean = s.run(workspace=workspace)
+    s.check(clean, lse_clean)
+    s.q[0, 2, 7] = s.q[3, 1, 0] = math.nan  # a head's query in a long and in a short request
+    bad = torch.zeros(6, 4, dtype=torch.bool)
+    bad[0, 2] = bad[3, 1] = True
+    key(s, 1, 0, 1)      # the only key
+    key(s, 2, 32, 33)    # the only key of a wave
+    key(s, 5, 128, 512)  # a part of the split form
+    bad[1, 2:] = bad[2, 2:] = bad[5, 2:] = True
+    out, lse = s.run(workspace=workspace)
+    assert torch.equal(torch.isnan(lse).cpu(), bad) and torch.equal(torch.isnan(out).all(-1).cpu(), bad)
+    assert torch.equal(out[~bad.cuda()], clean[~bad.cuda()]) and torch.equal(lse[~bad.cuda()], lse_clean[~bad.cuda()])
