@@ -46,7 +46,7 @@ struct PrefillArgs {
     const float* slopes;
     int64_t q_t, q_h, out_t, out_h;  // elements
     int64_t tokens, most_fresh;
-    float scale, cap_twice, cap_scaled, v_scale;
+    float scale, cap_factor, cap_scaled, v_scale;  // cap_factor: `twice` with the scale in it, or `scaled_inverse`
     float* part_out;   // [tokens * q_heads][parts][head_dim]
     float2* part_sum;  // [tokens * q_heads][parts]: reference and sum
     int32_t window, kv_heads, q_heads, group, dim;
@@ -86,8 +86,10 @@ MFH_DEV int place(int row, int piece)
     return piece ^ (((row & 3) << 2 | (row >> 2 & 3)) & (PIECES - 1));
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.  WAVES: 4 (one group) or 8.
-template <int DT, bool FP8, int DP, int WAVES>
+// DP: head_dim rounded up to 64, 128 or 256.  WAVES: 4 (one group) or 8.  WIDE:
+// scores have a wide cap; as a branch its code takes registers and time from calls
+// without one (heads of 256 13% slower, a prompt of 512 3%).
+template <int DT, bool FP8, int DP, int WAVES, bool WIDE>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a)
 {
     constexpr int kWaves = WAVES, kThreads = 64 * kWaves, kRows = 32 * kWaves;
@@ -374,12 +376,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             const mfh_u32 width = a.window > 0 ? (mfh_u32)a.window : 1u << 31;
             mfh_u64 mask = 0;   // bit i: key i is there
             if (!plain.value && !all && !band) mask = __ballot(there(key_first + lane));
-            if (a.cap_scaled != 0.0f) {
+            if constexpr (WIDE) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        s[b][i] = wide_capped(s[b][i] * a.scale, a.cap_factor, a.cap_scaled);
+                        asm volatile("" : "+v"(s[b][i]));  // one after the other: registers are short
+                    }
+                scale = 1.0f;
+            } else if (a.cap_scaled != 0.0f) {
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++)
 #pragma unroll
                     for (int i = 0; i < 16; i++)
-                        s[b][i] = -__builtin_amdgcn_rcpf(1.0f + exp2_fast(s[b][i] * a.cap_twice));
+                        s[b][i] = -__builtin_amdgcn_rcpf(1.0f + exp2_fast(s[b][i] * a.cap_factor));
                 scale = 2.0f * a.cap_scaled, offset = a.cap_scaled;
             }
             if (whole) {
@@ -688,14 +699,23 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     return l;
 }
 
-template <int DT, bool FP8>
+template <int DT, bool FP8, bool WIDE>
 void launch_dims(int dim, int waves, unsigned grid, hipStream_t s, const PrefillArgs& a)
 {
-    if (dim > 128) k_prefill<DT, FP8, 256, 4><<<grid, 256, 0, s>>>(a);
-    else if (waves == 4 && dim <= 64) k_prefill<DT, FP8, 64, 4><<<grid, 256, 0, s>>>(a);
-    else if (waves == 4) k_prefill<DT, FP8, 128, 4><<<grid, 256, 0, s>>>(a);
-    else if (dim <= 64) k_prefill<DT, FP8, 64, 8><<<grid, 512, 0, s>>>(a);
-    else k_prefill<DT, FP8, 128, 8><<<grid, 512, 0, s>>>(a);
+    if (dim > 128) k_prefill<DT, FP8, 256, 4, WIDE><<<grid, 256, 0, s>>>(a);
+    else if (waves == 4 && dim <= 64) k_prefill<DT, FP8, 64, 4, WIDE><<<grid, 256, 0, s>>>(a);
+    else if (waves == 4) k_prefill<DT, FP8, 128, 4, WIDE><<<grid, 256, 0, s>>>(a);
+    else if (dim <= 64) k_prefill<DT, FP8, 64, 8, WIDE><<<grid, 512, 0, s>>>(a);
+    else k_prefill<DT, FP8, 128, 8, WIDE><<<grid, 512, 0, s>>>(a);
+}
+
+template <int DT>
+void launch_form(bool fp8, bool wide, int dim, int waves, unsigned grid, hipStream_t s, const PrefillArgs& a)
+{
+    if (fp8 && wide) launch_dims<DT, true, true>(dim, waves, grid, s, a);
+    else if (fp8) launch_dims<DT, true, false>(dim, waves, grid, s, a);
+    else if (wide) launch_dims<DT, false, true>(dim, waves, grid, s, a);
+    else launch_dims<DT, false, false>(dim, waves, grid, s, a);
 }
 
 template <int DT>
@@ -759,12 +779,11 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     const Strides os(shape->out_token_stride, shape->out_head_stride, shape->q_heads, cache->head_dim);
     a.q_t = qs.token, a.q_h = qs.head, a.out_t = os.token, a.out_h = os.head;
     a.tokens = tokens, a.most_fresh = std::min(most_fresh, tokens);
-    a.scale = shape->scale * cache->k_scale;
+    a.scale = shape->scale * cache->k_scale * kLog2e;
+    const bool wide = shape->softcap > kWideCap;
     if (shape->softcap > 0.0f) {
-        a.cap_twice = 2.0f * kLog2e / shape->softcap * a.scale;  // (the score's scale is in it)
         a.cap_scaled = shape->softcap * kLog2e;
-    } else {
-        a.scale *= kLog2e;
+        a.cap_factor = wide ? 1.0f / a.cap_scaled : 2.0f / shape->softcap * a.scale;
     }
     a.v_scale = cache->v_scale;
     a.window = shape->window < kLongest ? shape->window : 0, a.kv_heads = cache->kv_heads, a.q_heads = shape->q_heads;
@@ -794,13 +813,8 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     a.by_row_tiles = Divider(a.row_tiles);
     hipStream_t s = (hipStream_t)stream;
     const bool fp8 = cache->dtype == kF8E4M3;
-    if (shape->dtype == kBFloat16) {
-        if (fp8) launch_dims<kBFloat16, true>(a.dim, l.waves, (unsigned)grid, s, a);
-        else launch_dims<kBFloat16, false>(a.dim, l.waves, (unsigned)grid, s, a);
-    } else {
-        if (fp8) launch_dims<kFloat16, true>(a.dim, l.waves, (unsigned)grid, s, a);
-        else launch_dims<kFloat16, false>(a.dim, l.waves, (unsigned)grid, s, a);
-    }
+    if (shape->dtype == kBFloat16) launch_form<kBFloat16>(fp8, wide, a.dim, l.waves, (unsigned)grid, s, a);
+    else launch_form<kFloat16>(fp8, wide, a.dim, l.waves, (unsigned)grid, s, a);
     MFH_TRY(launch_status("k_prefill"));
     if (l.parts > 1) {
         if (shape->dtype == kBFloat16) launch_join<kBFloat16>(a, requests, s);

@@ -273,3 +273,20 @@ def test_rows_whose_scores_are_all_nan(page, workspace):
     out, lse = s.run(workspace=workspace)
     assert torch.equal(torch.isnan(lse).cpu(), bad) and torch.equal(torch.isnan(out).all(-1).cpu(), bad)
     assert torch.equal(out[~bad.cuda()], clean[~bad.cuda()]) and torch.equal(lse[~bad.cuda()], lse_clean[~bad.cuda()])
+
+
+@pytest.mark.parametrize("cap", [60.0, 64.0, 65.0, 1e3, 1e5, 1e7, 1e30, 8e37])
+@pytest.mark.parametrize("dtype, cache", [(F16, F16), (BF16, FP8)])
+def test_caps_far_above_the_scores_leave_them_as_they_are(cap, dtype, cache):
+    # the bounds go by the scores alone, whatever the cap; of a request of one token lse is the score
+    s = Step(dtype, cache, [1, 1, 1, 2, 3, 70, 300], 8, 2, 16, 16, seed=31, q_std=6.0, softcap=cap)
+    out, lse = s.run()
+    check_attention(out, lse, s.oracle(), dtype, 16)
+
+
+@pytest.mark.parametrize("cap", [65.0, 1e3])
+def test_large_caps_still_cap(cap):
+    s = Step(F16, F16, [1, 2, 40, 300], 4, 2, 16, 16, seed=32, q_std=60.0, scale=4.0, softcap=cap)
+    out, lse = s.run()
+    assert s.oracle()[3].max() > cap
+    check_attention(out, lse, s.oracle(), F16, 16)

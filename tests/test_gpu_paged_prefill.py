@@ -313,3 +313,21 @@ def test_refused_arguments():
     call(most_fresh=0, q=0)
     with pytest.raises(M.MFHError, match="requests"):
         A.paged_prefill_workspace(A.Attention(BF16, 4, 1.0), A.KVCache(BF16, 16, 2, 64, 4), -1, 2, 2, 5)
+
+
+@pytest.mark.parametrize("cap", [60.0, 64.0, 65.0, 1e3, 1e5, 1e7, 1e30, 8e37])
+@pytest.mark.parametrize("dtype, cache", [(F16, F16), (BF16, FP8)])
+def test_caps_far_above_the_scores_leave_them_as_they_are(cap, dtype, cache):
+    # the bounds go by the scores alone, whatever the cap; of a prompt's first token lse is the score
+    c = Chunk(dtype, cache, [(0, 1), (0, 1), (0, 3), (0, 140), (60, 20)], 8, 2, 16, 16, seed=31, q_std=6.0, softcap=cap)
+    for longest in (None, 10 ** 9):
+        out, lse = c.run(longest=longest)
+        check_attention(out, lse, c.oracle(), dtype, 16)
+
+
+@pytest.mark.parametrize("cap", [65.0, 1e3])
+def test_large_caps_still_cap(cap):
+    c = Chunk(F16, F16, [(0, 1), (0, 140), (60, 20)], 4, 2, 16, 16, seed=32, q_std=60.0, scale=4.0, softcap=cap)
+    out, lse = c.run()
+    assert c.oracle()[3].max() > cap
+    check_attention(out, lse, c.oracle(), F16, 16)
