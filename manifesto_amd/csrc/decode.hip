@@ -19,10 +19,11 @@
 // lanes) and turns the 8 x 8 block in registers, one byte permute per dword.
 //
 // Softmax runs over the tiles with a running reference instead of the running
-// maximum: it moves, and the sums are rescaled, only where a score passes it by
-// 2^8.  Weights are at most 2^8 and the reference divides out; sums and
-// products stay in f32, weights are rounded to the queries' 16 bits for the
-// product with V alone, whose terms have that rounding already.
+// maximum: it moves, and the sums are rescaled, only where a score passes the last
+// move's largest by 2^8 (kBelow in paged.hpp says where it stands); it divides out.
+// Sums and products stay in f32.  The matrix units multiply 16-bit numbers, so
+// weights are rounded to the queries' type for the product with V; their sum is
+// that of the unrounded ones.
 #include "paged.hpp"
 
 namespace mfh {
@@ -83,7 +84,6 @@ constexpr int kTile = 32;    // tokens of a wave's step
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kHeads = 16;   // query heads of a workgroup
-constexpr float kStep = 8.0f;  // the reference moves where a score passes it by 2^kStep
 
 // A row is a request's key-value head with up to 16 of its query heads.
 struct DecodeArgs {
@@ -432,8 +432,9 @@ __global__ __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             if (top > limit) {
-                const float alpha = limit == -INFINITY ? 0.0f : exp2_fast(ref - top);
-                ref = top;
+                const float next = top - kBelow<DT>;
+                const float alpha = limit == -INFINITY ? 0.0f : exp2_fast(ref - next);
+                ref = next;
                 limit = top + kStep;
                 sum *= alpha;
 #pragma unroll

@@ -109,6 +109,16 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 MFH_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The softmax's running reference moves where a score passes `limit`, which is
+// 2^kStep above the largest score at the last move; weights are 2^(score - reference).
+// In f16 the reference stands kBelow under that score, so that weights fill the
+// type's range (up to 2^15) and the smallest ones, of which a long context can have
+// many, keep their bits down to 2^-21 of the largest; from 1 down they would lose
+// them from 2^-14 on.  bf16 has f32's exponents.
+constexpr float kStep = 8.0f;
+template <int DT>
+constexpr float kBelow = DT == kFloat16 ? 7.0f : 0.0f;
+
 // Scores are in units of log2(e) on the way to exp2: scaled * tanh(x / scaled) with
 // scaled = cap log2(e), from twice = 2 / cap: tanh y = 1 - 2 / (1 + e^2y), which ends
 // at -1 and 1 without a case of its own.

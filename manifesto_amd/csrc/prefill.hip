@@ -33,7 +33,6 @@ namespace {
 // Waves of a workgroup, 32 rows each, where rows fill the card: two a SIMD if their registers allow it.
 constexpr int waves_of(int dim) { return dim <= 128 ? 8 : 4; }
 constexpr int keys_of(int dim) { return dim <= 128 ? 64 : 32; }  // of a tile
-constexpr float kStep = 8.0f;       // the reference moves where a score passes it by 2^kStep
 
 struct PrefillArgs {
     PageArgs pages;
@@ -177,7 +176,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     for (int d = 0; d < kDimTiles; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
-    float ref = 0.0f, limit = -INFINITY, sum = 0.0f;
+    float ref = 0.0f, limit = -INFINITY;
+    // Of the tiles' sums: in f32 a thousand small ones beside a large weight were off by
+    // 2^-15 together (their roundings can all go one way); in f64 0.3% of the time.
+    double total = 0.0;
 
     // ---- staging: thread t takes the piece that belongs in place t % kPieces of
     // keys t / kPieces + i * kKeyStep, and follows these keys from tile to tile:
@@ -434,10 +436,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             top = fmaxf(top, __shfl_xor(top, 32));
             if (top > limit) {
                 // (at first there is nothing to scale but what add_odd put there)
-                const float alpha = limit == -INFINITY ? 1.0f : exp2_fast(ref - top);
-                ref = top;
+                const float next = top - kBelow<DT>;
+                const float alpha = limit == -INFINITY ? 1.0f : exp2_fast(ref - next);
+                ref = next;
                 limit = top + kStep;
-                sum *= alpha;
+                total *= alpha;
 #pragma unroll
                 for (int d = 0; d < kDimTiles; d++) acc[d] *= alpha;
             }
@@ -454,7 +457,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
 #pragma unroll
             for (int i = 0; i < 16; i += 2) p[2 * b + i / 8][i / 2 % 4] = enc16x2<DT>(s[b][i], s[b][i + 1]);
         }
-        sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
     };
     auto barrier = [&]() {
         __builtin_amdgcn_sched_barrier(0);
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             soften(before, plain);
 #pragma unroll
             for (int j = 0; j < 2 * kBlocks; j++) asm volatile("" : "+v"(p[j]));  // here, not behind the barrier
-            asm volatile("" : "+v"(sum));
+            asm volatile("" : "+v"(total));
             if (put_k) put(next, plain, s_k[behind], nullptr, k_raw);
             if (put_v && put(now, plain, s_v[ahead], s_raw[ahead], v_raw)) s_odd[ahead] = round + 1;
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): it is in LDS
@@ -564,6 +567,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         products(s_k[0], s_v[behind], std::false_type{});
     }
 
+    float sum = (float)total;
     sum += __shfl_xor(sum, 32);
     // the row's place anew: kept through the loop it costs registers there
     mfh_u32 out_at = row0 + 32 * wave + col;

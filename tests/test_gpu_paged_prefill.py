@@ -331,3 +331,28 @@ def test_large_caps_still_cap(cap):
     out, lse = c.run()
     assert c.oracle()[3].max() > cap
     check_attention(out, lse, c.oracle(), F16, 16)
+
+
+@pytest.mark.parametrize("below", [14.0, 16.5])
+@pytest.mark.parametrize("workspace", [True, False])
+def test_many_small_weights_beside_a_large_one(below, workspace):
+    # one key far above a long context, whose weights are each near the smallest 16-bit number: together they are all of the result
+    n = 60000
+    c = Chunk(F16, F16, [(n - 2, 2)], 2, 1, 64, 16, seed=41, scale=0.125)
+    c.q[:] = 0
+    c.q[..., 0] = 8.0
+    k, v = c.kv[0]
+    k[:, 0, 0] = -below + (0.0 if below > 15 else 1.0) * torch.randn(n, generator=c.cache.gen).half().double().clamp(-4, 4)
+    k[:, 0, 0] = k[:, 0, 0].half().double()
+    k[5, 0, 0], v[:, 0] = 0.0, (v[:, 0].abs() + 0.5).half().double()
+    v[5] = 0.0
+    t = torch.arange(n)
+    for view, x in zip(c.cache.views, (k, v)):
+        view[c.table[0, t // 16].long().cuda(), (t % 16).cuda()] = x.half().cuda()
+    out, lse = c.run(workspace=workspace)
+    want = c.oracle()
+    # besides every weight's relative rounding, a half step of its type: 2^-25 where the largest weight is 2^7 or more
+    tail = n * 2.0 ** -32 * v.abs().max()
+    u, got = 2.0 ** -11, out.double().cpu()
+    assert ((got - want[0]).abs() <= u * want[0].abs() + want[2] * (u + 2.0 ** -14) + tail).all(), float(((got - want[0]) / want[0]).abs().max())
+    assert (lse.double().cpu() - want[1]).abs().max() <= 2.0 ** -15
