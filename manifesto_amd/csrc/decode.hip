@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             if (top > limit) {
-                const float next = top - kBelow<DT>;
+                const float next = top - kBelow<DT, FP8>;
                 const float alpha = limit == -INFINITY ? 0.0f : exp2_fast(ref - next);
                 ref = next;
                 limit = top + kStep;

@@ -114,10 +114,12 @@ MFH_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // In f16 the reference stands kBelow under that score, so that weights fill the
 // type's range (up to 2^15) and the smallest ones, of which a long context can have
 // many, keep their bits down to 2^-21 of the largest; from 1 down they would lose
-// them from 2^-14 on.  bf16 has f32's exponents.
+// them from 2^-14 on.  In bf16, which has f32's exponents, it stands at the limit:
+// weights are 1 at most, and products with the largest values stay finite where the
+// result is.  (Eight-bit values are at most 448, their scale is the result's.)
 constexpr float kStep = 8.0f;
-template <int DT>
-constexpr float kBelow = DT == kFloat16 ? 7.0f : 0.0f;
+template <int DT, bool FP8>
+constexpr float kBelow = DT == kFloat16 ? 7.0f : FP8 ? 0.0f : -kStep;
 
 // Scores are in units of log2(e) on the way to exp2: scaled * tanh(x / scaled) with
 // scaled = cap log2(e), from twice = 2 / cap: tanh y = 1 - 2 / (1 + e^2y), which ends

@@ -436,7 +436,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
             top = fmaxf(top, __shfl_xor(top, 32));
             if (top > limit) {
                 // (at first there is nothing to scale but what add_odd put there)
-                const float next = top - kBelow<DT>;
+                const float next = top - kBelow<DT, FP8>;
                 const float alpha = limit == -INFINITY ? 1.0f : exp2_fast(ref - next);
                 ref = next;
                 limit = top + kStep;

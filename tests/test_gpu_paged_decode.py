@@ -314,3 +314,18 @@ def test_many_small_weights_beside_a_large_one(below, workspace):
     u, got = 2.0 ** -11, out.double().cpu()
     assert ((got - want[0]).abs() <= u * want[0].abs() + want[2] * (u + 2.0 ** -14) + tail).all(), float(((got - want[0]) / want[0]).abs().max())
     assert (lse.double().cpu() - want[1]).abs().max() <= 2.0 ** -15
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+def test_values_near_the_largest_number_stay_finite(workspace):
+    # the value of a late key whose score is above all before it: weights are never above 1 there
+    s = Step(BF16, BF16, [700], 2, 1, 64, 16, seed=51, scale=0.125)
+    s.q[:] = 0
+    s.q[..., 0] = 8.0
+    k, v = s.kv[0]
+    k[:, 0, 0] = 0.0
+    k[130, 0, 0], v[130] = 5.0, 2.0 ** 126
+    t = torch.arange(700)
+    for view, x in zip(s.cache.views, (k, v)):
+        view[s.table[0, t // 16].long().cuda(), (t % 16).cuda()] = x.bfloat16().cuda()
+    s.check(*s.run(workspace=workspace))
