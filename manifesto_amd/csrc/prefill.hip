@@ -211,7 +211,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
             const mfh_u32 in_page = keys.in_page[i] + a.step_bytes;
-            // (a page of one token has no bytes to go on by)
+            // (a page of one token has no bytes to go on by, and no use for them)
             const bool over = a.pages.token_bytes > 0 && in_page >= page_size_bytes;
             keys.in_page[i] = over ? in_page - page_size_bytes : in_page;
             keys.entry[i] += a.step_entries + (over ? 1 : 0);
@@ -480,8 +480,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         Keys keys;  // of the next tile whose K sets out
         int64_t from[kLoads];  // of the last tile whose K set out
         auto follow = [&](int tile) { return tile < tile_end ? next_tile(tile + 1) : tile; };
+        // Tokens that are one row (a stride of 0) have no bytes to go on by either.
+        const bool steady = a.pages.token_bytes > 0 || a.pages.by_page.d == 1;
         auto move = [&](int from, int to) {
-            if (to == from + 1) go_on(keys);
+            if (steady && to == from + 1) go_on(keys);
             else go_to(keys, to);
             ask(keys);
         };
@@ -522,7 +524,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         // questions that the others have to ask: their branches took as long as
         // the products.
         const int plain_begin = a.window > 0 ? max(high_position - a.window + kKeys, 0) / kKeys : 0;
-        const int plain_end = clean && a.dim == DP ? min(min(length, low_position + 1) / kKeys, tile_end) : 0;
+        const int plain_end = clean && steady && a.dim == DP ? min(min(length, low_position + 1) / kKeys, tile_end) : 0;
         auto turn = [&](auto plain) {
             const int ahead = third == 2 ? 0 : third + 1, behind = third == 0 ? 2 : third - 1;
             if (!plain.value && round > 0 && !before.open && s_odd[behind] == round - 1) add_odd(s_raw[behind], before);

@@ -373,3 +373,25 @@ def test_values_near_the_largest_number_stay_finite(fresh, workspace):
         view[c.table[0, t // 16].long().cuda(), (t % 16).cuda()] = x.bfloat16().cuda()
     c.check(*c.run(workspace=workspace))
     c.check(*c.run(workspace=workspace, longest=10 ** 9))
+
+
+@pytest.mark.parametrize("longest", [None, 10 ** 9])
+@pytest.mark.parametrize("page", [1, 7, 16, 24, 128])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_pages_whose_tokens_are_one_row(page, dim, longest):
+    # a token stride of 0: every token of a page has the page's one key and value
+    M.init(0)
+    gen = torch.Generator().manual_seed(page)
+    n, past = 300, 120
+    pages = -(-n // page) + 1
+    k, v = (torch.randn(pages, dim, generator=gen).bfloat16() for _ in range(2))
+    table = torch.randperm(pages, generator=gen)[: pages - 1].to(torch.int32)
+    q = torch.randn(n - past, 2, dim, generator=gen).bfloat16()
+    d = [t.cuda() for t in (q, k, v, table, torch.tensor([0, n - past], dtype=torch.int32), torch.tensor([n], dtype=torch.int32))]
+    out, lse = torch.full_like(d[0], math.nan), torch.empty(n - past, 2, device="cuda")
+    desc, shape = A.KVCache(BF16, page, 1, dim, pages, page_stride=dim, token_stride=0, head_stride=dim), A.Attention(BF16, 2, dim ** -0.5)
+    A.paged_prefill(shape, desc, 1, n - past, n - past, ptr(d[0]), ptr(d[1]), ptr(d[2]), ptr(d[3]), pages - 1, ptr(d[4]), ptr(d[5]), longest or n, 0, 0,
+                    ptr(out), ptr(lse), stream=stream())
+    at = table[torch.arange(n) // page].long()
+    want = attention_oracle(q.double(), k[at].double()[:, None], v[at].double()[:, None], list(range(past, n)), dim ** -0.5)
+    check_attention(out, lse, want, BF16, dim)
