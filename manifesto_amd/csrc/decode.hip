@@ -85,6 +85,8 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kHeads = 16;   // query heads of a workgroup
 
+enum Cap { kNone, kNarrow, kWide };
+
 // A row is a request's key-value head with up to 16 of its query heads.
 struct DecodeArgs {
     PageArgs pages;
@@ -97,7 +99,7 @@ struct DecodeArgs {
     const float* slopes;
     int64_t q_t, q_h, out_t, out_h;  // elements
     float scale, cap_scaled, cap_factor, v_scale;  // cap_factor: `twice` of a cap, `scaled_inverse` of a wide one
-    bool wide_cap;
+    int cap;
     int32_t window, requests, kv_heads, q_heads, group, head_groups, dim, part_heads;
     mfh_u32 request_rows;  // kv_heads * head_groups
     mfh_u32 blocks, uneven;  // of the split form, where requests are alike and where not
@@ -403,12 +405,12 @@ __global__ __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = (j < 4 ? s0[j & 3] : s1[j & 3]) * a.scale;
-        if (a.wide_cap) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = wide_capped(x[j], a.cap_factor, a.cap_scaled);
-        } else if (a.cap_scaled != 0.0f) {
+        if (a.cap == kNarrow) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = capped(x[j], a.cap_factor, a.cap_scaled);
+        } else if (a.cap == kWide) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = wide_capped(x[j], a.cap_factor, a.cap_scaled);
         }
         if (a.slopes) {
             const int back = (int)(c.length - 1) - (int)(tile * kTile + 4 * quad);
@@ -692,8 +694,8 @@ int mfh_paged_decode(const mfh_attention_shape* shape, const mfh_kv_cache* cache
     a.scale = shape->scale * cache->k_scale * kLog2e;
     if (shape->softcap > 0.0f) {
         a.cap_scaled = shape->softcap * kLog2e;
-        a.wide_cap = shape->softcap > kWideCap;
-        a.cap_factor = a.wide_cap ? 1.0f / a.cap_scaled : 2.0f / shape->softcap;
+        a.cap = shape->softcap > kWideCap ? kWide : kNarrow;
+        a.cap_factor = a.cap == kWide ? 1.0f / a.cap_scaled : 2.0f / shape->softcap;
     }
     a.v_scale = cache->v_scale;
     a.window = shape->window, a.requests = requests, a.kv_heads = cache->kv_heads, a.q_heads = shape->q_heads;
