@@ -29,6 +29,7 @@ namespace mfh {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMostBlocks = 1 << 23;  // of a launch dimension, which holds fewer than 2^32 threads
 constexpr int kMaxPairs = 1024;  // cosines and sines in LDS: tokens of a workgroup * rotary_dim / 2
 
 struct RotaryArgs {
@@ -139,7 +140,8 @@ template <int DT, int CACHE, int E, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a)
 {
     __shared__ float s_cos[kMaxPairs], s_sin[kMaxPairs];
-    const int64_t first = (int64_t)blockIdx.x * a.tokens_per_block;
+    const int64_t first = ((int64_t)blockIdx.y * kMostBlocks + blockIdx.x) * a.tokens_per_block;
+    if (first >= a.tokens) return;
     const mfh_u32 tokens = (mfh_u32)min((int64_t)a.tokens_per_block, a.tokens - first);
     const mfh_u32 total = tokens * a.units;
     constexpr mfh_u32 kNone = 0xffffffffu;
@@ -243,14 +245,14 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a)
 }
 
 template <int DT, int CACHE, int E>
-void launch_width(bool interleaved, unsigned grid, hipStream_t s, const RotaryArgs& a)
+void launch_width(bool interleaved, dim3 grid, hipStream_t s, const RotaryArgs& a)
 {
     if (interleaved) k_rotary<DT, CACHE, E, true><<<grid, kThreads, 0, s>>>(a);
     else k_rotary<DT, CACHE, E, false><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <int DT, int CACHE>
-void launch_types(int e, bool interleaved, unsigned grid, hipStream_t s, const RotaryArgs& a)
+void launch_types(int e, bool interleaved, dim3 grid, hipStream_t s, const RotaryArgs& a)
 {
     switch (e) {
     case 8:
@@ -314,7 +316,8 @@ int launch(const mfh_rotary_shape& sh, RotaryArgs a, int cache, hipStream_t s)
     a.by_head = Divider(a.units_per_head);
     a.factor = sh.factor;
     a.sine_factor = sh.inverse ? -sh.factor : sh.factor;
-    const unsigned grid = (unsigned)((a.tokens + a.tokens_per_block - 1) / a.tokens_per_block);
+    const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+    const dim3 grid((unsigned)std::min<int64_t>(blocks, kMostBlocks), (unsigned)((blocks + kMostBlocks - 1) / kMostBlocks));
     const bool il = sh.interleaved != 0;
     switch (sh.dtype) {
     case kFloat32: launch_types<kFloat32, kFloat32>(e, il, grid, s, a); break;

@@ -246,3 +246,22 @@ def test_refused_arguments():
                          (dict(slots=0), "NULL"), (dict(v=0), "NULL"), (dict(k_cache=0), "NULL"), (dict(q=0), "without")):
         with pytest.raises(M.MFHError, match=message):
             append(**bad)
+
+
+@gpu
+def test_more_tokens_than_one_launch_dimension_holds():
+    # a token a workgroup, 2^24 and more of them: against the same tokens in two calls
+    M.init(0)
+    n, dim, half = 2 ** 24 + 300, 258, 2 ** 23 + 7
+    if torch.cuda.mem_get_info()[0] < 4 * n * dim * 2:
+        pytest.skip("needs 35 GB of device memory")
+    x = torch.randint(0, 1 << 14, (n, dim), dtype=torch.int16, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).view(torch.bfloat16)
+    p = (torch.arange(n, device="cuda") % 100003).to(torch.int32)
+    f = torch.tensor(A.rotary_frequencies(dim), dtype=torch.float64).cuda()
+    shape = A.Rotary(BF16, 1, 0, dim)
+    whole, parts = (torch.zeros_like(x) for _ in range(2))
+    A.rotary(shape, n, ptr(x), ptr(whole), 0, 0, ptr(p), ptr(f), stream=stream())
+    for first, last in ((0, half), (half, n)):
+        A.rotary(shape, last - first, ptr(x[first:]), ptr(parts[first:]), 0, 0, ptr(p[first:]), ptr(f), stream=stream())
+    assert torch.equal(whole.view(torch.int16), parts.view(torch.int16))
+    near(whole[-50:, None], *turned(x[-50:, None].double().cpu(), p[-50:].cpu(), A.rotary_frequencies(dim), dim, False), BF16)
