@@ -608,6 +608,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     if (half == 0 && a.lse) a.lse[out_row] = sum == 0.0f ? -INFINITY : ref * kLn2 + logf(sum);
 }
 
+int join_lanes(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }
+
 // Joins the parts of the rows that were computed.  A row takes the lanes that
 // its dims need, four dims each, and the wave as many rows as fit.
 template <int DT, int LANES>
@@ -701,6 +703,8 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     const int64_t wanted = busy() > 0 ? (int64_t)((uneven ? 3 * cus : 2 * cus) / (2 * busy())) : 1;
     const int64_t least = tokens * sh.q_heads <= 48 * cus ? 4 : 8;  // tiles of a part
     l.parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({wanted, tiles / least, 64}));
+    // few rows may be computed of many: the join's launch holds fewer than 2^32 threads
+    if (tokens * sh.q_heads * join_lanes(c.head_dim) > (int64_t(1) << 32) - 256) l.parts = 1;
     l.bytes = l.parts > 1 ? (size_t)tokens * sh.q_heads * l.parts * (c.head_dim + 2) * sizeof(float) : 0;
     return l;
 }
@@ -727,7 +731,7 @@ void launch_form(bool fp8, bool wide, int dim, int waves, unsigned grid, hipStre
 template <int DT>
 void launch_join(const PrefillArgs& a, int requests, hipStream_t s)
 {
-    const int lanes = a.dim <= 64 ? 16 : a.dim <= 128 ? 32 : 64;
+    const int lanes = join_lanes(a.dim);
     const unsigned blocks = (unsigned)((a.tokens * a.q_heads * lanes + 255) / 256);
     if (lanes == 16) k_prefill_join<DT, 16><<<blocks, 256, 0, s>>>(a, requests);
     else if (lanes == 32) k_prefill_join<DT, 32><<<blocks, 256, 0, s>>>(a, requests);
@@ -797,7 +801,6 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     a.dim = cache->head_dim;
     Layout l = layout(dev, *shape, *cache, requests, tokens, most_fresh,
                       std::min<int64_t>(longest, (int64_t)table_width * cache->page_size));
-    if (tokens * shape->q_heads > kLongest) l.parts = 1;
     if (l.parts > 1) {  // as many as there is room for
         const size_t room = workspace_bytes / (l.bytes / l.parts);
         l.parts = (mfh_u32)std::max<size_t>(1, std::min<size_t>(l.parts, room));

@@ -395,3 +395,24 @@ def test_pages_whose_tokens_are_one_row(page, dim, longest):
     at = table[torch.arange(n) // page].long()
     want = attention_oracle(q.double(), k[at].double()[:, None], v[at].double()[:, None], list(range(past, n)), dim ** -0.5)
     check_attention(out, lse, want, BF16, dim)
+
+
+def test_more_rows_than_one_launch_dimension_joins():
+    # few of very many rows are computed, over a context long enough for parts
+    M.init(0)
+    tokens, heads, dim, length = 2 ** 26 + 8, 4, 8, 3000
+    if torch.cuda.mem_get_info()[0] < 40 * 2 ** 30:
+        pytest.skip("needs 40 GB of device memory")
+    c = Chunk(F16, F16, [(length - 3, 3)], heads, 1, dim, 16, seed=61)
+    q = torch.zeros(tokens, heads, dim, dtype=torch.float16, device="cuda")
+    q[:3] = c.q.cuda()
+    out = torch.full((tokens, heads, dim), -3.0, dtype=torch.float16, device="cuda")
+    lse = torch.full((tokens, heads), -3.0, device="cuda")
+    d = [t.cuda() for t in (c.table, torch.tensor([0, 3], dtype=torch.int32), torch.tensor([length], dtype=torch.int32))]
+    shape, width = A.Attention(F16, heads, c.scale), c.table.shape[1] - 1
+    room = tokens * heads * 2 * (dim + 2) * 4  # of two parts
+    ws = torch.empty(room, dtype=torch.uint8, device="cuda")
+    A.paged_prefill(shape, c.cache.desc, 1, tokens, 3, ptr(q), ptr(c.cache.buffers[0]), ptr(c.cache.buffers[1]), ptr(d[0]), width, ptr(d[1]), ptr(d[2]), length, 0,
+                    0, ptr(out), ptr(lse), ptr(ws), room, table_stride=width + 1, stream=stream())
+    c.check(out[:3], lse[:3])
+    assert (out[3:] == -3).all() and (lse[3:] == -3).all()
