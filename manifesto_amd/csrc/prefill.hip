@@ -27,6 +27,8 @@
 // workgroups of four waves 890 us.
 #include "paged.hpp"
 
+#include <cfloat>
+
 namespace mfh {
 namespace {
 
@@ -794,6 +796,7 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     if (shape->softcap > 0.0f) {
         a.cap_scaled = shape->softcap * kLog2e;
         a.cap_factor = wide ? 1.0f / a.cap_scaled : 2.0f / shape->softcap * a.scale;
+        if (!__builtin_isfinite(a.cap_factor)) a.cap_factor = __builtin_copysignf(FLT_MAX, a.cap_factor);  // a score of 0 is capped at 0
     }
     a.v_scale = cache->v_scale;
     a.window = shape->window < kLongest ? shape->window : 0, a.kv_heads = cache->kv_heads, a.q_heads = shape->q_heads;

@@ -416,3 +416,11 @@ def test_more_rows_than_one_launch_dimension_joins():
                     0, ptr(out), ptr(lse), ptr(ws), room, table_stride=width + 1, stream=stream())
     c.check(out[:3], lse[:3])
     assert (out[3:] == -3).all() and (lse[3:] == -3).all()
+
+
+def test_caps_too_small_for_their_reciprocal_beside_a_scale():
+    # every score that is not zero ends at the cap, which is as good as zero; a zero stays one
+    c = Chunk(F16, F16, [(3, 70)], 2, 1, 64, 16, seed=71, scale=100.0, softcap=2.0 ** -125)
+    c.q[5] = 0
+    for longest in (None, 10 ** 9):
+        c.check(*c.run(longest=longest))
