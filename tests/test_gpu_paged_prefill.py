@@ -424,3 +424,65 @@ def test_caps_too_small_for_their_reciprocal_beside_a_scale():
     c.q[5] = 0
     for longest in (None, 10 ** 9):
         c.check(*c.run(longest=longest))
+
+
+def test_a_captured_call():
+    # lengths, starts and pages are read on the device at each replay
+    c = Chunk(BF16, BF16, [(1500, 20), (0, 0), (40, 9), (0, 3)], 4, 2, 64, 16, seed=15)
+    shape, width = A.Attention(BF16, 4, c.scale), c.table.shape[1] - 1
+    tokens, most, longest, n = c.starts[-1], 20, 2000, 4
+    q, table = c.q.cuda(), c.table.cuda()
+    starts, lengths = (torch.tensor(v, dtype=torch.int32).cuda() for v in (c.starts, c.lengths))
+    out, lse = torch.empty_like(q), torch.empty(tokens, 4, device="cuda")
+    need = A.paged_prefill_workspace(shape, c.cache.desc, n, tokens, most, longest)
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+
+    def call():
+        A.paged_prefill(shape, c.cache.desc, n, tokens, most, ptr(q), ptr(c.cache.buffers[0]), ptr(c.cache.buffers[1]), ptr(table), width, ptr(starts),
+                        ptr(lengths), longest, 0, 0, ptr(out), ptr(lse), ptr(ws), need, table_stride=width + 1, stream=stream())
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        call()
+    full, kv = list(c.lengths), c.kv
+    for now, new in ((full, [20, 0, 9, 3]), ([1520, 0, 11, 0], [20, 0, 11, 0]), ([700, 0, 49, 2], [1, 0, 17, 2]), (full, [20, 0, 9, 3])):
+        c.requests, c.lengths = [(x - f, f) for x, f in zip(now, new)], now
+        c.kv = [(k[:x], v[:x]) for (k, v), x in zip(kv, now)]
+        c.starts = [sum(new[:i]) for i in range(5)]
+        starts.copy_(torch.tensor(c.starts, dtype=torch.int32))
+        lengths.copy_(torch.tensor(now, dtype=torch.int32))
+        rows = c.starts[-1]
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(out[:rows], lse[:rows])
+        replayed = out.clone(), lse.clone()
+        out.fill_(math.nan)
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed[0][:rows], out[:rows]) and torch.equal(replayed[1][:rows], lse[:rows]) and torch.isnan(replayed[0][rows:]).all()
+
+
+def test_one_new_token_beside_a_request_without_one():
+    # as many rows as two of three requests: not a decode step, whose rows stand one per request
+    c = Chunk(BF16, BF16, [(40, 1), (25, 0), (300, 1)], 4, 2, 64, 16, seed=16)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("page", [16, 10])
+@pytest.mark.parametrize("prefix", [None, [40, 0]])
+def test_pages_behind_a_window_may_be_gone(page, prefix):
+    # a program that keeps a window returns what lies behind it and writes -1 there; long enough for parts
+    def chunk():
+        return Chunk(BF16, BF16, [(2500, 12), (900, 30)], 4, 2, 64, page, seed=18, window=1000, prefix=prefix)
+
+    c = chunk()
+    for workspace in (True, False):
+        c.check(*c.run(workspace=workspace))
+    kept = 40 // page + 1 if prefix else 0
+    c.table[0, kept: (2500 - 1000) // page] = -1
+    for workspace in (True, False):
+        for longest in (None, 10 ** 9):
+            c.check(*c.run(workspace=workspace, longest=longest))

@@ -6,7 +6,9 @@ import pytest
 import torch
 
 import manifesto_amd as M
-from paged_util import HALF_STEP, SMALLEST, attention_oracle, check_attention
+from manifesto_amd import attention as A
+from manifesto_amd.backend import Backend
+from paged_util import HALF_STEP, SMALLEST, attention_oracle, check_attention, ptr
 
 pytestmark = pytest.mark.gpu
 PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
@@ -86,3 +88,45 @@ def test_prompts_that_find_no_pages_are_refused():
     with pytest.raises(RuntimeError, match=r"requests \[1\]"):
         layer.prompts(torch.zeros(50, 32, dtype=torch.bfloat16, device="cuda"), [30, 20])
     assert layer.lengths.tolist() == [30, 0]
+
+
+def test_a_step_over_resident_tensors():
+    # caches, queries and results that are the backend's own tensors
+    b, p = Backend(0), lambda t: t.dispatch_pointer()  # noqa: E731
+    gen = torch.Generator().manual_seed(5)
+    n, hq, hk, dim, page, pages = 21, 4, 2, 64, 16, 4
+
+    def up(t, dtype):
+        return b.upload(list(t.shape), dtype, t.contiguous().view(torch.uint8).numpy().tobytes())
+
+    x = torch.randn(n, hq + 2 * hk, dim, generator=gen).bfloat16()
+    q, k, v = x[:, :hq].contiguous(), x[:, hq: hq + hk].contiguous(), x[:, hq + hk:].contiguous()
+    slots = torch.cat([torch.arange(16) + 32, torch.arange(5)])  # pages 2 and 0
+    dq, dk, dv = (up(t, M.BFLOAT16) for t in (q, k, v))
+    turned_q, out = (up(torch.zeros(n, hq, dim, dtype=torch.bfloat16), M.BFLOAT16) for _ in range(2))
+    keys, values = (up(torch.zeros(pages, hk, page, dim, dtype=torch.bfloat16), M.BFLOAT16) for _ in range(2))
+    d = [t.cuda() for t in (torch.arange(n, dtype=torch.int32), slots, torch.tensor(A.rotary_frequencies(dim), dtype=torch.float64),
+                            torch.tensor([[2, 0]], dtype=torch.int32), torch.tensor([0, n], dtype=torch.int32), torch.tensor([n], dtype=torch.int32))]
+    cache, shape = A.KVCache(M.BFLOAT16, page, hk, dim, pages), A.Attention(M.BFLOAT16, hq, dim ** -0.5)
+    for t in (dq, dk, dv, turned_q, out, keys, values):
+        t.sync()
+    torch.cuda.synchronize()
+    A.rotary_append(A.Rotary(M.BFLOAT16, hq, hk, dim), cache, n, p(dq), p(turned_q), p(dk), p(dv), ptr(d[0]), ptr(d[1]), ptr(d[2]), p(keys), p(values))
+    A.paged_prefill(shape, cache, 1, n, n, p(turned_q), p(keys), p(values), ptr(d[3]), 2, ptr(d[4]), ptr(d[5]), n, 0, 0, p(out), 0)
+    torch.cuda.synchronize()
+
+    def down(t, *shape):
+        return torch.frombuffer(bytearray(bytes(b.download(t)[1])), dtype=torch.bfloat16).view(*shape)
+
+    at = torch.tensor([2, 0])[torch.arange(n) // page]
+    ks, vs = (down(t, pages, hk, page, dim)[at, :, torch.arange(n) % page] for t in (keys, values))
+    assert torch.equal(vs, v)
+    want = turned(k.double(), torch.arange(n), dim)
+    assert ((ks.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18).all()
+    rows = attention_oracle(down(turned_q, n, hq, dim).double(), ks.double(), vs.double(), list(range(n)), dim ** -0.5)
+    check_attention(down(out, n, hq, dim), rows[1], rows, M.BFLOAT16, dim)
+    last, one = up(torch.zeros(1, hq, dim, dtype=torch.bfloat16), M.BFLOAT16), turned_q.slice((n - 1) * hq * dim, hq * dim)
+    last.sync()
+    A.paged_decode(shape, cache, 1, p(one), p(keys), p(values), ptr(d[3]), 2, ptr(d[5]), n, 0, p(last), 0)
+    torch.cuda.synchronize()
+    check_attention(down(last, 1, hq, dim), rows[1][-1:], [t[-1:] for t in rows], M.BFLOAT16, dim)

@@ -265,3 +265,43 @@ def test_more_tokens_than_one_launch_dimension_holds():
         A.rotary(shape, last - first, ptr(x[first:]), ptr(parts[first:]), 0, 0, ptr(p[first:]), ptr(f), stream=stream())
     assert torch.equal(whole.view(torch.int16), parts.view(torch.int16))
     near(whole[-50:, None], *turned(x[-50:, None].double().cpu(), p[-50:].cpu(), A.rotary_frequencies(dim), dim, False), BF16)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_keys_or_queries_alone(dtype):
+    M.init(0)
+    gen = torch.Generator().manual_seed(8)
+    n, dim, rot = 19, 64, 32
+    positions, freqs = torch.arange(n, dtype=torch.int32) * 91, A.rotary_frequencies(rot)
+    p, f = positions.cuda(), torch.tensor(freqs, dtype=torch.float64).cuda()
+    for hq, hk in ((6, 2), (0, 3), (5, 0)):
+        for of_q in (False, True):
+            x = torch.randn(n, hq if of_q else hk, dim, generator=gen).to(TORCH[dtype])
+            d = x.cuda()
+            alone = torch.full_like(d, math.nan)
+            mine = (ptr(d), ptr(alone))
+            A.rotary(A.Rotary(dtype, hq, hk, dim, rot), n, *(mine if of_q else (0, 0)), *((0, 0) if of_q else mine), ptr(p), ptr(f), stream=stream())
+            near(alone, *turned(x.double(), positions, freqs, rot, False), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_turning_back_gives_what_was_turned(interleaved):
+    M.init(0)
+    n, h, dim, rot = 40, 3, 48, 32
+    x = torch.randn(n, h, dim, generator=torch.Generator().manual_seed(9))
+    d, f = x.cuda(), torch.tensor(A.rotary_frequencies(rot), dtype=torch.float64).cuda()
+    there, back = torch.empty_like(d), torch.empty_like(d)
+    p = (torch.arange(n, dtype=torch.int32) * 40009).cuda()
+    for inverse, a, b in ((False, d, there), (True, there, back)):
+        A.rotary(A.Rotary(F32, h, 0, dim, rot, interleaved=interleaved, inverse=inverse), n, ptr(a), ptr(b), 0, 0, ptr(p), ptr(f), stream=stream())
+    # both turns have the same cosines and sines: c^2 + s^2 is 1 to within their errors of 2^-24 of a phase and of a value, and
+    # each turn rounds two products and a sum
+    size = torch.zeros_like(x)
+    i = torch.arange(rot // 2)
+    first, second = (2 * i, 2 * i + 1) if interleaved else (i, i + rot // 2)
+    size[..., first] = size[..., second] = x[..., first].abs() + x[..., second].abs()
+    off = (back.cpu() - x).abs()
+    assert (off <= size * 12 * 2.0 ** -24).all() and torch.equal(back.cpu()[..., rot:], x[..., rot:])
+    assert not torch.equal(there.cpu()[..., :rot], x[..., :rot])
