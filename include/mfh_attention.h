@@ -162,8 +162,8 @@ typedef struct {
  * Long contexts are split over workgroups; their parts meet in `workspace`
  * (mfh_paged_decode_workspace bytes, any 16-byte aligned device memory, free
  * for other use once the call's work is done; with less, or none, the call
- * splits less).  longest is the caller's upper bound of the lengths: results
- * do not depend on it, the split does. */
+ * does not split).  longest is the caller's upper bound of the lengths: it
+ * decides the split, and with it the order of the sums, nothing else. */
 int mfh_paged_decode(const mfh_attention_shape* shape, const mfh_kv_cache* cache, int32_t requests, const void* q,
                      const void* k_cache, const void* v_cache, const int32_t* table, int64_t table_stride,
                      int32_t table_width, const int32_t* lengths, int64_t longest, const float* slopes, void* out,
@@ -181,7 +181,8 @@ int mfh_paged_decode_workspace(const mfh_attention_shape* shape, const mfh_kv_ca
  *
  * tokens is the number of rows of q and out (starts past it are cut off);
  * most_fresh is an upper bound of the requests' new tokens, and a request's
- * tokens past it are not computed; longest and the workspace are as above. */
+ * tokens past it are not computed.  longest is as above, and so is the workspace,
+ * but that with less of it the call has fewer parts. */
 int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cache, int32_t requests, int64_t tokens,
                       int64_t most_fresh, const void* q, const void* k_cache, const void* v_cache,
                       const int32_t* table, int64_t table_stride, int32_t table_width, const int32_t* starts,

@@ -23,8 +23,8 @@
 // in registers meanwhile, and 8-bit caches become 16-bit on the way.
 //
 // One prompt of 8192 tokens, 32 heads over 8 of 128, bf16: 575 to 650 us from card
-// to card, 850 to 956 TFLOP/s of the 1360 that a large matrix product reaches; by
-// workgroups of four waves 890 us.
+// to card (mostly 590, 932 TFLOP/s), 850 to 956 TFLOP/s of the 1360 that a large
+// matrix product reaches; by workgroups of four waves 890 us.
 #include "paged.hpp"
 
 #include <cfloat>
@@ -77,10 +77,10 @@ MFH_DEV mfh_u32 not_finite(mfh_u32 pair)
     return ((pair & kExponents) + kOnes) & 0x80008000u;
 }
 
-// Where 16 bytes of a row stand among the row's pieces in LDS.  Rows have no
-// gaps (a load into LDS writes 64 lanes' pieces one after the other), so pieces
+// Where 16 bytes of a row stand among the row's pieces in LDS.  Rows have no gaps
+// (with them two workgroups of heads of 64 would not fit a CU's LDS), so pieces
 // change places by row: 16 rows of one piece, as K is read, lie in 16 different
-// places, and four rows of four pieces, as V is, too.
+// places, and four rows of four pieces, as V is, too.  Counted: no bank conflicts.
 template <int PIECES>
 MFH_DEV int place(int row, int piece)
 {
@@ -167,8 +167,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         if (real && d < a.dim) q[s] = load16<false>(a.q + ((begin + token) * a.q_t + head * a.q_h + d) * 2);
     }
     float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
-    // Q is waited for here: in the loop the compiler would wait for all loads
-    // on its account, those into LDS among them.
+    // Q is waited for here: at its first use in the loop the compiler would wait for
+    // all loads on its account, those of the next tiles among them, in every round.
 #pragma unroll
     for (int s = 0; s < kSteps; s++) asm volatile("" : "+v"(q[s]));
     asm volatile("" : "+v"(slope));
