@@ -80,8 +80,10 @@ typedef struct {
  * (0 where that is negative); of the others lengths[r] is after[r].
  *
  * table is [requests][table_stride] with table_width entries in use; entries
- * behind a request's pages keep what they held.  starts has requests + 1
- * entries.  requests >= 0, 0 <= tokens <= 2^30, 0 < ring_size <= 2^30. */
+ * behind a request's pages keep what they held.  lengths is another buffer than
+ * before and after, or, in a call of at most 512 tokens, may be one of them.
+ * starts has requests + 1 entries.  requests >= 0, 0 <= tokens <= 2^30,
+ * 0 < ring_size <= 2^30. */
 int mfh_page_plan(const int32_t* before, const int32_t* after, int32_t requests, int32_t page_size,
                   int32_t* table, int64_t table_stride, int32_t table_width,
                   int32_t* ring, int64_t ring_size, const int64_t* ring_state, int64_t* ring_state_out,

@@ -218,6 +218,11 @@ __global__ __launch_bounds__(kThreads) void k_page_plan(PlanArgs a)
     }
 }
 
+bool overlap(const int32_t* a, const int32_t* b, int64_t n)
+{
+    return (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)(a + n);
+}
+
 }  // namespace
 }  // namespace mfh
 
@@ -253,6 +258,9 @@ int mfh_page_plan(const int32_t* before, const int32_t* after, int32_t requests,
                   lengths, status, (mfh_u32)requests, (mfh_u32)page_size, (mfh_u32)table_width, (mfh_u32)ring_size,
                   (mfh_u32)tokens, Divider((mfh_u32)page_size)};
     const unsigned grid = (unsigned)std::max<int64_t>(1, (tokens + kThreads - 1) / kThreads);
+    if (grid > 1 && requests > 0 && (overlap(lengths, before, requests) || overlap(lengths, after, requests)))
+        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: lengths is before or after, which other workgroups still read (%lld tokens, %d at most)",
+                    what, (long long)tokens, kThreads);
     k_page_plan<<<grid, kThreads, 0, (hipStream_t)stream>>>(args);
     return launch_status("k_page_plan");
 }

@@ -131,3 +131,42 @@ def test_refused_arguments():
                          ({"starts": 0}, "NULL"), ({"ring_state_out": p}, "ring_state_out")):
         with pytest.raises(M.MFHError, match=message):
             A.page_plan(**{**good, **bad})
+
+
+def test_lengths_in_place():
+    # where one workgroup does it all; with more of them the others still read what it writes
+    M.init(0)
+    page, width = 16, 40
+    for n, each, fits in ((3, 170, True), (600, 0, True), (3, 171, False), (600, 1, False)):
+        before = np.arange(n, dtype=np.int32) % 30
+        after = before + each
+        pages = int((-(-after // page)).sum()) + 1
+        table = np.full((n, width), -1, np.int32)
+        held = 0
+        for r in range(n):
+            have = -(-int(before[r]) // page)
+            table[r, :have] = np.arange(held, held + have)
+            held += have
+        ring = np.concatenate([np.arange(held, pages), np.full(held, -1)]).astype(np.int32)
+        tokens = n * each
+        want = plan_oracle(before, after, page, table, width, ring, 0, pages - held, tokens)
+        for target in ("before", "after"):
+            d = {k: torch.from_numpy(v.copy()).cuda() for k, v in (("before", before), ("after", after), ("table", table), ("ring", ring))}
+            state, state_out = torch.tensor([0, pages - held]).cuda(), torch.zeros(2, dtype=torch.int64, device="cuda")
+            slots, positions = torch.zeros(tokens, dtype=torch.int64, device="cuda"), torch.zeros(tokens, dtype=torch.int32, device="cuda")
+            starts, status = torch.zeros(n + 1, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+
+            def call(lengths):
+                A.page_plan(ptr(d["before"]), ptr(d["after"]), n, page, ptr(d["table"]), width, ptr(d["ring"]), pages, ptr(state), ptr(state_out),
+                            ptr(slots), ptr(positions), tokens, ptr(starts), lengths, ptr(status), stream=stream())
+
+            if not fits:
+                for lengths in (ptr(d[target]), ptr(d[target]) + 4 * (n - 1)):
+                    with pytest.raises(M.MFHError, match="lengths is before or after"):
+                        call(lengths)
+                continue
+            call(ptr(d[target]))
+            torch.cuda.synchronize()
+            got = {"lengths": d[target], "slots": slots, "positions": positions, "status": status, "table": d["table"], "starts": starts}
+            for k, v in got.items():
+                assert np.array_equal(v.cpu().numpy(), want[k]), k
