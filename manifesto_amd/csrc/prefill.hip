@@ -265,7 +265,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
                           e4m3_pair<DT, false>(raw[i][1]), e4m3_pair<DT, true>(raw[i][1])};
             else x = raw[i];
             if (!plain.value && (!w.open || a.dim != DP)) {
-                const bool keep = (place<kPieces>(key, slot) * 8 < a.dim) & there(w.index * kKeys + key);
+                bool keep = place<kPieces>(key, slot) * 8 < a.dim;
+                keep &= there(w.index * kKeys + key);
 #pragma unroll
                 for (int j = 0; j < 4; j++) x[j] &= keep ? ~0u : 0u;
             }
