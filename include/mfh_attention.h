@@ -13,6 +13,12 @@
  *   mfh_paged_prefill     or, where every request has one new token,
  *   mfh_paged_decode      attention over what the cache now holds
  *
+ * Where requests grow out of one another (beams, several answers to a prompt,
+ * a prompt that begins like another one), their tables hold the same pages:
+ *
+ *   mfh_page_fork           requests become copies of others, or end
+ *   mfh_page_copy           the pages that a fork lists for copying
+ *
  * Conventions are those of mfh.h: device pointers, dtype wire codes, a stream
  * per call, MFH_OK or a negative code with mfh_last_error.  Every call is
  * asynchronous, allocates nothing and may be captured into a graph; what
@@ -89,6 +95,60 @@ int mfh_page_plan(const int32_t* before, const int32_t* after, int32_t requests,
                   int32_t* ring, int64_t ring_size, const int64_t* ring_state, int64_t* ring_state_out,
                   int64_t* slots, int32_t* positions, int64_t tokens, int32_t* starts, int32_t* lengths,
                   int32_t* status, void* stream);
+
+/* ---- requests that share pages ----------------------------------------------- */
+
+/* Request r becomes the first keep[r] tokens (NULL: all of them) of request
+ * parents[r], which may be r itself; with a parent below 0 it ends, and is
+ * empty.  All requests do so at once, from `table` and the lengths `before` to
+ * table_out and lengths, so a parent may end or change in the same call.
+ *
+ * Whole pages are shared, not copied: shares[page] is the number of requests
+ * that hold the page beyond the first (0 for a free one, and for each page as
+ * mfh_page_plan hands it out).  A partly filled last page, which grows, has one
+ * holder: of the requests that reach into their parent's the first keeps it,
+ * and every other one gets a page from the ring's head and a line in the list
+ * of copies: copy_tokens[r] tokens of page copy_from[r] to page copy_to[r] (-1,
+ * -1 and 0 for requests without), for mfh_page_copy.  Those of a request whose
+ * keep ends inside a whole page of its parent's are copied too.  Pages that no
+ * request holds any more go to the ring's tail in the order of their numbers
+ * and can be taken from the next call on.
+ *
+ * status[r]: 0 done; 1 no page was left for the copy (each later request that
+ * needs one is refused too); 2 the parent is not a request, or its length is
+ * negative or needs more than table_width pages (what such a request itself
+ * held is not returned).  A refused request is empty.
+ *
+ * Requests that share pages are shortened and ended by this call:
+ * mfh_page_plan returns a request's pages whoever else holds them; it is for
+ * growing, and for requests that share nothing.
+ *
+ * table and table_out are different buffers [requests][table_stride]; entries
+ * behind a request's pages keep what table_out held.  shares and shares_out
+ * have `pages` entries and may be one buffer, ring and its states are
+ * mfh_page_plan's, lengths is another buffer than before.  requests <= 8192,
+ * pages <= ring_size.  Negative shares count as 0; page numbers outside the
+ * cache are handed on, and not counted.
+ *
+ * The workspace (mfh_page_fork_workspace bytes, any 16-byte aligned device
+ * memory, free for other use once the call's work is done) has to be as large
+ * as it says, which may be 0. */
+int mfh_page_fork(const int32_t* parents, const int32_t* before, const int32_t* keep, int32_t requests,
+                  int32_t page_size, const int32_t* table, int32_t* table_out, int64_t table_stride,
+                  int32_t table_width, const int32_t* shares, int32_t* shares_out, int64_t pages, int32_t* ring,
+                  int64_t ring_size, const int64_t* ring_state, int64_t* ring_state_out, int32_t* lengths,
+                  int32_t* status, int32_t* copy_from, int32_t* copy_to, int32_t* copy_tokens, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int mfh_page_fork_workspace(int32_t requests, int64_t pages, size_t* bytes);
+
+/* Copies the first tokens[i] tokens (NULL: whole pages; more count as those of
+ * a page) of page from[i] to page to[i], keys and values of every head, for
+ * `pairs` pairs.  A pair with a page outside the cache is left out.  The pages
+ * written differ from one another and from those read, but that a pair may
+ * name one page twice; a page may be read by several pairs.  k_cache or
+ * v_cache may be NULL: then there is only the other one. */
+int mfh_page_copy(const mfh_kv_cache* cache, int32_t pairs, const int32_t* from, const int32_t* to,
+                  const int32_t* tokens, void* k_cache, void* v_cache, void* stream);
 
 /* ---- rotary positions ------------------------------------------------------ */
 

@@ -63,6 +63,13 @@ class AttentionShape(ctypes.Structure):
                 ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64)]
 
 
+class BeamShape(ctypes.Structure):
+    """mfh_beam_shape"""
+    _fields_ = [("dtype", ctypes.c_uint8), ("reserved", ctypes.c_uint8 * 3), ("beams", ctypes.c_int32),
+                ("picks", ctypes.c_int32), ("vocab", ctypes.c_int32), ("end_token", ctypes.c_int32),
+                ("reserved2", ctypes.c_int32), ("logits_stride", ctypes.c_int64), ("history_stride", ctypes.c_int64)]
+
+
 _lib = None
 
 
@@ -132,6 +139,12 @@ def _declare(L):
                                         i64, i32, vp, vp, i64, vp, vp, vp, vp, vp, c.c_size_t, vp]),
         "mfh_paged_prefill_workspace": (c.c_int, [c.POINTER(AttentionShape), c.POINTER(KVCacheStruct), i32, i64, i64, i64,
                                                   c.POINTER(c.c_size_t)]),
+        "mfh_page_fork": (c.c_int, [vp, vp, vp, i32, i32, vp, vp, i64, i32, vp, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp,
+                                    vp, c.c_size_t, vp]),
+        "mfh_page_fork_workspace": (c.c_int, [i32, i64, c.POINTER(c.c_size_t)]),
+        "mfh_page_copy": (c.c_int, [c.POINTER(KVCacheStruct), i32, vp, vp, vp, vp, vp, vp]),
+        "mfh_beam_select": (c.c_int, [c.POINTER(BeamShape), i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c.c_size_t, vp]),
+        "mfh_beam_select_workspace": (c.c_int, [c.POINTER(BeamShape), i32, c.POINTER(c.c_size_t)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

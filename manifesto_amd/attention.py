@@ -74,6 +74,30 @@ def page_plan(before: int, after: int, requests: int, page_size: int, table: int
                               ring_state, ring_state_out, slots, positions, tokens, starts, lengths, status, stream))
 
 
+def page_fork_workspace(requests: int, pages: int) -> int:
+    """Bytes of workspace that page_fork needs."""
+    need = ctypes.c_size_t()
+    check(lib().mfh_page_fork_workspace(requests, pages, ctypes.byref(need)))
+    return need.value
+
+
+def page_fork(parents: int, before: int, keep: int, requests: int, page_size: int, table: int, table_out: int,
+              table_width: int, shares: int, shares_out: int, pages: int, ring: int, ring_size: int, ring_state: int,
+              ring_state_out: int, lengths: int, status: int, copy_from: int, copy_to: int, copy_tokens: int,
+              workspace: int = 0, workspace_bytes: int = 0, table_stride: int | None = None, stream: int = 0) -> None:
+    """Requests become copies of others, or end: tables, shares and the list of pages to copy."""
+    check(lib().mfh_page_fork(parents, before, keep, requests, page_size, table, table_out,
+                              table_width if table_stride is None else table_stride, table_width, shares, shares_out,
+                              pages, ring, ring_size, ring_state, ring_state_out, lengths, status, copy_from, copy_to,
+                              copy_tokens, workspace, workspace_bytes, stream))
+
+
+def page_copy(cache: KVCache, pairs: int, page_from: int, page_to: int, tokens: int, k_cache: int, v_cache: int,
+              stream: int = 0) -> None:
+    """Copies the first tokens of pages to other pages, keys and values of every head."""
+    check(lib().mfh_page_copy(cache, pairs, page_from, page_to, tokens, k_cache, v_cache, stream))
+
+
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: int = ROTARY_PLAIN, factor: float = 1.0,
                        original_length: float = 0.0, low: float = 1.0, high: float = 32.0) -> list:
     """The rotary_dim / 2 frequencies in radians per position, as f64 on the host."""
