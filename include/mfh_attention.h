@@ -18,6 +18,7 @@
  *
  *   mfh_page_fork           requests become copies of others, or end
  *   mfh_page_copy           the pages that a fork lists for copying
+ *   mfh_paged_decode_shared decode that reads the tokens in common once
  *
  * Conventions are those of mfh.h: device pointers, dtype wire codes, a stream
  * per call, MFH_OK or a negative code with mfh_last_error.  Every call is
@@ -232,6 +233,29 @@ int mfh_paged_decode(const mfh_attention_shape* shape, const mfh_kv_cache* cache
                      float* lse, void* workspace, size_t workspace_bytes, void* stream);
 int mfh_paged_decode_workspace(const mfh_attention_shape* shape, const mfh_kv_cache* cache, int32_t requests,
                                int64_t longest, size_t* bytes);
+
+/* mfh_paged_decode where requests have tokens in common: the first shared[g]
+ * tokens of the requests starts[g] .. starts[g+1]-1 stand in the pages that the
+ * first of them holds, and are read from there, once for all of the group;
+ * what those requests' own tables hold for them is not read.  Each request's
+ * tokens from shared[g] on are its own.  The result is mfh_paged_decode's:
+ * each request sees the positions below its length (of the window), of the
+ * shared ones too, so a request of length 0 gives zeros and -inf.  Requests
+ * in no group share nothing.
+ *
+ * starts has groups + 1 entries that do not fall; groups <= 4096.  most_shared
+ * and most_own are the caller's upper bounds of the shared tokens and of a
+ * request's own ones: they decide how both are split over workgroups, and with
+ * it the order of the sums, nothing else.  The workspace has to be as large as
+ * mfh_paged_decode_shared_workspace says for these sizes. */
+int mfh_paged_decode_shared(const mfh_attention_shape* shape, const mfh_kv_cache* cache, int32_t requests,
+                            int32_t groups, const void* q, const void* k_cache, const void* v_cache,
+                            const int32_t* table, int64_t table_stride, int32_t table_width, const int32_t* starts,
+                            const int32_t* shared, int64_t most_shared, const int32_t* lengths, int64_t most_own,
+                            const float* slopes, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                            void* stream);
+int mfh_paged_decode_shared_workspace(const mfh_attention_shape* shape, const mfh_kv_cache* cache, int32_t requests,
+                                      int32_t groups, int64_t most_shared, int64_t most_own, size_t* bytes);
 
 /* Attention of each request's new tokens, whose keys and values are already in
  * the cache.  Tokens starts[r] .. starts[r+1]-1 of q and out are the last ones

@@ -143,6 +143,10 @@ def _declare(L):
                                     vp, c.c_size_t, vp]),
         "mfh_page_fork_workspace": (c.c_int, [i32, i64, c.POINTER(c.c_size_t)]),
         "mfh_page_copy": (c.c_int, [c.POINTER(KVCacheStruct), i32, vp, vp, vp, vp, vp, vp]),
+        "mfh_paged_decode_shared": (c.c_int, [c.POINTER(AttentionShape), c.POINTER(KVCacheStruct), i32, i32, vp, vp, vp, vp,
+                                              i64, i32, vp, vp, i64, vp, i64, vp, vp, vp, vp, c.c_size_t, vp]),
+        "mfh_paged_decode_shared_workspace": (c.c_int, [c.POINTER(AttentionShape), c.POINTER(KVCacheStruct), i32, i32, i64,
+                                                        i64, c.POINTER(c.c_size_t)]),
         "mfh_beam_select": (c.c_int, [c.POINTER(BeamShape), i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c.c_size_t, vp]),
         "mfh_beam_select_workspace": (c.c_int, [c.POINTER(BeamShape), i32, c.POINTER(c.c_size_t)]),
     }

@@ -135,6 +135,26 @@ def paged_decode(shape: Attention, cache: KVCache, requests: int, q: int, k_cach
                                  slopes, out, lse, workspace, workspace_bytes, stream))
 
 
+def paged_decode_shared_workspace(shape: Attention, cache: KVCache, requests: int, groups: int, most_shared: int,
+                                  most_own: int) -> int:
+    """Bytes of workspace that paged_decode_shared needs."""
+    need = ctypes.c_size_t()
+    check(lib().mfh_paged_decode_shared_workspace(shape, cache, requests, groups, most_shared, most_own,
+                                                  ctypes.byref(need)))
+    return need.value
+
+
+def paged_decode_shared(shape: Attention, cache: KVCache, requests: int, groups: int, q: int, k_cache: int, v_cache: int,
+                        table: int, table_width: int, starts: int, shared: int, most_shared: int, lengths: int,
+                        most_own: int, slopes: int, out: int, lse: int, workspace: int, workspace_bytes: int,
+                        table_stride: int | None = None, stream: int = 0) -> None:
+    """Attention of one new token per request, where the requests of a group have their first tokens in common."""
+    check(lib().mfh_paged_decode_shared(shape, cache, requests, groups, q, k_cache, v_cache, table,
+                                        table_width if table_stride is None else table_stride, table_width, starts, shared,
+                                        most_shared, lengths, most_own, slopes, out, lse, workspace, workspace_bytes,
+                                        stream))
+
+
 def paged_prefill_workspace(shape: Attention, cache: KVCache, requests: int, tokens: int, most_fresh: int,
                             longest: int) -> int:
     """Bytes of workspace with which paged_prefill splits as far as it pays."""

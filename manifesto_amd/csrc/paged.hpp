@@ -61,6 +61,16 @@ MFH_DEV mfh_u32 enc16x2(float lo, float hi)
     else return mfh_f16x2_rne(lo, hi);
 }
 
+// The top bits of those halves of a dword that are infinite or NaN: an exponent
+// of ones carries into them.
+template <int DT>
+MFH_DEV mfh_u32 not_finite(mfh_u32 pair)
+{
+    constexpr mfh_u32 kExponents = DT == kBFloat16 ? 0x7f807f80u : 0x7c007c00u;
+    constexpr mfh_u32 kOnes = DT == kBFloat16 ? 0x00800080u : 0x04000400u;
+    return ((pair & kExponents) + kOnes) & 0x80008000u;
+}
+
 // Four E4M3 codes by the hardware's conversion (nearest, ties to even, into
 // subnormals too; the codec of mfh_convert keeps the reference's subnormal
 // rule instead), limited to the largest finite value first.  NaN stays NaN.

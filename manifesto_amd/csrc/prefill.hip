@@ -67,16 +67,6 @@ MFH_DEV u32x2 read_column(const char* at)
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at)));
 }
 
-// The top bits of those halves of a dword that are infinite or NaN: an exponent
-// of ones carries into them.
-template <int DT>
-MFH_DEV mfh_u32 not_finite(mfh_u32 pair)
-{
-    constexpr mfh_u32 kExponents = DT == kBFloat16 ? 0x7f807f80u : 0x7c007c00u;
-    constexpr mfh_u32 kOnes = DT == kBFloat16 ? 0x00800080u : 0x04000400u;
-    return ((pair & kExponents) + kOnes) & 0x80008000u;
-}
-
 // Where 16 bytes of a row stand among the row's pieces in LDS.  Rows have no gaps
 // (with them two workgroups of heads of 64 would not fit a CU's LDS), so pieces
 // change places by row: 16 rows of one piece, as K is read, lie in 16 different
