@@ -123,7 +123,11 @@ struct Part {
     static constexpr int kBytes = FP8 ? 1 : 2;
     static constexpr int kSetDims = 16 * kDims;
     typedef typename Piece<FP8, kDims>::type VPiece;
+    // The queries of several sets leave no registers for the rest: they are read from
+    // LDS in each tile.
+    static constexpr bool kQueriesInLds = SETS > 1;
     struct Lds {
+        u32x4 q[kQueriesInLds ? SETS * kSteps : 1][64];
         float ref[kWaves][kHeads], sum[kWaves][kHeads];
         float out[kWaves][kHeads][kSetDims + 4];
     };
@@ -136,7 +140,7 @@ struct Part {
         const mfh_u32 columns = members * a.group;
 
         // This lane's columns: their queries, and the tokens they see.
-        u32x4 q[SETS][kSteps];
+        u32x4 q[kQueriesInLds ? 1 : SETS][kSteps];
         float slope[SETS];
         mfh_u32 its_first[SETS], its_length[SETS];
         mfh_u32 all_first = 0, all_length = ~0u;
@@ -154,10 +158,14 @@ struct Part {
 #pragma unroll
             for (int s = 0; s < kSteps; s++) {
                 const int d = dim_of(s);
-                q[n][s] = u32x4{0, 0, 0, 0};
-                if (real && d < a.dim) q[n][s] = load16<false>(a.q + ((int64_t)r * a.q_t + (int64_t)head * a.q_h + d) * 2);
+                if (kQueriesInLds && n % kWaves != wave) continue;
+                u32x4 x = {0, 0, 0, 0};
+                if (real && d < a.dim) x = load16<false>(a.q + ((int64_t)r * a.q_t + (int64_t)head * a.q_h + d) * 2);
+                if constexpr (kQueriesInLds) lds.q[n * kSteps + s][lane] = x;
+                else q[n][s] = x;
             }
         }
+        if (kQueriesInLds) __syncthreads();
 #pragma unroll
         for (int x = 1; x < 16; x <<= 1) {
             all_first = max(all_first, (mfh_u32)__shfl_xor((int)all_first, x));
@@ -180,17 +188,27 @@ struct Part {
         const char* k_base = a.pages.k + kv * a.pages.head_bytes;
         const char* v_base = a.pages.v + kv * a.pages.head_bytes;
 
+        // One tile's registers: the next tile's keys set out when this one's scores
+        // are there, its values when this one's are used up.
         Pages<FAST> pages;
-        auto load = [&](u32x4(&k)[2][kLoads], VPiece(&v)[kSets][8], mfh_u32& valid, mfh_u32 tile) {
-            const TileAt<FAST> at = pages.place(a.pages, seen, tile * kTile, lane, tile < end);
-            valid = at.valid;
-            if constexpr (FAST) {
+        u32x4 k[2][kLoads];
+        VPiece v[kSets][8];
+        auto load_k = [&](const TileAt<FAST>& at) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < 2; h++) {
+                if constexpr (FAST) {
                     const __amdgpu_buffer_rsrc_t rows = page_buffer(k_base, at.page[h], a.pages);
 #pragma unroll
                     for (int s = 0; s < kLoads; s++) k[h][s] = buffer_piece<u32x4>(rows, k_lane[s], at.in_page[h]);
+                } else {
+                    const char* row = k_base + shuffle64(at.mine, 16 * h + col);
+#pragma unroll
+                    for (int s = 0; s < kLoads; s++) k[h][s] = load16<true>(row + k_lane[s]);
                 }
+            }
+        };
+        auto load_v = [&](const TileAt<FAST>& at) {
+            if constexpr (FAST) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const __amdgpu_buffer_rsrc_t rows = page_buffer(v_base, at.page[h], a.pages);
@@ -201,12 +219,6 @@ struct Part {
                             v[u][4 * h + j] = buffer_piece<VPiece>(rows, v_lane[u], at.in_page[h] + j * token_bytes);
                 }
             } else {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const char* row = k_base + shuffle64(at.mine, 16 * h + col);
-#pragma unroll
-                    for (int s = 0; s < kLoads; s++) k[h][s] = load16<true>(row + k_lane[s]);
-                }
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const char* row = v_base + shuffle64(at.mine, 16 * (j >> 2) + 4 * quad + (j & 3));
@@ -232,12 +244,175 @@ struct Part {
             const mfh_u32 high = its_length[n] > t0 ? min(its_length[n] - t0, 32u) : 0;
             return high > low ? (mfh_u32)(((mfh_u64)1 << high) - ((mfh_u64)1 << low)) : 0;
         };
-        // What a tile's values that are not finite add to the columns that see them.
-        auto add_odd = [&](mfh_u32 t0, mfh_u32 valid) {
-            for (mfh_u32 left = valid; left; left &= left - 1) {
-                const mfh_u32 i = __ffs((int)left) - 1, t = t0 + i, entry = a.pages.by_page.quotient(t);
-                const char* row = v_base + (mfh_u64)(mfh_u32)table[entry] * a.pages.page_bytes +
-                                  (t - entry * a.pages.by_page.d) * token_bytes;
+        int q_lane = lane;
+        auto scores = [&](int n, float (&x)[8]) {
+            f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+            auto product = [&](auto cut) {
+#pragma unroll
+                for (int s = 0; s < kSteps; s++) {
+                    u32x4 k0, k1;
+                    if constexpr (FP8) {
+                        const int w = 2 * (s & 1);
+                        k0 = widen<DT>(k[0][s / 2][w], k[0][s / 2][w + 1]);
+                        k1 = widen<DT>(k[1][s / 2][w], k[1][s / 2][w + 1]);
+                    } else {
+                        k0 = k[0][s], k1 = k[1][s];
+                    }
+                    if (cut.value && dim_of(s) >= a.dim) k0 = k1 = u32x4{0, 0, 0, 0};
+                    u32x4 x;
+                    if constexpr (kQueriesInLds) x = lds.q[n * kSteps + s][q_lane];
+                    else x = q[n][s];
+                    s0 = mfma16<DT>(k0, x, s0);
+                    s1 = mfma16<DT>(k1, x, s1);
+                }
+            };
+            if (ragged) product(std::true_type{});
+            else product(std::false_type{});
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = j < 4 ? s0[j & 3] : s1[j & 3];
+        };
+        auto soften = [&](int n, float (&x)[8], mfh_u32 t0, mfh_u32 valid, bool open) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] *= a.scale;
+            if (a.cap == kNarrow) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = capped(x[j], a.cap_factor, a.cap_scaled);
+            } else if (a.cap == kWide) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = wide_capped(x[j], a.cap_factor, a.cap_scaled);
+            }
+            if (a.slopes) {
+                const int back = (int)(its_length[n] - 1) - (int)(t0 + 4 * quad);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] -= slope[n] * (float)(back - (16 * (j >> 2) + (j & 3)));
+            }
+            if (!open) {
+                const mfh_u32 bits = valid & sees(n, t0);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (!(bits >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1)) x[j] = -INFINITY;
+            }
+            float top = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) top = fmaxf(top, x[j]);
+            if (__any(top > limit[n])) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                if (top > limit[n]) {
+                    const float next = top - kBelow<DT, FP8>;
+                    const float alpha = limit[n] == -INFINITY ? 0.0f : exp2_fast(ref[n] - next);
+                    ref[n] = next;
+                    limit[n] = top + kStep;
+                    sum[n] *= alpha;
+#pragma unroll
+                    for (int u = 0; u < kSets; u++)
+#pragma unroll
+                        for (int d = 0; d < kDims; d++) acc[n][u][d] *= alpha;
+                }
+            }
+            u32x4 p;
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = exp2_fast(x[j] - ref[n]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[j] = enc16x2<DT>(x[2 * j], x[2 * j + 1]);
+            sum[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            return p;
+        };
+        // Cuts values to zero that are of no token (0 * NaN would be NaN) or not
+        // finite; whether there are any of those.
+        auto cut = [&](mfh_u32 valid) {
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const bool keep = valid >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1;
+#pragma unroll
+                for (int u = 0; u < kSets; u++) {
+                    constexpr int kWords = sizeof(VPiece) / 4;
+                    typedef mfh_u32 Words __attribute__((ext_vector_type(kWords)));
+                    Words w = __builtin_bit_cast(Words, v[u][j]);
+#pragma unroll
+                    for (int i = 0; i < kWords; i++) {
+                        mfh_u32 whole;
+                        if constexpr (FP8) {
+                            const mfh_u32 tops = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                            whole = tops | (tops - (tops >> 7));
+                        } else {
+                            const mfh_u32 tops = not_finite<DT>(w[i]);
+                            whole = tops | (tops - (tops >> 15));
+                        }
+                        odd |= keep && whole != 0;
+                        w[i] &= keep ? ~whole : 0u;
+                    }
+                    v[u][j] = __builtin_bit_cast(VPiece, w);
+                }
+            }
+            return __any(odd);
+        };
+        auto add = [&](const u32x4 (&p)[SETS]) {
+#pragma unroll
+            for (int u = 0; u < kSets; u++) {
+                u32x4 t[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) t[j] = dims_of<DT, FP8, kDims>(v[u][j]);
+#pragma unroll
+                for (int d = 0; d < kDims; d += 2) {
+                    const int i = d / 2;
+                    const u32x4 even = {low_halves(t[0][i], t[1][i]), low_halves(t[2][i], t[3][i]),
+                                        low_halves(t[4][i], t[5][i]), low_halves(t[6][i], t[7][i])};
+                    const u32x4 other = {high_halves(t[0][i], t[1][i]), high_halves(t[2][i], t[3][i]),
+                                         high_halves(t[4][i], t[5][i]), high_halves(t[6][i], t[7][i])};
+#pragma unroll
+                    for (int n = 0; n < SETS; n++) {
+                        acc[n][u][d] = mfma16<DT>(even, p[n], acc[n][u][d]);
+                        acc[n][u][d + 1] = mfma16<DT>(other, p[n], acc[n][u][d + 1]);
+                    }
+                }
+            }
+        };
+
+        auto page_of = [&](mfh_u32 t) { return (mfh_u32)table[a.pages.by_page.quotient(t)]; };
+
+        mfh_u32 tile = begin + wave;
+        bool odd = false;  // some tile had values that are not finite, and columns that do not see it
+        if (tile < end) {
+            pages.ask(a.pages, table, seen, tile * kTile, lane);
+            TileAt<FAST> at = pages.place(a.pages, seen, tile * kTile, lane, true);
+            load_k(at);
+            load_v(at);
+            pages.ask(a.pages, table, seen, (tile + kWaves) * kTile, lane);
+            // Loads of a tile past the last one are made too, and move nothing:
+            // behind loads that only some iterations make, the compiler waits for
+            // all that are on their way.
+            for (; tile < end; tile += kWaves) {
+                const mfh_u32 t0 = tile * kTile, valid = at.valid;
+                const bool open = valid == 0xffffffffu && t0 >= all_first && t0 + kTile <= all_length;  // to every column
+                float x[SETS][8];
+                asm volatile("" : "+v"(q_lane));  // else all of Q is read ahead of the loop, into registers
+#pragma unroll
+                for (int n = 0; n < SETS; n++) scores(n, x[n]);
+                at = pages.place(a.pages, seen, t0 + kWaves * kTile, lane, tile + kWaves < end);
+                load_k(at);
+                pages.ask(a.pages, table, seen, t0 + 2 * kWaves * kTile, lane);
+                u32x4 p[SETS];
+#pragma unroll
+                for (int n = 0; n < SETS; n++) p[n] = soften(n, x[n], t0, valid, open);
+                if (!open) odd |= cut(valid);
+                add(p);
+                load_v(at);
+            }
+        }
+        // Those values, added to the columns that see them (here, and not in their
+        // tile: what the loop holds beside the sums leaves no registers for it).
+        for (tile = odd ? begin + wave : end; tile < end; tile += kWaves) {
+            const mfh_u32 t0 = tile * kTile;
+            const bool open = t0 >= max(all_first, seen.first) && t0 + kTile <= min(all_length, seen.length);
+            bool whole = open;  // such a tile was not cut
+            for (mfh_u32 i = 0; i < kTile && whole; i++) whole = page_of(t0 + i) < a.pages.pages;
+            for (mfh_u32 t = max(t0, seen.first); t < min(t0 + kTile, seen.length) && !whole; t++) {
+                const mfh_u32 page = page_of(t);
+                if (page >= a.pages.pages) continue;
+                const char* row = v_base + (mfh_u64)page * a.pages.page_bytes +
+                                  (t - a.pages.by_page.quotient(t) * a.pages.by_page.d) * token_bytes;
 #pragma unroll
                 for (int u = 0; u < kSets; u++)
 #pragma unroll
@@ -253,139 +428,9 @@ struct Part {
                             if (__builtin_isfinite(value)) continue;
 #pragma unroll
                             for (int n = 0; n < SETS; n++)
-                                if (sees(n, t0) >> i & 1) acc[n][u][d][x] += value;
+                                if (t >= its_first[n] && t < its_length[n]) acc[n][u][d][x] += value;
                         }
             }
-        };
-
-        auto compute = [&](u32x4(&k)[2][kLoads], VPiece(&v)[kSets][8], mfh_u32 valid, mfh_u32 tile) {
-            const mfh_u32 t0 = tile * kTile;
-            const bool open = valid == 0xffffffffu && t0 >= all_first && t0 + kTile <= all_length;  // to every column
-            u32x4 p[SETS];
-#pragma unroll
-            for (int n = 0; n < SETS; n++) {
-                f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
-                auto product = [&](auto cut) {
-#pragma unroll
-                    for (int s = 0; s < kSteps; s++) {
-                        u32x4 k0, k1;
-                        if constexpr (FP8) {
-                            const int w = 2 * (s & 1);
-                            k0 = widen<DT>(k[0][s / 2][w], k[0][s / 2][w + 1]);
-                            k1 = widen<DT>(k[1][s / 2][w], k[1][s / 2][w + 1]);
-                        } else {
-                            k0 = k[0][s], k1 = k[1][s];
-                        }
-                        if (cut.value && dim_of(s) >= a.dim) k0 = k1 = u32x4{0, 0, 0, 0};
-                        s0 = mfma16<DT>(k0, q[n][s], s0);
-                        s1 = mfma16<DT>(k1, q[n][s], s1);
-                    }
-                };
-                if (ragged) product(std::true_type{});
-                else product(std::false_type{});
-
-                float x[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = (j < 4 ? s0[j & 3] : s1[j & 3]) * a.scale;
-                if (a.cap == kNarrow) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = capped(x[j], a.cap_factor, a.cap_scaled);
-                } else if (a.cap == kWide) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = wide_capped(x[j], a.cap_factor, a.cap_scaled);
-                }
-                if (a.slopes) {
-                    const int back = (int)(its_length[n] - 1) - (int)(t0 + 4 * quad);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] -= slope[n] * (float)(back - (16 * (j >> 2) + (j & 3)));
-                }
-                if (!open) {
-                    const mfh_u32 bits = valid & sees(n, t0);
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (!(bits >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1)) x[j] = -INFINITY;
-                }
-                float top = x[0];
-#pragma unroll
-                for (int j = 1; j < 8; j++) top = fmaxf(top, x[j]);
-                if (__any(top > limit[n])) {
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    if (top > limit[n]) {
-                        const float next = top - kBelow<DT, FP8>;
-                        const float alpha = limit[n] == -INFINITY ? 0.0f : exp2_fast(ref[n] - next);
-                        ref[n] = next;
-                        limit[n] = top + kStep;
-                        sum[n] *= alpha;
-#pragma unroll
-                        for (int u = 0; u < kSets; u++)
-#pragma unroll
-                            for (int d = 0; d < kDims; d++) acc[n][u][d] *= alpha;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = exp2_fast(x[j] - ref[n]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) p[n][j] = enc16x2<DT>(x[2 * j], x[2 * j + 1]);
-                sum[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            }
-            bool odd = false;
-#pragma unroll
-            for (int u = 0; u < kSets; u++) {
-                u32x4 t[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    t[j] = dims_of<DT, FP8, kDims>(v[u][j]);
-                    if (!open) {
-                        const bool keep = valid >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1;
-#pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            const mfh_u32 tops = not_finite<DT>(t[j][w]);
-                            odd |= keep && tops != 0;
-                            t[j][w] &= keep ? ~(tops | (tops - (tops >> 15))) : 0u;  // 0 * NaN would be NaN
-                        }
-                    }
-                }
-#pragma unroll
-                for (int d = 0; d < kDims; d += 2) {
-                    const int i = d / 2;
-                    const u32x4 even = {low_halves(t[0][i], t[1][i]), low_halves(t[2][i], t[3][i]),
-                                        low_halves(t[4][i], t[5][i]), low_halves(t[6][i], t[7][i])};
-                    const u32x4 other = {high_halves(t[0][i], t[1][i]), high_halves(t[2][i], t[3][i]),
-                                         high_halves(t[4][i], t[5][i]), high_halves(t[6][i], t[7][i])};
-#pragma unroll
-                    for (int n = 0; n < SETS; n++) {
-                        acc[n][u][d] = mfma16<DT>(even, p[n], acc[n][u][d]);
-                        acc[n][u][d + 1] = mfma16<DT>(other, p[n], acc[n][u][d + 1]);
-                    }
-                }
-            }
-            if (!open && __any(odd)) add_odd(t0, valid);
-        };
-
-        mfh_u32 tile = begin + wave;
-        // Two tiles' registers: one is on its way while the other is computed.
-        u32x4 k_a[2][kLoads], k_b[2][kLoads];
-        VPiece v_a[kSets][8], v_b[kSets][8];
-        mfh_u32 valid_a = 0, valid_b = 0;
-        if (tile < end) {
-            pages.ask(a.pages, table, seen, tile * kTile, lane);
-            load(k_a, v_a, valid_a, tile);
-            pages.ask(a.pages, table, seen, (tile + kWaves) * kTile, lane);
-        }
-        // Loads of a tile past the last one are made too, and move nothing:
-        // behind loads that only some iterations make, the compiler waits for
-        // all that are on their way.
-        while (tile < end) {
-            load(k_b, v_b, valid_b, tile + kWaves);
-            pages.ask(a.pages, table, seen, (tile + 2 * kWaves) * kTile, lane);
-            compute(k_a, v_a, valid_a, tile);
-            tile += kWaves;
-            if (tile >= end) break;
-            load(k_a, v_a, valid_a, tile + kWaves);
-            pages.ask(a.pages, table, seen, (tile + 2 * kWaves) * kTile, lane);
-            compute(k_b, v_b, valid_b, tile);
-            tile += kWaves;
         }
 
         // The waves' results meet, as in decode.hip.
@@ -442,7 +487,10 @@ __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ?
 {
     typedef Part<DT, FP8, DP, FAST, SETS> Common;
     typedef Part<DT, FP8, DP, FAST, 1> Own;
-    __shared__ typename Common::Lds lds;  // of one size for all
+    __shared__ union {
+        typename Common::Lds common;
+        typename Own::Lds own;
+    } lds;
     const int lane = threadIdx.x & 63;
     if (blockIdx.x < a.shared_blocks) {
         // Workgroups of one head and part, which read the same keys if they are of
@@ -476,7 +524,7 @@ __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ?
         const Tiles tiles(group, a.by_shared_piece, a.shared_parts);
         if (part >= tiles.parts) return;
         const mfh_u32 share = uniform((tiles.count + tiles.parts - 1) / tiles.parts);
-        Common::run(a, lds, group.begin, group.members, tile_of * kColumns, kv, group, group.begin,
+        Common::run(a, lds.common, group.begin, group.members, tile_of * kColumns, kv, group, group.begin,
                     tiles.first + min(part * share, tiles.count), tiles.first + min((part + 1) * share, tiles.count), part);
         return;
     }
@@ -493,7 +541,7 @@ __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ?
     const Tiles tiles(own, a.by_own_piece, a.own_parts);
     if (part >= tiles.parts) return;
     const mfh_u32 share = uniform((tiles.count + tiles.parts - 1) / tiles.parts);
-    Own::run(a, reinterpret_cast<typename Own::Lds&>(lds), r, 1, head_group * kHeads, kv, own, r,
+    Own::run(a, lds.own, r, 1, head_group * kHeads, kv, own, r,
              tiles.first + min(part * share, tiles.count), tiles.first + min((part + 1) * share, tiles.count),
              a.shared_parts + part);
 }
