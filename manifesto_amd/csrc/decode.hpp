@@ -46,7 +46,8 @@ MFH_DEV mfh_u32 range_bits(mfh_u32 first, mfh_u32 from, mfh_u32 to)
 template <bool FAST>
 struct Pages {
     int32_t page[2];
-    __device__ void ask(const PageArgs& p, const int32_t* table, const Seen& c, mfh_u32 t0, int lane)
+    template <typename Table>
+    __device__ void ask(const PageArgs& p, Table table, const Seen& c, mfh_u32 t0, int lane)
     {
         // past the length its last page again
 #pragma unroll
@@ -88,12 +89,12 @@ MFH_DEV __amdgpu_buffer_rsrc_t page_buffer(const char* base, mfh_i64 page, const
 
 constexpr int kStreamed = 2;  // nt: keys and values are read once
 
-template <typename T>
+template <typename T, int POLICY = kStreamed>
 MFH_DEV T buffer_piece(__amdgpu_buffer_rsrc_t r, mfh_u32 lane_at, mfh_u32 at)
 {
-    if constexpr (sizeof(T) == 16) return __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane_at, (int)at, kStreamed);
-    else if constexpr (sizeof(T) == 8) return __builtin_amdgcn_raw_buffer_load_b64(r, (int)lane_at, (int)at, kStreamed);
-    else return __builtin_amdgcn_raw_buffer_load_b32(r, (int)lane_at, (int)at, kStreamed);
+    if constexpr (sizeof(T) == 16) return __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane_at, (int)at, POLICY);
+    else if constexpr (sizeof(T) == 8) return __builtin_amdgcn_raw_buffer_load_b64(r, (int)lane_at, (int)at, POLICY);
+    else return __builtin_amdgcn_raw_buffer_load_b32(r, (int)lane_at, (int)at, POLICY);
 }
 
 // Eight codes as 16-bit values.
@@ -109,11 +110,11 @@ template <> struct Piece<false, 4> { typedef u32x2 type; };
 template <> struct Piece<true, 8> { typedef u32x2 type; };
 template <> struct Piece<true, 4> { typedef mfh_u32 type; };
 
-template <typename T>
+template <typename T, bool STREAMED = true>
 MFH_DEV T load_piece(const char* p)
 {
-    if constexpr (sizeof(T) == 16) return load16<true>(p);
-    else if constexpr (sizeof(T) == 8) return load8<true>(p);
+    if constexpr (sizeof(T) == 16) return load16<STREAMED>(p);
+    else if constexpr (sizeof(T) == 8) return load8<STREAMED>(p);
     else return load4(p);
 }
 

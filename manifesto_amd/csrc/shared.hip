@@ -126,6 +126,9 @@ struct Part {
     // The queries of several sets leave no registers for the rest: they are read from
     // LDS in each tile.
     static constexpr bool kQueriesInLds = SETS > 1;
+    // Shared tokens are read by several workgroups where their columns fill more than
+    // one: nt would keep them out of the L2.
+    static constexpr int kPolicy = SETS > 1 ? 0 : kStreamed;
     struct Lds {
         u32x4 q[kQueriesInLds ? SETS * kSteps : 1][64];
         float ref[kWaves][kHeads], sum[kWaves][kHeads];
@@ -174,17 +177,22 @@ struct Part {
         all_first = uniform(all_first), all_length = uniform(all_length);
 
         const mfh_u32 token_bytes = a.pages.token_bytes;
-        // Lanes past head_dim read its last dims again, inside the row: their
-        // steps have zeros in Q (and, below, in K), their results are not written.
+        // Lanes past head_dim have zeros in Q and in K: buffer loads past every page's
+        // end give them, else they read its last dims again, inside the row, and
+        // are cut.  In V they do so too, their results are not written.
         mfh_u32 k_lane[kLoads], v_lane[kSets];
 #pragma unroll
-        for (int s = 0; s < kLoads; s++)
-            k_lane[s] = (FAST ? col * token_bytes : 0) + (FP8 ? min(64 * s + 16 * quad, a.dim - 16) : min(32 * s + 8 * quad, a.dim - 8) * 2);
+        for (int s = 0; s < kLoads; s++) {
+            const int d = FP8 ? 64 * s + 16 * quad : 32 * s + 8 * quad, last = a.dim - 16 / kBytes;
+            k_lane[s] = FAST ? d <= last ? col * token_bytes + d * kBytes : 1u << 31 : min(d, last) * kBytes;
+        }
 #pragma unroll
         for (int u = 0; u < kSets; u++)
             v_lane[u] = (FAST ? 4 * quad * token_bytes : 0) + min(u * kSetDims + kDims * col, a.dim - kDims) * kBytes;
         const bool ragged = a.dim != DP;
-        const int32_t* table = a.pages.table + (int64_t)table_row * a.pages.table_stride;
+        // (read as scalars)
+        typedef const __attribute__((address_space(4))) int32_t* Table;
+        const Table table = (Table)(uintptr_t)(a.pages.table + (int64_t)table_row * a.pages.table_stride);
         const char* k_base = a.pages.k + kv * a.pages.head_bytes;
         const char* v_base = a.pages.v + kv * a.pages.head_bytes;
 
@@ -199,11 +207,11 @@ struct Part {
                 if constexpr (FAST) {
                     const __amdgpu_buffer_rsrc_t rows = page_buffer(k_base, at.page[h], a.pages);
 #pragma unroll
-                    for (int s = 0; s < kLoads; s++) k[h][s] = buffer_piece<u32x4>(rows, k_lane[s], at.in_page[h]);
+                    for (int s = 0; s < kLoads; s++) k[h][s] = buffer_piece<u32x4, kPolicy>(rows, k_lane[s], at.in_page[h]);
                 } else {
                     const char* row = k_base + shuffle64(at.mine, 16 * h + col);
 #pragma unroll
-                    for (int s = 0; s < kLoads; s++) k[h][s] = load16<true>(row + k_lane[s]);
+                    for (int s = 0; s < kLoads; s++) k[h][s] = load16<kPolicy == kStreamed>(row + k_lane[s]);
                 }
             }
         };
@@ -216,14 +224,14 @@ struct Part {
                     for (int j = 0; j < 4; j++)
 #pragma unroll
                         for (int u = 0; u < kSets; u++)
-                            v[u][4 * h + j] = buffer_piece<VPiece>(rows, v_lane[u], at.in_page[h] + j * token_bytes);
+                            v[u][4 * h + j] = buffer_piece<VPiece, kPolicy>(rows, v_lane[u], at.in_page[h] + j * token_bytes);
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const char* row = v_base + shuffle64(at.mine, 16 * (j >> 2) + 4 * quad + (j & 3));
 #pragma unroll
-                    for (int u = 0; u < kSets; u++) v[u][j] = load_piece<VPiece>(row + v_lane[u]);
+                    for (int u = 0; u < kSets; u++) v[u][j] = load_piece<VPiece, kPolicy == kStreamed>(row + v_lane[u]);
                 }
             }
         };
@@ -266,12 +274,13 @@ struct Part {
                     s1 = mfma16<DT>(k1, x, s1);
                 }
             };
-            if (ragged) product(std::true_type{});
+            if (!FAST && ragged) product(std::true_type{});
             else product(std::false_type{});
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = j < 4 ? s0[j & 3] : s1[j & 3];
         };
-        auto soften = [&](int n, float (&x)[8], mfh_u32 t0, mfh_u32 valid, bool open) {
+        // Scores as the softmax takes them: scaled, capped, biased, masked.
+        auto shape = [&](int n, float (&x)[8], mfh_u32 t0, mfh_u32 valid, bool open) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] *= a.scale;
             if (a.cap == kNarrow) {
@@ -292,31 +301,55 @@ struct Part {
                 for (int j = 0; j < 8; j++)
                     if (!(bits >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1)) x[j] = -INFINITY;
             }
-            float top = x[0];
+        };
+        // The weights of x * scale.
+        auto soften = [&](float (&x)[SETS][8], float scale, u32x4 (&p)[SETS]) {
+            float top[SETS];
+            bool above = false;
 #pragma unroll
-            for (int j = 1; j < 8; j++) top = fmaxf(top, x[j]);
-            if (__any(top > limit[n])) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                if (top > limit[n]) {
-                    const float next = top - kBelow<DT, FP8>;
-                    const float alpha = limit[n] == -INFINITY ? 0.0f : exp2_fast(ref[n] - next);
-                    ref[n] = next;
-                    limit[n] = top + kStep;
-                    sum[n] *= alpha;
+            for (int n = 0; n < SETS; n++) {
+                top[n] = x[n][0];
 #pragma unroll
-                    for (int u = 0; u < kSets; u++)
+                for (int j = 1; j < 8; j++) top[n] = fmaxf(top[n], x[n][j]);
+                top[n] *= scale;
+                above |= top[n] > limit[n];
+            }
+            if (__any(above)) {
+                // (the sums are taken out of the accumulation registers here, and not, for all
+                // tiles, ahead of the question)
+                if constexpr (SETS > 1) {
 #pragma unroll
-                        for (int d = 0; d < kDims; d++) acc[n][u][d] *= alpha;
+                    for (int n = 0; n < SETS; n++)
+#pragma unroll
+                        for (int u = 0; u < kSets; u++)
+#pragma unroll
+                            for (int d = 0; d < kDims; d++) asm volatile("" : "+a"(acc[n][u][d]));
+                }
+#pragma unroll
+                for (int n = 0; n < SETS; n++) {
+                    top[n] = fmaxf(top[n], __shfl_xor(top[n], 16));
+                    top[n] = fmaxf(top[n], __shfl_xor(top[n], 32));
+                    if (top[n] > limit[n]) {
+                        const float next = top[n] - kBelow<DT, FP8>;
+                        const float alpha = limit[n] == -INFINITY ? 0.0f : exp2_fast(ref[n] - next);
+                        ref[n] = next;
+                        limit[n] = top[n] + kStep;
+                        sum[n] *= alpha;
+#pragma unroll
+                        for (int u = 0; u < kSets; u++)
+#pragma unroll
+                            for (int d = 0; d < kDims; d++) acc[n][u][d] *= alpha;
+                    }
                 }
             }
-            u32x4 p;
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = exp2_fast(x[j] - ref[n]);
+            for (int n = 0; n < SETS; n++) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) p[j] = enc16x2<DT>(x[2 * j], x[2 * j + 1]);
-            sum[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            return p;
+                for (int j = 0; j < 8; j++) x[n][j] = exp2_fast(__builtin_fmaf(x[n][j], scale, -ref[n]));
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[n][j] = enc16x2<DT>(x[n][2 * j], x[n][2 * j + 1]);
+                sum[n] += ((x[n][0] + x[n][1]) + (x[n][2] + x[n][3])) + ((x[n][4] + x[n][5]) + (x[n][6] + x[n][7]));
+            }
         };
         // Cuts values to zero that are of no token (0 * NaN would be NaN) or not
         // finite; whether there are any of those.
@@ -378,27 +411,42 @@ struct Part {
             pages.ask(a.pages, table, seen, tile * kTile, lane);
             TileAt<FAST> at = pages.place(a.pages, seen, tile * kTile, lane, true);
             load_k(at);
-            load_v(at);
             pages.ask(a.pages, table, seen, (tile + kWaves) * kTile, lane);
-            // Loads of a tile past the last one are made too, and move nothing:
-            // behind loads that only some iterations make, the compiler waits for
-            // all that are on their way.
-            for (; tile < end; tile += kWaves) {
+            load_v(at);
+            const bool simple = a.cap == kNone && !a.slopes && a.scale > 0.0f;
+            // A tile that is seen whole by every column, and whose scores only need
+            // their scale, goes without the other questions.  Loads of a tile past
+            // the last one are made too, and move nothing: behind loads that only some
+            // iterations make, the compiler waits for all that are on their way.
+            auto open = [&]() {
+                return at.valid == 0xffffffffu && tile * kTile >= all_first && tile * kTile + kTile <= all_length;
+            };
+            auto turn = [&](auto plain) {
                 const mfh_u32 t0 = tile * kTile, valid = at.valid;
-                const bool open = valid == 0xffffffffu && t0 >= all_first && t0 + kTile <= all_length;  // to every column
+                const bool whole = plain.value || open();
                 float x[SETS][8];
+                u32x4 p[SETS];
                 asm volatile("" : "+v"(q_lane));  // else all of Q is read ahead of the loop, into registers
 #pragma unroll
                 for (int n = 0; n < SETS; n++) scores(n, x[n]);
                 at = pages.place(a.pages, seen, t0 + kWaves * kTile, lane, tile + kWaves < end);
                 load_k(at);
                 pages.ask(a.pages, table, seen, t0 + 2 * kWaves * kTile, lane);
-                u32x4 p[SETS];
+                if constexpr (plain.value) {
+                    soften(x, a.scale, p);
+                } else {
 #pragma unroll
-                for (int n = 0; n < SETS; n++) p[n] = soften(n, x[n], t0, valid, open);
-                if (!open) odd |= cut(valid);
+                    for (int n = 0; n < SETS; n++) shape(n, x[n], t0, valid, whole);
+                    soften(x, 1.0f, p);
+                    if (!whole) odd |= cut(valid);
+                }
                 add(p);
                 load_v(at);
+                tile += kWaves;
+            };
+            while (tile < end) {
+                while (simple && tile < end && open()) turn(std::true_type{});
+                if (tile < end) turn(std::false_type{});
             }
         }
         // Those values, added to the columns that see them (here, and not in their
