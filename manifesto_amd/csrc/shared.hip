@@ -65,11 +65,25 @@ MFH_DEV mfh_u32 first_of(const SharedArgs& a, mfh_u32 length)
 // Requests that share tokens, and those that some of them see: [first, length).
 struct Group : Seen {
     mfh_u32 begin, members;
-    MFH_DEV void of(const SharedArgs& a, mfh_u32 g, int lane)
+    // 64 groups from `base` on, one a lane
+    struct Lanes {
+        mfh_u32 begin, end, length;
+        MFH_DEV Lanes(const SharedArgs& a, mfh_u32 base, int lane)
+        {
+            const mfh_u32 g = base + lane;
+            begin = end = length = 0;
+            if (g >= a.groups) return;
+            const int32_t from = a.starts[g], to = a.starts[g + 1], tokens = a.shared[g];
+            begin = (mfh_u32)min(max(from, 0), (int)a.requests);
+            end = (mfh_u32)min(max(to, (int)begin), (int)a.requests);
+            length = limited(a, tokens);
+        }
+    };
+    MFH_DEV void of(const SharedArgs& a, const Lanes& lanes, int at, int lane)
     {
-        begin = uniform((mfh_u32)min(max(a.starts[g], 0), (int)a.requests));
-        members = uniform((mfh_u32)min(max(a.starts[g + 1], (int)begin), (int)a.requests)) - begin;
-        length = uniform(limited(a, a.shared[g]));
+        begin = (mfh_u32)__builtin_amdgcn_readlane((int)lanes.begin, at);
+        members = (mfh_u32)__builtin_amdgcn_readlane((int)lanes.end, at) - begin;
+        length = (mfh_u32)__builtin_amdgcn_readlane((int)lanes.length, at);
         first = 0;
         if (a.window > 0) {
             first = length;
@@ -86,18 +100,16 @@ struct Group : Seen {
     MFH_DEV void with(const SharedArgs& a, mfh_u32 r, int lane)
     {
         begin = members = length = first = 0;
-        auto upto = [&](mfh_u32 g, mfh_u32 end) {
-            return (mfh_u32)__popcll(__ballot(g < end && a.starts[min(g, a.groups)] <= (int64_t)r));
-        };
-        mfh_u32 found = upto(lane * a.group_step, a.groups);
-        if (found == 0) return;
-        mfh_u32 g = (found - 1) * a.group_step;
-        if (a.group_step > 1) {
-            found = upto(g + lane, min(g + a.group_step, a.groups));
-            if (found == 0) return;
-            g += found - 1;
+        mfh_u32 base = 0;
+        if (a.group_step > 1) {  // every group_step-th group first
+            const mfh_u32 g = lane * a.group_step;
+            const mfh_u64 upto = __ballot(g < a.groups && a.starts[min(g, a.groups)] <= (int64_t)r);
+            if (!upto) return;
+            base = ((mfh_u32)__popcll(upto) - 1) * a.group_step;
         }
-        if ((int64_t)a.starts[g + 1] > (int64_t)r) of(a, g, lane);
+        const Lanes lanes(a, base, lane);
+        const mfh_u64 its = __ballot(lanes.begin <= r && r < lanes.end);
+        if (its) of(a, lanes, __ffsll((unsigned long long)its) - 1, lane);
     }
 };
 
@@ -113,8 +125,9 @@ struct Tiles {
 };
 
 // One part: the tiles begin .. end of `seen`, read through `table`, for the
-// columns column0 .. of `members` requests from `request0` on.
-template <int DT, bool FP8, int DP, bool FAST, int SETS>
+// columns column0 .. of `members` requests from `request0` on.  WAVES: of the
+// workgroup that take the tiles in turn; 1: the wave is alone.
+template <int DT, bool FP8, int DP, bool FAST, int SETS, int WAVES>
 struct Part {
     static constexpr int kSteps = DP / 32;                    // of the product with K
     static constexpr int kLoads = FP8 ? kSteps / 2 : kSteps;  // of 16 bytes of a token of K
@@ -122,18 +135,29 @@ struct Part {
     static constexpr int kDims = DP == 64 ? 4 : 8;            // of a lane in a set
     static constexpr int kBytes = FP8 ? 1 : 2;
     static constexpr int kSetDims = 16 * kDims;
+    static constexpr int kSums = SETS * kSets * kDims;        // registers of four sums
+    static constexpr int kGiven = kSums / kWaves;             // of a wave where all meet
     typedef typename Piece<FP8, kDims>::type VPiece;
-    // The queries of several sets leave no registers for the rest: they are read from
-    // LDS in each tile.
-    static constexpr bool kQueriesInLds = SETS > 1;
     // Shared tokens are read by several workgroups where their columns fill more than
     // one: nt would keep them out of the L2.
     static constexpr int kPolicy = SETS > 1 ? 0 : kStreamed;
+    // Keys go through LDS where other workgroups read them too.  As the products take
+    // them 16 lanes read 16 rows, and the texture unit takes a lane at a time: a
+    // quarter of what it does for whole rows, which is enough for memory, but not for the
+    // L2 (256 requests over 16384 tokens, 178 us so).
+    static constexpr bool kStaged = SETS > 1;
+    static constexpr int kPieces = DP * kBytes / 16;          // of a row of K
+    static constexpr int kRowsAtOnce = 64 / kPieces;          // of a load
+    static constexpr int kRaw = kStaged ? 32 / kRowsAtOnce : 1;
     struct Lds {
-        u32x4 q[kQueriesInLds ? SETS * kSteps : 1][64];
-        float ref[kWaves][kHeads], sum[kWaves][kHeads];
-        float out[kWaves][kHeads][kSetDims + 4];
+        float ref[kWaves][SETS][kHeads], sum[kWaves][SETS][kHeads];
+        union {
+            u32x4 k[kStaged ? kWaves : 1][kStaged ? 32 * kPieces : 1];
+            f32x4 given[WAVES > 1 ? kWaves - 1 : 1][WAVES > 1 ? kSums : 1][64];
+        };
     };
+    // Where piece c of row r stands in LDS among the row's: 16 rows' in 16 places.
+    static MFH_DEV int place(int r, int c) { return c ^ ((kPieces < 16 ? r / (16 / kPieces) : r) & (kPieces < 16 ? kPieces - 1 : 15)); }
 
     static MFH_DEV void run(const SharedArgs& a, Lds& lds, mfh_u32 request0, mfh_u32 members, mfh_u32 column0, mfh_u32 kv,
                             const Seen& seen, mfh_u32 table_row, mfh_u32 begin, mfh_u32 end, mfh_u32 slot)
@@ -142,80 +166,94 @@ struct Part {
         const int col = lane & 15, quad = lane >> 4;
         const mfh_u32 columns = members * a.group;
 
+        // (the table is read as scalars)
+        typedef const __attribute__((address_space(4))) int32_t* Table;
+        const Table table = (Table)(uintptr_t)(a.pages.table + (int64_t)table_row * a.pages.table_stride);
+        Pages<FAST> pages;
+        mfh_u32 tile = begin + (WAVES > 1 ? wave : 0);
+        pages.ask(a.pages, table, seen, tile * kTile, lane);
+
         // This lane's columns: their queries, and the tokens they see.
-        u32x4 q[kQueriesInLds ? 1 : SETS][kSteps];
+        u32x4 q[SETS][kSteps];
         float slope[SETS];
         mfh_u32 its_first[SETS], its_length[SETS];
         mfh_u32 all_first = 0, all_length = ~0u;
         auto dim_of = [&](int s) { return FP8 ? 64 * (s / 2) + 16 * quad + 8 * (s & 1) : 32 * s + 8 * quad; };
+        auto column = [&](int n) { return column0 + 16 * n + col; };
+        auto row_of = [&](int n) {  // request * q_heads + head, of the first column where there is no such one
+            const mfh_u32 c = column(n) < columns ? column(n) : 0, member = a.by_group.quotient(c);
+            return (int64_t)(request0 + member) * a.q_heads + kv * a.group + (c - member * a.group);
+        };
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
-            const mfh_u32 c = column0 + 16 * n + col;
-            const bool real = c < columns;
-            const mfh_u32 member = a.by_group.quotient(real ? c : 0), head = kv * a.group + ((real ? c : 0) - member * a.group);
+            const bool real = column(n) < columns;
+            const mfh_u32 c = real ? column(n) : 0, member = a.by_group.quotient(c), head = kv * a.group + (c - member * a.group);
             const mfh_u32 r = request0 + member;
             its_length[n] = length_of(a, r);
-            its_first[n] = first_of(a, its_length[n]);
-            if (real) all_first = max(all_first, its_first[n]), all_length = min(all_length, its_length[n]);
             slope[n] = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
 #pragma unroll
             for (int s = 0; s < kSteps; s++) {
                 const int d = dim_of(s);
-                if (kQueriesInLds && n % kWaves != wave) continue;
-                u32x4 x = {0, 0, 0, 0};
-                if (real && d < a.dim) x = load16<false>(a.q + ((int64_t)r * a.q_t + (int64_t)head * a.q_h + d) * 2);
-                if constexpr (kQueriesInLds) lds.q[n * kSteps + s][lane] = x;
-                else q[n][s] = x;
+                q[n][s] = u32x4{0, 0, 0, 0};
+                if (real && d < a.dim) q[n][s] = load16<false>(a.q + ((int64_t)r * a.q_t + (int64_t)head * a.q_h + d) * 2);
             }
         }
-        if (kQueriesInLds) __syncthreads();
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) {
-            all_first = max(all_first, (mfh_u32)__shfl_xor((int)all_first, x));
-            all_length = min(all_length, (mfh_u32)__shfl_xor((int)all_length, x));
-        }
-        all_first = uniform(all_first), all_length = uniform(all_length);
 
         const mfh_u32 token_bytes = a.pages.token_bytes;
         // Lanes past head_dim have zeros in Q and in K: buffer loads past every page's
         // end give them, else they read its last dims again, inside the row, and
         // are cut.  In V they do so too, their results are not written.
-        mfh_u32 k_lane[kLoads], v_lane[kSets];
+        constexpr int kKinds = kStaged ? 16 / kRowsAtOnce : kLoads;  // of lanes' places in K
+        mfh_u32 k_lane[kKinds], v_lane[kSets];
+        const int last = a.dim - 16 / kBytes;
 #pragma unroll
-        for (int s = 0; s < kLoads; s++) {
-            const int d = FP8 ? 64 * s + 16 * quad : 32 * s + 8 * quad, last = a.dim - 16 / kBytes;
-            k_lane[s] = FAST ? d <= last ? col * token_bytes + d * kBytes : 1u << 31 : min(d, last) * kBytes;
+        for (int s = 0; s < kKinds; s++) {
+            // staged: of row kRowsAtOnce * s + lane / kPieces the piece whose place this lane fills
+            const int row = kStaged ? lane / kPieces : col;
+            const int d = kStaged ? place(kRowsAtOnce * s + row, lane % kPieces) * (16 / kBytes) : FP8 ? 64 * s + 16 * quad : 32 * s + 8 * quad;
+            k_lane[s] = FAST ? d <= last ? row * token_bytes + d * kBytes : 1u << 31 : min(d, last) * kBytes;
         }
+        int k_at[kLoads];  // in LDS
+#pragma unroll
+        for (int s = 0; s < kLoads; s++) k_at[s] = col * kPieces + place(col, 4 * s + quad);
 #pragma unroll
         for (int u = 0; u < kSets; u++)
             v_lane[u] = (FAST ? 4 * quad * token_bytes : 0) + min(u * kSetDims + kDims * col, a.dim - kDims) * kBytes;
         const bool ragged = a.dim != DP;
-        // (read as scalars)
-        typedef const __attribute__((address_space(4))) int32_t* Table;
-        const Table table = (Table)(uintptr_t)(a.pages.table + (int64_t)table_row * a.pages.table_stride);
         const char* k_base = a.pages.k + kv * a.pages.head_bytes;
         const char* v_base = a.pages.v + kv * a.pages.head_bytes;
 
-        // One tile's registers: the next tile's keys set out when this one's scores
-        // are there, its values when this one's are used up.
-        Pages<FAST> pages;
-        u32x4 k[2][kLoads];
-        VPiece v[kSets][8];
-        auto load_k = [&](const TileAt<FAST>& at) {
+        // Staged: rows as they stand in memory; else the products' operands.
+        typedef u32x4 Keys[kStaged ? kRaw : 2 * kLoads];
+        typedef VPiece Values[kSets][8];
+        auto load_k = [&](Keys& k, const TileAt<FAST>& at) {
+            if constexpr (FAST) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (FAST) {
+                for (int h = 0; h < 2; h++) {
                     const __amdgpu_buffer_rsrc_t rows = page_buffer(k_base, at.page[h], a.pages);
+                    if constexpr (kStaged) {
 #pragma unroll
-                    for (int s = 0; s < kLoads; s++) k[h][s] = buffer_piece<u32x4, kPolicy>(rows, k_lane[s], at.in_page[h]);
-                } else {
+                        for (int s = 0; s < kKinds; s++)
+                            k[h * kKinds + s] = buffer_piece<u32x4, kPolicy>(rows, k_lane[s], at.in_page[h] + s * kRowsAtOnce * token_bytes);
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < kLoads; s++) k[h * kLoads + s] = buffer_piece<u32x4, kPolicy>(rows, k_lane[s], at.in_page[h]);
+                    }
+                }
+            } else if constexpr (kStaged) {
+#pragma unroll
+                for (int i = 0; i < kRaw; i++)
+                    k[i] = load16<kPolicy == kStreamed>(k_base + shuffle64(at.mine, i * kRowsAtOnce + lane / kPieces) + k_lane[i % kKinds]);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
                     const char* row = k_base + shuffle64(at.mine, 16 * h + col);
 #pragma unroll
-                    for (int s = 0; s < kLoads; s++) k[h][s] = load16<kPolicy == kStreamed>(row + k_lane[s]);
+                    for (int s = 0; s < kLoads; s++) k[h * kLoads + s] = load16<kPolicy == kStreamed>(row + k_lane[s]);
                 }
             }
         };
-        auto load_v = [&](const TileAt<FAST>& at) {
+        auto load_v = [&](Values& v, const TileAt<FAST>& at) {
             if constexpr (FAST) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -235,75 +273,119 @@ struct Part {
                 }
             }
         };
+        // One tile's registers: the next tile's keys set out when this one's are used up
+        // (or in LDS), and its values then too.  Loads of a tile past the last one are
+        // made too, and move nothing: behind loads that only some waves or rounds
+        // make, the compiler waits for all that are on their way.
+        Keys k;
+        Values v;
+        TileAt<FAST> at = pages.place(a.pages, seen, tile * kTile, lane, tile < end);
+        load_k(k, at);
+        load_v(v, at);
+        pages.ask(a.pages, table, seen, (tile + WAVES) * kTile, lane);
 
-        f32x4 acc[SETS][kSets][kDims];
-        float ref[SETS], limit[SETS], sum[SETS];
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
-            ref[n] = 0.0f, limit[n] = -INFINITY, sum[n] = 0.0f;
-#pragma unroll
-            for (int u = 0; u < kSets; u++)
-#pragma unroll
-                for (int d = 0; d < kDims; d++) acc[n][u][d] = f32x4{0, 0, 0, 0};
+            its_first[n] = first_of(a, its_length[n]);
+            if (column(n) < columns) all_first = max(all_first, its_first[n]), all_length = min(all_length, its_length[n]);
         }
-        // The tokens of a tile from t0 on that a column sees, a bit each.
-        auto sees = [&](int n, mfh_u32 t0) {
-            const mfh_u32 low = its_first[n] > t0 ? min(its_first[n] - t0, 32u) : 0;
-            const mfh_u32 high = its_length[n] > t0 ? min(its_length[n] - t0, 32u) : 0;
-            return high > low ? (mfh_u32)(((mfh_u64)1 << high) - ((mfh_u64)1 << low)) : 0;
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) {
+            all_first = max(all_first, (mfh_u32)__shfl_xor((int)all_first, x));
+            all_length = min(all_length, (mfh_u32)__shfl_xor((int)all_length, x));
+        }
+        all_first = uniform(all_first), all_length = uniform(all_length);
+        // Queries of several sets wait in accumulation registers, where the products take
+        // them from.
+        if constexpr (SETS > 1) {
+#pragma unroll
+            for (int n = 0; n < SETS; n++)
+#pragma unroll
+                for (int s = 0; s < kSteps; s++) asm volatile("" : "+a"(q[n][s]));
+        }
+
+        f32x4 acc[kSums];  // [set][set of dims][dim]
+        float ref[SETS], limit[SETS], sum[SETS];
+#pragma unroll
+        for (int n = 0; n < SETS; n++) ref[n] = 0.0f, limit[n] = -INFINITY, sum[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSums; i++) acc[i] = f32x4{0, 0, 0, 0};
+        auto stage = [&](const Keys& k) {
+            if constexpr (kStaged) {
+#pragma unroll
+                for (int i = 0; i < kRaw; i++) lds.k[wave][i * 64 + lane] = k[i];
+            }
         };
-        int q_lane = lane;
-        auto scores = [&](int n, float (&x)[8]) {
-            f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+        auto scores = [&](const Keys& k, float (&x)[SETS][8]) {
+            f32x4 s0[SETS], s1[SETS];
+#pragma unroll
+            for (int n = 0; n < SETS; n++) s0[n] = s1[n] = f32x4{0, 0, 0, 0};
+            u32x4 from[2][kLoads];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int s = 0; s < kLoads; s++) {
+                    if constexpr (kStaged) from[h][s] = lds.k[wave][16 * kPieces * h + k_at[s]];
+                    else from[h][s] = k[h * kLoads + s];
+                }
+            // (left to itself the compiler reads right ahead of each product, and waits there)
+            if constexpr (kStaged) __builtin_amdgcn_sched_barrier(0);
             auto product = [&](auto cut) {
 #pragma unroll
                 for (int s = 0; s < kSteps; s++) {
                     u32x4 k0, k1;
                     if constexpr (FP8) {
                         const int w = 2 * (s & 1);
-                        k0 = widen<DT>(k[0][s / 2][w], k[0][s / 2][w + 1]);
-                        k1 = widen<DT>(k[1][s / 2][w], k[1][s / 2][w + 1]);
+                        k0 = widen<DT>(from[0][s / 2][w], from[0][s / 2][w + 1]);
+                        k1 = widen<DT>(from[1][s / 2][w], from[1][s / 2][w + 1]);
                     } else {
-                        k0 = k[0][s], k1 = k[1][s];
+                        k0 = from[0][s], k1 = from[1][s];
                     }
                     if (cut.value && dim_of(s) >= a.dim) k0 = k1 = u32x4{0, 0, 0, 0};
-                    u32x4 x;
-                    if constexpr (kQueriesInLds) x = lds.q[n * kSteps + s][q_lane];
-                    else x = q[n][s];
-                    s0 = mfma16<DT>(k0, x, s0);
-                    s1 = mfma16<DT>(k1, x, s1);
+#pragma unroll
+                    for (int n = 0; n < SETS; n++) {
+                        s0[n] = mfma16<DT>(k0, q[n][s], s0[n]);
+                        s1[n] = mfma16<DT>(k1, q[n][s], s1[n]);
+                    }
                 }
             };
             if (!FAST && ragged) product(std::true_type{});
             else product(std::false_type{});
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = j < 4 ? s0[j & 3] : s1[j & 3];
-        };
-        // Scores as the softmax takes them: scaled, capped, biased, masked.
-        auto shape = [&](int n, float (&x)[8], mfh_u32 t0, mfh_u32 valid, bool open) {
+            for (int n = 0; n < SETS; n++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] *= a.scale;
+                for (int j = 0; j < 8; j++) x[n][j] = j < 4 ? s0[n][j & 3] : s1[n][j & 3];
+        };
+        // Where scores need more than their scale, they get it here.
+        const bool simple = a.cap == kNone && !a.slopes && a.scale > 0.0f;
+        const float scale = simple ? a.scale : 1.0f;
+        auto shape = [&](float (&x)[SETS][8], mfh_u32 t0) {
+#pragma unroll
+            for (int n = 0; n < SETS; n++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[n][j] *= a.scale;
             if (a.cap == kNarrow) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = capped(x[j], a.cap_factor, a.cap_scaled);
+                for (int n = 0; n < SETS; n++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[n][j] = capped(x[n][j], a.cap_factor, a.cap_scaled);
             } else if (a.cap == kWide) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = wide_capped(x[j], a.cap_factor, a.cap_scaled);
+                for (int n = 0; n < SETS; n++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[n][j] = wide_capped(x[n][j], a.cap_factor, a.cap_scaled);
             }
             if (a.slopes) {
-                const int back = (int)(its_length[n] - 1) - (int)(t0 + 4 * quad);
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] -= slope[n] * (float)(back - (16 * (j >> 2) + (j & 3)));
-            }
-            if (!open) {
-                const mfh_u32 bits = valid & sees(n, t0);
+                for (int n = 0; n < SETS; n++) {
+                    const int back = (int)(its_length[n] - 1) - (int)(t0 + 4 * quad);
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (!(bits >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1)) x[j] = -INFINITY;
+                    for (int j = 0; j < 8; j++) x[n][j] -= slope[n] * (float)(back - (16 * (j >> 2) + (j & 3)));
+                }
             }
         };
         // The weights of x * scale.
-        auto soften = [&](float (&x)[SETS][8], float scale, u32x4 (&p)[SETS]) {
+        auto soften = [&](float (&x)[SETS][8], u32x4 (&p)[SETS]) {
             float top[SETS];
             bool above = false;
 #pragma unroll
@@ -319,11 +401,7 @@ struct Part {
                 // tiles, ahead of the question)
                 if constexpr (SETS > 1) {
 #pragma unroll
-                    for (int n = 0; n < SETS; n++)
-#pragma unroll
-                        for (int u = 0; u < kSets; u++)
-#pragma unroll
-                            for (int d = 0; d < kDims; d++) asm volatile("" : "+a"(acc[n][u][d]));
+                    for (int i = 0; i < kSums; i++) asm volatile("" : "+a"(acc[i]));
                 }
 #pragma unroll
                 for (int n = 0; n < SETS; n++) {
@@ -336,9 +414,7 @@ struct Part {
                         limit[n] = top[n] + kStep;
                         sum[n] *= alpha;
 #pragma unroll
-                        for (int u = 0; u < kSets; u++)
-#pragma unroll
-                            for (int d = 0; d < kDims; d++) acc[n][u][d] *= alpha;
+                        for (int i = 0; i < kSets * kDims; i++) acc[n * kSets * kDims + i] *= alpha;
                     }
                 }
             }
@@ -351,9 +427,20 @@ struct Part {
                 sum[n] += ((x[n][0] + x[n][1]) + (x[n][2] + x[n][3])) + ((x[n][4] + x[n][5]) + (x[n][6] + x[n][7]));
             }
         };
+        auto mask = [&](float (&x)[SETS][8], mfh_u32 t0, mfh_u32 valid) {
+#pragma unroll
+            for (int n = 0; n < SETS; n++) {
+                const mfh_u32 low = its_first[n] > t0 ? min(its_first[n] - t0, 32u) : 0;
+                const mfh_u32 high = its_length[n] > t0 ? min(its_length[n] - t0, 32u) : 0;
+                const mfh_u32 sees = high > low ? (mfh_u32)(((mfh_u64)1 << high) - ((mfh_u64)1 << low)) & valid : 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (!(sees >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1)) x[n][j] = -INFINITY;
+            }
+        };
         // Cuts values to zero that are of no token (0 * NaN would be NaN) or not
         // finite; whether there are any of those.
-        auto cut = [&](mfh_u32 valid) {
+        auto cut = [&](Values& v, mfh_u32 valid) {
             bool odd = false;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -381,7 +468,7 @@ struct Part {
             }
             return __any(odd);
         };
-        auto add = [&](const u32x4 (&p)[SETS]) {
+        auto add = [&](const Values& v, const u32x4 (&p)[SETS]) {
 #pragma unroll
             for (int u = 0; u < kSets; u++) {
                 u32x4 t[8];
@@ -396,65 +483,43 @@ struct Part {
                                          high_halves(t[4][i], t[5][i]), high_halves(t[6][i], t[7][i])};
 #pragma unroll
                     for (int n = 0; n < SETS; n++) {
-                        acc[n][u][d] = mfma16<DT>(even, p[n], acc[n][u][d]);
-                        acc[n][u][d + 1] = mfma16<DT>(other, p[n], acc[n][u][d + 1]);
+                        f32x4* to = acc + (n * kSets + u) * kDims + d;
+                        to[0] = mfma16<DT>(even, p[n], to[0]);
+                        to[1] = mfma16<DT>(other, p[n], to[1]);
                     }
                 }
             }
         };
 
-        auto page_of = [&](mfh_u32 t) { return (mfh_u32)table[a.pages.by_page.quotient(t)]; };
-
-        mfh_u32 tile = begin + wave;
         bool odd = false;  // some tile had values that are not finite, and columns that do not see it
-        if (tile < end) {
-            pages.ask(a.pages, table, seen, tile * kTile, lane);
-            TileAt<FAST> at = pages.place(a.pages, seen, tile * kTile, lane, true);
-            load_k(at);
-            pages.ask(a.pages, table, seen, (tile + kWaves) * kTile, lane);
-            load_v(at);
-            const bool simple = a.cap == kNone && !a.slopes && a.scale > 0.0f;
-            // A tile that is seen whole by every column, and whose scores only need
-            // their scale, goes without the other questions.  Loads of a tile past
-            // the last one are made too, and move nothing: behind loads that only some
-            // iterations make, the compiler waits for all that are on their way.
-            auto open = [&]() {
-                return at.valid == 0xffffffffu && tile * kTile >= all_first && tile * kTile + kTile <= all_length;
+        for (; tile < end; tile += WAVES) {
+            const mfh_u32 t0 = tile * kTile, valid = at.valid;
+            const bool open = valid == 0xffffffffu && t0 >= all_first && t0 + kTile <= all_length;  // to every column
+            float x[SETS][8];
+            u32x4 p[SETS];
+            auto next = [&]() {
+                at = pages.place(a.pages, seen, t0 + WAVES * kTile, lane, tile + WAVES < end);
+                load_k(k, at);
             };
-            auto turn = [&](auto plain) {
-                const mfh_u32 t0 = tile * kTile, valid = at.valid;
-                const bool whole = plain.value || open();
-                float x[SETS][8];
-                u32x4 p[SETS];
-                asm volatile("" : "+v"(q_lane));  // else all of Q is read ahead of the loop, into registers
-#pragma unroll
-                for (int n = 0; n < SETS; n++) scores(n, x[n]);
-                at = pages.place(a.pages, seen, t0 + kWaves * kTile, lane, tile + kWaves < end);
-                load_k(at);
-                pages.ask(a.pages, table, seen, t0 + 2 * kWaves * kTile, lane);
-                if constexpr (plain.value) {
-                    soften(x, a.scale, p);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < SETS; n++) shape(n, x[n], t0, valid, whole);
-                    soften(x, 1.0f, p);
-                    if (!whole) odd |= cut(valid);
-                }
-                add(p);
-                load_v(at);
-                tile += kWaves;
-            };
-            while (tile < end) {
-                while (simple && tile < end && open()) turn(std::true_type{});
-                if (tile < end) turn(std::false_type{});
-            }
+            if constexpr (kStaged) stage(k), next();
+            scores(k, x);
+            if constexpr (!kStaged) next();
+            pages.ask(a.pages, table, seen, t0 + 2 * WAVES * kTile, lane);
+            if (!simple) shape(x, t0);
+            if (!open) mask(x, t0, valid);
+            soften(x, p);
+            if (!open) odd |= cut(v, valid);
+            add(v, p);
+            load_v(v, at);
         }
+
         // Those values, added to the columns that see them (here, and not in their
         // tile: what the loop holds beside the sums leaves no registers for it).
-        for (tile = odd ? begin + wave : end; tile < end; tile += kWaves) {
+        auto page_of = [&](mfh_u32 t) { return (mfh_u32)table[a.pages.by_page.quotient(t)]; };
+        for (tile = odd ? begin + (WAVES > 1 ? wave : 0) : end; tile < end; tile += WAVES) {
             const mfh_u32 t0 = tile * kTile;
-            const bool open = t0 >= max(all_first, seen.first) && t0 + kTile <= min(all_length, seen.length);
-            bool whole = open;  // such a tile was not cut
+            // a tile that every column sees whole was not cut
+            bool whole = t0 >= max(all_first, seen.first) && t0 + kTile <= min(all_length, seen.length);
             for (mfh_u32 i = 0; i < kTile && whole; i++) whole = page_of(t0 + i) < a.pages.pages;
             for (mfh_u32 t = max(t0, seen.first); t < min(t0 + kTile, seen.length) && !whole; t++) {
                 const mfh_u32 page = page_of(t);
@@ -476,56 +541,90 @@ struct Part {
                             if (__builtin_isfinite(value)) continue;
 #pragma unroll
                             for (int n = 0; n < SETS; n++)
-                                if (t >= its_first[n] && t < its_length[n]) acc[n][u][d][x] += value;
+                                if (t >= its_first[n] && t < its_length[n]) acc[(n * kSets + u) * kDims + d][x] += value;
                         }
             }
         }
 
-        // The waves' results meet, as in decode.hip.
+        // C floats of each of a lane's four rows of dims, from dim on, and where they go
+        auto store = [&](auto values, int n, int dim, const f32x4* from) {
+            constexpr int kCount = values.value;
+            if (column(n) >= columns) return;
+            float* to = a.part_out + (row_of(n) * a.parts + slot) * a.dim;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int first = dim + kDims * (4 * quad + i);
+                if (first >= a.dim) continue;
+                typedef float Out __attribute__((ext_vector_type(kCount < 4 ? kCount : 4)));
+#pragma unroll
+                for (int c = 0; c < kCount; c += 4) {
+                    Out x;
+                    if constexpr (kCount == 1) x = from[0][i];
+                    else
+#pragma unroll
+                        for (int e = 0; e < (kCount < 4 ? kCount : 4); e++) x[e] = from[c + e][i];
+                    *reinterpret_cast<Out*>(to + first + c) = x;
+                }
+            }
+        };
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
             sum[n] += __shfl_xor(sum[n], 16);
             sum[n] += __shfl_xor(sum[n], 32);
-            const float wave_ref = limit[n] == -INFINITY ? -INFINITY : ref[n];
-            __syncthreads();
-            if (quad == 0) lds.ref[wave][col] = wave_ref, lds.sum[wave][col] = sum[n];
-            __syncthreads();
-            float top = lds.ref[0][col];
+            if (limit[n] == -INFINITY) ref[n] = -INFINITY;  // nothing seen, or nothing but NaN
+        }
+        if constexpr (WAVES == 1) {
 #pragma unroll
-            for (int w = 1; w < kWaves; w++) top = fmaxf(top, lds.ref[w][col]);
-            const float weight = wave_ref == -INFINITY ? 0.0f : exp2_fast(wave_ref - top);
-            const mfh_u32 first_column = column0 + 16 * n;
-            const int heads = first_column < columns ? (int)min((mfh_u32)kHeads, columns - first_column) : 0;
+            for (int n = 0; n < SETS; n++) {
 #pragma unroll
-            for (int u = 0; u < kSets; u++) {
-                if (u) __syncthreads();
+                for (int u = 0; u < kSets; u++)
+                    store(std::integral_constant<int, kDims>{}, n, u * kSetDims, acc + (n * kSets + u) * kDims);
+                if (quad == 0 && column(n) < columns) a.part_sum[row_of(n) * a.parts + slot] = make_float2(ref[n], sum[n]);
+            }
+            return;
+        }
+        // The waves' results meet: a common reference, and sums weighted by it, of which
+        // each wave adds up a quarter.  A wave without a reference has seen nothing,
+        // and its sum is 0, or nothing but NaN, and its sum is NaN: it is added as it
+        // stands, for the row is NaN then.
+        if (quad == 0) {
 #pragma unroll
-                for (int d = 0; d < kDims; d++)
+            for (int n = 0; n < SETS; n++) lds.ref[wave][n][col] = ref[n], lds.sum[wave][n][col] = sum[n];
+        }
+        __syncthreads();
+        float weight[SETS];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) lds.out[wave][col][kDims * (4 * quad + i) + d] = weight * acc[n][u][d][i];
-                __syncthreads();
-                const int dims = min(kSetDims, a.dim - u * kSetDims);
-                for (int i = threadIdx.x; i < heads * (kSetDims / 2); i += kThreads) {
-                    const int h = i / (kSetDims / 2), d = 2 * (i % (kSetDims / 2)), dim = u * kSetDims + d;
-                    if (d >= dims) continue;
-                    float o0 = 0.0f, o1 = 0.0f;
+        for (int n = 0; n < SETS; n++) {
+            float all = lds.ref[0][n][col], total = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < kWaves; w++) o0 += lds.out[w][h][d], o1 += lds.out[w][h][d + 1];
-                    const mfh_u32 c = first_column + h, member = a.by_group.quotient(c);
-                    const int64_t at = ((int64_t)(request0 + member) * a.q_heads + kv * a.group + (c - member * a.group)) * a.parts + slot;
-                    *reinterpret_cast<float2*>(a.part_out + at * a.dim + dim) = make_float2(o0, o1);
-                    if (dim == 0) {
-                        float all = lds.ref[0][h], total = 0.0f;
+            for (int w = 1; w < kWaves; w++) all = fmaxf(all, lds.ref[w][n][col]);
+            weight[n] = ref[n] == -INFINITY ? 0.0f : exp2_fast(ref[n] - all);
+            if (n % kWaves != wave) continue;
 #pragma unroll
-                        for (int w = 1; w < kWaves; w++) all = fmaxf(all, lds.ref[w][h]);
+            for (int w = 0; w < kWaves; w++) {
+                const float its = lds.ref[w][n][col];
+                total += its == -INFINITY ? lds.sum[w][n][col] : exp2_fast(its - all) * lds.sum[w][n][col];  // 0, or NaN
+            }
+            if (quad == 0 && column(n) < columns) a.part_sum[row_of(n) * a.parts + slot] = make_float2(all, total);
+        }
+        f32x4 mine[kGiven];
 #pragma unroll
-                        for (int w = 0; w < kWaves; w++)
-                            total += lds.ref[w][h] == -INFINITY ? lds.sum[w][h] : exp2_fast(lds.ref[w][h] - all) * lds.sum[w][h];  // 0, or NaN
-                        a.part_sum[at] = make_float2(all, total);
-                    }
-                }
+        for (int w = 0; w < kWaves; w++) {
+#pragma unroll
+            for (int c = 0; c < kGiven; c++) {
+                const int i = w * kGiven + c;
+                const f32x4 x = acc[i] * weight[i / (kSets * kDims)];
+                if (w == wave) mine[c] = x;
+                else lds.given[wave < w ? wave : wave - 1][i][lane] = x;
             }
         }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kGiven; c++)
+#pragma unroll
+            for (int g = 0; g < kWaves - 1; g++) mine[c] += lds.given[g][wave * kGiven + c][lane];
+        const int unit = wave * kGiven / kDims;
+        store(std::integral_constant<int, kGiven>{}, unit / kSets, unit % kSets * kSetDims + wave * kGiven % kDims, mine);
     }
 };
 
@@ -533,8 +632,8 @@ struct Part {
 template <int DT, bool FP8, int DP, bool FAST, int SETS>
 __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_shared(SharedArgs a)
 {
-    typedef Part<DT, FP8, DP, FAST, SETS> Common;
-    typedef Part<DT, FP8, DP, FAST, 1> Own;
+    typedef Part<DT, FP8, DP, FAST, SETS, kWaves> Common;
+    typedef Part<DT, FP8, DP, FAST, 1, kWaves> Own;
     __shared__ union {
         typename Common::Lds common;
         typename Own::Lds own;
@@ -548,27 +647,22 @@ __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ?
         const mfh_u32 kv = a.by_shared_parts.quotient(kv_part), part = kv_part - kv * a.shared_parts;
         if (kv >= (mfh_u32)a.kv_heads) return;
         constexpr mfh_u32 kColumns = kHeads * SETS;
-        mfh_u32 before = 0, g = ~0u, tile_of = 0;
+        Group group;
+        mfh_u32 before = 0, tile_of = ~0u;
         for (mfh_u32 base = 0; base < a.groups; base += 64) {
-            mfh_u32 its = 0;
-            if (base + lane < a.groups) {
-                const int from = min(max(a.starts[base + lane], 0), (int)a.requests);
-                its = ((mfh_u32)(min(max(a.starts[base + lane + 1], from), (int)a.requests) - from) * a.group + kColumns - 1) / kColumns;
-            }
-            const mfh_u32 upto = before + lanes_upto(its);
+            const typename Group::Lanes lanes(a, base, lane);
+            const mfh_u32 its = ((lanes.end - lanes.begin) * a.group + kColumns - 1) / kColumns, upto = before + lanes_upto(its);
             const mfh_u64 past = __ballot(upto > line);
             if (past) {
                 const int at = __ffsll((unsigned long long)past) - 1;
-                g = base + at;
                 tile_of = line - ((mfh_u32)__builtin_amdgcn_readlane((int)upto, at) - (mfh_u32)__builtin_amdgcn_readlane((int)its, at));
+                group.of(a, lanes, at, lane);
                 break;
             }
             before = last_lane(upto);
         }
-        if (g == ~0u) return;
-        g = uniform(g), tile_of = uniform(tile_of);
-        Group group;
-        group.of(a, g, lane);
+        if (tile_of == ~0u) return;
+        tile_of = uniform(tile_of);
         const Tiles tiles(group, a.by_shared_piece, a.shared_parts);
         if (part >= tiles.parts) return;
         const mfh_u32 share = uniform((tiles.count + tiles.parts - 1) / tiles.parts);
@@ -589,9 +683,8 @@ __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ?
     const Tiles tiles(own, a.by_own_piece, a.own_parts);
     if (part >= tiles.parts) return;
     const mfh_u32 share = uniform((tiles.count + tiles.parts - 1) / tiles.parts);
-    Own::run(a, lds.own, r, 1, head_group * kHeads, kv, own, r,
-             tiles.first + min(part * share, tiles.count), tiles.first + min((part + 1) * share, tiles.count),
-             a.shared_parts + part);
+    Own::run(a, lds.own, r, 1, head_group * kHeads, kv, own, r, tiles.first + min(part * share, tiles.count),
+             tiles.first + min((part + 1) * share, tiles.count), a.shared_parts + part);
 }
 
 // Joins a row's parts, of the shared tokens and of its own.  A workgroup takes
