@@ -103,7 +103,8 @@ struct Logit {
 };
 
 // The `picks` largest of a workgroup's elements, in order, into `best` behind a
-// barrier.  each(f) calls f for every element of the thread; top is the largest.
+// barrier.  each(least, f) calls f for every element of the thread, but may leave out
+// lower ones than `least`; top is the largest.
 template <typename K>
 struct Selection {
     K by_wave[kWaves][64];
@@ -140,7 +141,7 @@ struct Selection {
         __syncthreads();
         const K least = bound;
         if (top.some() && top >= least)
-            each([&](K k) {
+            each(least, [&](K k) {
                 if (k.some() && k >= least) {
                     const mfh_u32 at = atomicAdd(&count, 1u);
                     if (at < kList) list[at] = k;
@@ -160,7 +161,7 @@ struct Selection {
         K last = K::all();
         for (mfh_u32 i = 0; i < picks; i++) {
             K most = K::none();
-            each([&](K k) {
+            each(K::none(), [&](K k) {
                 if (last > k && k > most) most = k;
             });
 #pragma unroll
@@ -193,7 +194,7 @@ MFH_DEV float logit_of(const u32x4& p, int e)
 
 // PACKETS: of 16 bytes in a thread's registers.
 template <int DT, int PACKETS>
-__global__ __launch_bounds__(kThreads) void k_beam_rows(BeamArgs a)
+__global__ __launch_bounds__(kThreads, 8) void k_beam_rows(BeamArgs a)
 {
     constexpr int P = kPacket<DT>, kBytes = 16 / P;
     __shared__ Selection<Logit> s;
@@ -208,21 +209,24 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(BeamArgs a)
     auto token_of = [&](int i) { return ((piece * PACKETS + i) * kThreads + threadIdx.x) * P; };
 
     u32x4 packet[PACKETS];
+    if ((mfh_u64)(piece + 1) * (PACKETS * kThreads * P) <= a.vocab) {
 #pragma unroll
-    for (int i = 0; i < PACKETS; i++) {
-        const mfh_u32 t = token_of(i);
-        if (t + P <= a.vocab) {
-            packet[i] = load16<true>(from + (int64_t)t * kBytes);
-        } else {  // past the end: -inf
+        for (int i = 0; i < PACKETS; i++) packet[i] = load16<true>(from + (int64_t)token_of(i) * kBytes);
+    } else {  // a row's last piece: -inf past its end
+        constexpr mfh_u32 kLowest = DT == kFloat32 ? 0xff800000u : DT == kBFloat16 ? 0xff80ff80u : 0xfc00fc00u;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                if constexpr (DT == kFloat32) {
-                    packet[i][w] = t + w < a.vocab ? load4(from + (int64_t)(t + w) * 4) : 0xff800000u;
-                } else {
-                    constexpr mfh_u32 kLowest = DT == kBFloat16 ? 0xff80u : 0xfc00u;
-                    const mfh_u32 lo = t + 2 * w < a.vocab ? load2(from + (int64_t)(t + 2 * w) * 2) : kLowest;
-                    const mfh_u32 hi = t + 2 * w + 1 < a.vocab ? load2(from + (int64_t)(t + 2 * w + 1) * 2) : kLowest;
-                    packet[i][w] = lo | hi << 16;
+        for (int i = 0; i < PACKETS; i++) {
+            const mfh_u32 t = token_of(i);
+            packet[i] = u32x4{kLowest, kLowest, kLowest, kLowest};
+            if (t + P <= a.vocab) {
+                packet[i] = load16<true>(from + (int64_t)t * kBytes);
+            } else if (t < a.vocab) {
+#pragma unroll
+                for (int e = 0; e < P; e++) {
+                    if (t + e >= a.vocab) continue;
+                    if constexpr (DT == kFloat32) packet[i][e] = load4(from + (int64_t)(t + e) * 4);
+                    else packet[i][e / 2] = e & 1 ? (packet[i][e / 2] & 0xffffu) | load2(from + (int64_t)(t + e) * 2) << 16
+                                                  : (packet[i][e / 2] & 0xffff0000u) | load2(from + (int64_t)(t + e) * 2);
                 }
             }
         }
@@ -237,7 +241,15 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(BeamArgs a)
 #pragma unroll
         for (int e = 1; e < P; e++) most = fmaxf(most, logit_of<DT>(packet[i], e));
         if (most > top) top = most, at = i;
+        
     }
+    // (unpacked anew for each of its uses: kept unpacked, a workgroup's registers would
+    // leave room for no other one)
+    auto packed = [&]() {
+#pragma unroll
+        for (int i = 0; i < PACKETS; i++) asm volatile("" : "+v"(packet[i]));
+    };
+    packed();
     // sum of exponentials below the wave's largest; NaN and +inf make it NaN
     float wave_top = top;
 #pragma unroll
@@ -245,9 +257,12 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(BeamArgs a)
     const float base = wave_top == -INFINITY ? 0.0f : wave_top;
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < PACKETS; i++)
+    for (int i = 0; i < PACKETS; i++) {
 #pragma unroll
         for (int e = 0; e < P; e++) part[e % 4] += exp2_fast((logit_of<DT>(packet[i], e) - base) * kLog2e);
+        
+    }
+    packed();
     double sum = (double)(part[0] + part[1]) + (double)(part[2] + part[3]);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
@@ -260,14 +275,22 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(BeamArgs a)
 #pragma unroll
     for (int e = P - 1; e >= 0; e--) in_packet = logit_of<DT>(with_top, e) == top ? e : in_packet;
     const Logit best{top > -INFINITY ? logit_key(top, token_of(at) + in_packet) : 0};
-    s.run(a.picks, best, s_best, [&](auto f) {
+    s.run(a.picks, best, s_best, [&](const Logit& least, auto f) {
+        const float above = least.some() ? unordered((mfh_u32)(least.key >> 32)) : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < PACKETS; i++)
+        for (int i = 0; i < PACKETS; i++) {
+            float most = logit_of<DT>(packet[i], 0);
+#pragma unroll
+            for (int e = 1; e < P; e++) most = fmaxf(most, logit_of<DT>(packet[i], e));
+            if (!(most >= above)) continue;
+            mfh_u32 token = token_of(i);
+            asm volatile("" : "+v"(packet[i]), "+v"(token));  // nothing of it ahead of the question
 #pragma unroll
             for (int e = 0; e < P; e++) {
                 const float x = logit_of<DT>(packet[i], e);
-                if (x > -INFINITY) f(Logit{logit_key(x, token_of(i) + e)});
+                if (x > -INFINITY) f(Logit{logit_key(x, token + e)});
             }
+        }
     });
     __syncthreads();
     if (threadIdx.x < a.picks) a.best[(int64_t)blockIdx.x * a.picks + threadIdx.x] = s_best[threadIdx.x].key;
@@ -338,14 +361,14 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
         const mfh_u64 low = (mfh_u64)(kMostBeams - 1 - b) << 56 | (key >> 32) << kTokenBits | (key & ((1u << kTokenBits) - 1));
         return Key{ordered(score), low};
     };
-    auto each = [&](auto f) {
+    auto each = [&](const Key&, auto f) {
         for (mfh_u32 n = threadIdx.x; n < lists * a.picks; n += kThreads) {
             const Key k = candidate(n);
             if (k.some()) f(k);
         }
     };
     Key top = Key::none();
-    each([&](Key k) { top = k > top ? k : top; });
+    each(Key::none(), [&](Key k) { top = k > top ? k : top; });
     s.run(a.picks, top, s_best, each);
     __syncthreads();
 
