@@ -61,6 +61,16 @@ MFH_DEV mfh_u32 enc16x2(float lo, float hi)
     else return mfh_f16x2_rne(lo, hi);
 }
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// Four 16-bit values of one column: in each 16 lanes, lane i gives the address
+// of four values of row i / 4, columns 4 (i % 4) .., and gets column i's.
+MFH_DEV u32x2 read_column(const char* at)
+{
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at)));
+}
+
 // The top bits of those halves of a dword that are infinite or NaN: an exponent
 // of ones carries into them.
 template <int DT>

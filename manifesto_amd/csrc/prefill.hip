@@ -57,16 +57,6 @@ struct PrefillArgs {
     Divider by_group, by_kv_heads, by_row_tiles, by_parts, by_q_heads;
 };
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-// Four 16-bit values of one column: in each 16 lanes, lane i gives the address
-// of four values of row i / 4, columns 4 (i % 4) .., and gets column i's.
-MFH_DEV u32x2 read_column(const char* at)
-{
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at)));
-}
-
 // Where 16 bytes of a row stand among the row's pieces in LDS.  Rows have no gaps
 // (with them two workgroups of heads of 64 would not fit a CU's LDS), so pieces
 // change places by row: 16 rows of one piece, as K is read, lie in 16 different

@@ -129,35 +129,38 @@ struct Tiles {
 // workgroup that take the tiles in turn; 1: the wave is alone.
 template <int DT, bool FP8, int DP, bool FAST, int SETS, int WAVES>
 struct Part {
+    static constexpr int kBytes = FP8 ? 1 : 2;
     static constexpr int kSteps = DP / 32;                    // of the product with K
     static constexpr int kLoads = FP8 ? kSteps / 2 : kSteps;  // of 16 bytes of a token of K
-    static constexpr int kSets = DP == 64 ? 1 : DP / 128;     // of 16 lanes' dims in V
-    static constexpr int kDims = DP == 64 ? 4 : 8;            // of a lane in a set
-    static constexpr int kBytes = FP8 ? 1 : 2;
-    static constexpr int kSetDims = 16 * kDims;
-    static constexpr int kSums = SETS * kSets * kDims;        // registers of four sums
+    static constexpr int kDimTiles = DP / 16;
+    static constexpr int kSums = SETS * kDimTiles;            // registers of four sums
     static constexpr int kGiven = kSums / kWaves;             // of a wave where all meet
-    typedef typename Piece<FP8, kDims>::type VPiece;
+    static constexpr int kPieces = DP * kBytes / 16;          // of 16 bytes in a row
+    static constexpr int kRowsAtOnce = 64 / kPieces;          // of a load
+    static constexpr int kRaw = 32 / kRowsAtOnce;
+    static constexpr int kKinds = 16 / kRowsAtOnce;           // of lanes' places in a page
+    static constexpr int kPitch = DP * 2;                     // of a row of V in LDS, in bytes
     // Shared tokens are read by several workgroups where their columns fill more than
     // one: nt would keep them out of the L2.
     static constexpr int kPolicy = SETS > 1 ? 0 : kStreamed;
-    // Keys go through LDS where other workgroups read them too.  As the products take
-    // them 16 lanes read 16 rows, and the texture unit takes a lane at a time: a
-    // quarter of what it does for whole rows, which is enough for memory, but not for the
-    // L2 (256 requests over 16384 tokens, 178 us so).
-    static constexpr bool kStaged = SETS > 1;
-    static constexpr int kPieces = DP * kBytes / 16;          // of a row of K
-    static constexpr int kRowsAtOnce = 64 / kPieces;          // of a load
-    static constexpr int kRaw = kStaged ? 32 / kRowsAtOnce : 1;
     struct Lds {
         float ref[kWaves][SETS][kHeads], sum[kWaves][SETS][kHeads];
         union {
-            u32x4 k[kStaged ? kWaves : 1][kStaged ? 32 * kPieces : 1];
+            struct {
+                u32x4 k[32 * kPieces];
+                u32x4 v[32 * kPitch / 16];
+            } tile[kWaves];
             f32x4 given[WAVES > 1 ? kWaves - 1 : 1][WAVES > 1 ? kSums : 1][64];
         };
     };
-    // Where piece c of row r stands in LDS among the row's: 16 rows' in 16 places.
-    static MFH_DEV int place(int r, int c) { return c ^ ((kPieces < 16 ? r / (16 / kPieces) : r) & (kPieces < 16 ? kPieces - 1 : 15)); }
+    // Where piece c of row r stands in LDS among the PIECES of the row: 16 rows'
+    // pieces in 16 different places, as K is read, and so two of each in V.
+    template <int PIECES>
+    static MFH_DEV int place(int r, int c)
+    {
+        if constexpr (PIECES >= 16) return c ^ (r & 15);
+        else return c ^ (r / (16 / PIECES) & (PIECES - 1));
+    }
 
     static MFH_DEV void run(const SharedArgs& a, Lds& lds, mfh_u32 request0, mfh_u32 members, mfh_u32 column0, mfh_u32 kv,
                             const Seen& seen, mfh_u32 table_row, mfh_u32 begin, mfh_u32 end, mfh_u32 slot)
@@ -199,89 +202,48 @@ struct Part {
             }
         }
 
+        // A load takes whole rows, a piece a lane; where it goes to LDS as it is, the
+        // lane takes the piece whose place it fills.  Pieces past head_dim are zeros, which
+        // buffer loads past every page's end give, or else the row's last one again,
+        // cut below.
         const mfh_u32 token_bytes = a.pages.token_bytes;
-        // Lanes past head_dim have zeros in Q and in K: buffer loads past every page's
-        // end give them, else they read its last dims again, inside the row, and
-        // are cut.  In V they do so too, their results are not written.
-        constexpr int kKinds = kStaged ? 16 / kRowsAtOnce : kLoads;  // of lanes' places in K
-        mfh_u32 k_lane[kKinds], v_lane[kSets];
-        const int last = a.dim - 16 / kBytes;
+        mfh_u32 k_lane[kKinds], v_lane[kKinds];
+        const int last = a.dim * kBytes - 16;
 #pragma unroll
         for (int s = 0; s < kKinds; s++) {
-            // staged: of row kRowsAtOnce * s + lane / kPieces the piece whose place this lane fills
-            const int row = kStaged ? lane / kPieces : col;
-            const int d = kStaged ? place(kRowsAtOnce * s + row, lane % kPieces) * (16 / kBytes) : FP8 ? 64 * s + 16 * quad : 32 * s + 8 * quad;
-            k_lane[s] = FAST ? d <= last ? row * token_bytes + d * kBytes : 1u << 31 : min(d, last) * kBytes;
+            const int row = lane / kPieces, own = lane % kPieces;
+            auto at_piece = [&](int c) {
+                return FAST ? 16 * c <= last ? row * token_bytes + 16 * c : 1u << 31 : (mfh_u32)min(16 * c, last);
+            };
+            k_lane[s] = at_piece(place<kPieces>(kRowsAtOnce * s + row, own));
+            v_lane[s] = FP8 ? at_piece(own) : k_lane[s];
         }
-        int k_at[kLoads];  // in LDS
-#pragma unroll
-        for (int s = 0; s < kLoads; s++) k_at[s] = col * kPieces + place(col, 4 * s + quad);
-#pragma unroll
-        for (int u = 0; u < kSets; u++)
-            v_lane[u] = (FAST ? 4 * quad * token_bytes : 0) + min(u * kSetDims + kDims * col, a.dim - kDims) * kBytes;
         const bool ragged = a.dim != DP;
         const char* k_base = a.pages.k + kv * a.pages.head_bytes;
         const char* v_base = a.pages.v + kv * a.pages.head_bytes;
-
-        // Staged: rows as they stand in memory; else the products' operands.
-        typedef u32x4 Keys[kStaged ? kRaw : 2 * kLoads];
-        typedef VPiece Values[kSets][8];
-        auto load_k = [&](Keys& k, const TileAt<FAST>& at) {
+        typedef u32x4 Rows[kRaw];
+        auto load = [&](Rows& raw, const char* base, const mfh_u32 (&at_lane)[kKinds], const TileAt<FAST>& at) {
             if constexpr (FAST) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const __amdgpu_buffer_rsrc_t rows = page_buffer(k_base, at.page[h], a.pages);
-                    if constexpr (kStaged) {
+                    const __amdgpu_buffer_rsrc_t rows = page_buffer(base, at.page[h], a.pages);
 #pragma unroll
-                        for (int s = 0; s < kKinds; s++)
-                            k[h * kKinds + s] = buffer_piece<u32x4, kPolicy>(rows, k_lane[s], at.in_page[h] + s * kRowsAtOnce * token_bytes);
-                    } else {
-#pragma unroll
-                        for (int s = 0; s < kLoads; s++) k[h * kLoads + s] = buffer_piece<u32x4, kPolicy>(rows, k_lane[s], at.in_page[h]);
-                    }
+                    for (int s = 0; s < kKinds; s++)
+                        raw[h * kKinds + s] = buffer_piece<u32x4, kPolicy>(rows, at_lane[s], at.in_page[h] + s * kRowsAtOnce * token_bytes);
                 }
-            } else if constexpr (kStaged) {
+            } else {
 #pragma unroll
                 for (int i = 0; i < kRaw; i++)
-                    k[i] = load16<kPolicy == kStreamed>(k_base + shuffle64(at.mine, i * kRowsAtOnce + lane / kPieces) + k_lane[i % kKinds]);
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const char* row = k_base + shuffle64(at.mine, 16 * h + col);
-#pragma unroll
-                    for (int s = 0; s < kLoads; s++) k[h * kLoads + s] = load16<kPolicy == kStreamed>(row + k_lane[s]);
-                }
+                    raw[i] = load16<kPolicy == kStreamed>(base + shuffle64(at.mine, i * kRowsAtOnce + lane / kPieces) + at_lane[i % kKinds]);
             }
         };
-        auto load_v = [&](Values& v, const TileAt<FAST>& at) {
-            if constexpr (FAST) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const __amdgpu_buffer_rsrc_t rows = page_buffer(v_base, at.page[h], a.pages);
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int u = 0; u < kSets; u++)
-                            v[u][4 * h + j] = buffer_piece<VPiece, kPolicy>(rows, v_lane[u], at.in_page[h] + j * token_bytes);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const char* row = v_base + shuffle64(at.mine, 16 * (j >> 2) + 4 * quad + (j & 3));
-#pragma unroll
-                    for (int u = 0; u < kSets; u++) v[u][j] = load_piece<VPiece, kPolicy == kStreamed>(row + v_lane[u]);
-                }
-            }
-        };
-        // One tile's registers: the next tile's keys set out when this one's are used up
-        // (or in LDS), and its values then too.  Loads of a tile past the last one are
-        // made too, and move nothing: behind loads that only some waves or rounds
-        // make, the compiler waits for all that are on their way.
-        Keys k;
-        Values v;
+        // One tile's registers: the next tile sets out when this one is in LDS.  Loads of
+        // a tile past the last one are made too, and move nothing: behind loads that only
+        // some waves or rounds make, the compiler waits for all that are on their way.
+        Rows k, v;
         TileAt<FAST> at = pages.place(a.pages, seen, tile * kTile, lane, tile < end);
-        load_k(k, at);
-        load_v(v, at);
+        load(k, k_base, k_lane, at);
+        load(v, v_base, v_lane, at);
         pages.ask(a.pages, table, seen, (tile + WAVES) * kTile, lane);
 
 #pragma unroll
@@ -304,32 +266,26 @@ struct Part {
                 for (int s = 0; s < kSteps; s++) asm volatile("" : "+a"(q[n][s]));
         }
 
-        f32x4 acc[kSums];  // [set][set of dims][dim]
+        f32x4 acc[kSums];  // [set][tile of 16 dims]: dims 4 quad .. of the tile
         float ref[SETS], limit[SETS], sum[SETS];
 #pragma unroll
         for (int n = 0; n < SETS; n++) ref[n] = 0.0f, limit[n] = -INFINITY, sum[n] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSums; i++) acc[i] = f32x4{0, 0, 0, 0};
-        auto stage = [&](const Keys& k) {
-            if constexpr (kStaged) {
-#pragma unroll
-                for (int i = 0; i < kRaw; i++) lds.k[wave][i * 64 + lane] = k[i];
-            }
-        };
-        auto scores = [&](const Keys& k, float (&x)[SETS][8]) {
+
+        auto& mine = lds.tile[wave];
+        const int k_at = col * kPieces + place<kPieces>(col, quad);  // pieces 4 s + quad of rows col and 16 + col
+        auto scores = [&](float (&x)[SETS][8]) {
             f32x4 s0[SETS], s1[SETS];
 #pragma unroll
             for (int n = 0; n < SETS; n++) s0[n] = s1[n] = f32x4{0, 0, 0, 0};
             u32x4 from[2][kLoads];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int s = 0; s < kLoads; s++)
 #pragma unroll
-                for (int s = 0; s < kLoads; s++) {
-                    if constexpr (kStaged) from[h][s] = lds.k[wave][16 * kPieces * h + k_at[s]];
-                    else from[h][s] = k[h * kLoads + s];
-                }
+                for (int h = 0; h < 2; h++) from[h][s] = mine.k[16 * kPieces * h + (k_at ^ (4 * s))];
             // (left to itself the compiler reads right ahead of each product, and waits there)
-            if constexpr (kStaged) __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);
             auto product = [&](auto cut) {
 #pragma unroll
                 for (int s = 0; s < kSteps; s++) {
@@ -414,7 +370,7 @@ struct Part {
                         limit[n] = top[n] + kStep;
                         sum[n] *= alpha;
 #pragma unroll
-                        for (int i = 0; i < kSets * kDims; i++) acc[n * kSets * kDims + i] *= alpha;
+                        for (int i = 0; i < kDimTiles; i++) acc[n * kDimTiles + i] *= alpha;
                     }
                 }
             }
@@ -440,54 +396,62 @@ struct Part {
         };
         // Cuts values to zero that are of no token (0 * NaN would be NaN) or not
         // finite; whether there are any of those.
-        auto cut = [&](Values& v, mfh_u32 valid) {
+        auto cut = [&](mfh_u32 valid) {
             bool odd = false;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const bool keep = valid >> (16 * (j >> 2) + 4 * quad + (j & 3)) & 1;
+            for (int i = 0; i < kRaw; i++) {
+                const bool keep = valid >> (i * kRowsAtOnce + lane / kPieces) & 1;
 #pragma unroll
-                for (int u = 0; u < kSets; u++) {
-                    constexpr int kWords = sizeof(VPiece) / 4;
-                    typedef mfh_u32 Words __attribute__((ext_vector_type(kWords)));
-                    Words w = __builtin_bit_cast(Words, v[u][j]);
-#pragma unroll
-                    for (int i = 0; i < kWords; i++) {
-                        mfh_u32 whole;
-                        if constexpr (FP8) {
-                            const mfh_u32 tops = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                            whole = tops | (tops - (tops >> 7));
-                        } else {
-                            const mfh_u32 tops = not_finite<DT>(w[i]);
-                            whole = tops | (tops - (tops >> 15));
-                        }
-                        odd |= keep && whole != 0;
-                        w[i] &= keep ? ~whole : 0u;
+                for (int w = 0; w < 4; w++) {
+                    mfh_u32 whole;
+                    if constexpr (FP8) {
+                        const mfh_u32 tops = ((v[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                        whole = tops | (tops - (tops >> 7));
+                    } else {
+                        const mfh_u32 tops = not_finite<DT>(v[i][w]);
+                        whole = tops | (tops - (tops >> 15));
                     }
-                    v[u][j] = __builtin_bit_cast(VPiece, w);
+                    odd |= keep && whole != 0;
+                    v[i][w] &= keep ? ~whole : 0u;
                 }
             }
             return __any(odd);
         };
-        auto add = [&](const Values& v, const u32x4 (&p)[SETS]) {
+        auto stage = [&]() {
 #pragma unroll
-            for (int u = 0; u < kSets; u++) {
-                u32x4 t[8];
+            for (int i = 0; i < kRaw; i++) mine.k[i * 64 + lane] = k[i];
 #pragma unroll
-                for (int j = 0; j < 8; j++) t[j] = dims_of<DT, FP8, kDims>(v[u][j]);
+            for (int i = 0; i < kRaw; i++) {
+                if constexpr (FP8) {
+                    const int row = i * kRowsAtOnce + lane / kPieces, c = 2 * (lane % kPieces);
 #pragma unroll
-                for (int d = 0; d < kDims; d += 2) {
-                    const int i = d / 2;
-                    const u32x4 even = {low_halves(t[0][i], t[1][i]), low_halves(t[2][i], t[3][i]),
-                                        low_halves(t[4][i], t[5][i]), low_halves(t[6][i], t[7][i])};
-                    const u32x4 other = {high_halves(t[0][i], t[1][i]), high_halves(t[2][i], t[3][i]),
-                                         high_halves(t[4][i], t[5][i]), high_halves(t[6][i], t[7][i])};
-#pragma unroll
-                    for (int n = 0; n < SETS; n++) {
-                        f32x4* to = acc + (n * kSets + u) * kDims + d;
-                        to[0] = mfma16<DT>(even, p[n], to[0]);
-                        to[1] = mfma16<DT>(other, p[n], to[1]);
-                    }
+                    for (int e = 0; e < 2; e++)
+                        mine.v[row * 2 * kPieces + place<2 * kPieces>(row, c + e)] = widen<DT>(v[i][2 * e], v[i][2 * e + 1]);
+                } else {
+                    mine.v[i * 64 + lane] = v[i];
                 }
+            }
+        };
+        // V^T of 32 tokens, in the order of the weights, and 16 dims: see read_column.
+        const int v_row = 4 * quad + (lane & 15) / 4;
+        const int v_at = v_row * kPitch + place<DP / 8>(v_row, (lane & 3) / 2) * 16 + 8 * (lane & 1);
+        auto add = [&](const u32x4 (&p)[SETS]) {
+            const char* from = reinterpret_cast<const char*>(mine.v);
+            constexpr int kAhead = kDimTiles < 4 ? kDimTiles : 4;
+            u32x4 piece[kDimTiles];
+            auto read = [&](int d) {
+                const u32x2 lo = read_column(from + (v_at ^ (32 * d))), hi = read_column(from + 16 * kPitch + (v_at ^ (32 * d)));
+                piece[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            };
+#pragma unroll
+            for (int d = 0; d < kAhead; d++) read(d);
+#pragma unroll
+            for (int d = 0; d < kDimTiles; d++) {
+                if (d + kAhead < kDimTiles) read(d + kAhead);
+                if constexpr (SETS > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < SETS; n++) acc[n * kDimTiles + d] = mfma16<DT>(piece[d], p[n], acc[n * kDimTiles + d]);
+                if constexpr (SETS > 1) __builtin_amdgcn_sched_barrier(0);
             }
         };
 
@@ -497,20 +461,17 @@ struct Part {
             const bool open = valid == 0xffffffffu && t0 >= all_first && t0 + kTile <= all_length;  // to every column
             float x[SETS][8];
             u32x4 p[SETS];
-            auto next = [&]() {
-                at = pages.place(a.pages, seen, t0 + WAVES * kTile, lane, tile + WAVES < end);
-                load_k(k, at);
-            };
-            if constexpr (kStaged) stage(k), next();
-            scores(k, x);
-            if constexpr (!kStaged) next();
+            if (!open) odd |= cut(valid);
+            stage();
+            at = pages.place(a.pages, seen, t0 + WAVES * kTile, lane, tile + WAVES < end);
+            load(k, k_base, k_lane, at);
+            load(v, v_base, v_lane, at);
+            scores(x);
             pages.ask(a.pages, table, seen, t0 + 2 * WAVES * kTile, lane);
             if (!simple) shape(x, t0);
             if (!open) mask(x, t0, valid);
             soften(x, p);
-            if (!open) odd |= cut(v, valid);
-            add(v, p);
-            load_v(v, at);
+            add(p);
         }
 
         // Those values, added to the columns that see them (here, and not in their
@@ -527,45 +488,27 @@ struct Part {
                 const char* row = v_base + (mfh_u64)page * a.pages.page_bytes +
                                   (t - a.pages.by_page.quotient(t) * a.pages.by_page.d) * token_bytes;
 #pragma unroll
-                for (int u = 0; u < kSets; u++)
+                for (int d = 0; d < kDimTiles; d++)
 #pragma unroll
-                    for (int d = 0; d < kDims; d++)
+                    for (int x = 0; x < 4; x++) {
+                        const int dim = 16 * d + 4 * quad + x;
+                        if (dim >= a.dim) continue;
+                        mfh_u32 code;
+                        if constexpr (FP8) code = e4m3_pair<DT, false>(*reinterpret_cast<const uint8_t*>(row + dim)) & 0xffffu;
+                        else code = load2(row + dim * 2);
+                        const float value = dec16<DT>(code);
+                        if (__builtin_isfinite(value)) continue;
 #pragma unroll
-                        for (int x = 0; x < 4; x++) {
-                            const int dim = u * kSetDims + kDims * (4 * quad + x) + d;
-                            if (dim >= a.dim) continue;
-                            mfh_u32 code;
-                            if constexpr (FP8) code = e4m3_pair<DT, false>(*reinterpret_cast<const uint8_t*>(row + dim)) & 0xffffu;
-                            else code = load2(row + dim * 2);
-                            const float value = dec16<DT>(code);
-                            if (__builtin_isfinite(value)) continue;
-#pragma unroll
-                            for (int n = 0; n < SETS; n++)
-                                if (t >= its_first[n] && t < its_length[n]) acc[(n * kSets + u) * kDims + d][x] += value;
-                        }
+                        for (int n = 0; n < SETS; n++)
+                            if (t >= its_first[n] && t < its_length[n]) acc[n * kDimTiles + d][x] += value;
+                    }
             }
         }
 
-        // C floats of each of a lane's four rows of dims, from dim on, and where they go
-        auto store = [&](auto values, int n, int dim, const f32x4* from) {
-            constexpr int kCount = values.value;
-            if (column(n) >= columns) return;
-            float* to = a.part_out + (row_of(n) * a.parts + slot) * a.dim;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int first = dim + kDims * (4 * quad + i);
-                if (first >= a.dim) continue;
-                typedef float Out __attribute__((ext_vector_type(kCount < 4 ? kCount : 4)));
-#pragma unroll
-                for (int c = 0; c < kCount; c += 4) {
-                    Out x;
-                    if constexpr (kCount == 1) x = from[0][i];
-                    else
-#pragma unroll
-                        for (int e = 0; e < (kCount < 4 ? kCount : 4); e++) x[e] = from[c + e][i];
-                    *reinterpret_cast<Out*>(to + first + c) = x;
-                }
-            }
+        auto store = [&](int i, const f32x4& x) {  // register i of acc
+            const int n = i / kDimTiles, dim = 16 * (i % kDimTiles) + 4 * quad;
+            if (column(n) < columns && dim < a.dim)
+                *reinterpret_cast<f32x4*>(a.part_out + (row_of(n) * a.parts + slot) * a.dim + dim) = x;
         };
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
@@ -577,8 +520,7 @@ struct Part {
 #pragma unroll
             for (int n = 0; n < SETS; n++) {
 #pragma unroll
-                for (int u = 0; u < kSets; u++)
-                    store(std::integral_constant<int, kDims>{}, n, u * kSetDims, acc + (n * kSets + u) * kDims);
+                for (int d = 0; d < kDimTiles; d++) store(n * kDimTiles + d, acc[n * kDimTiles + d]);
                 if (quad == 0 && column(n) < columns) a.part_sum[row_of(n) * a.parts + slot] = make_float2(ref[n], sum[n]);
             }
             return;
@@ -607,24 +549,24 @@ struct Part {
             }
             if (quad == 0 && column(n) < columns) a.part_sum[row_of(n) * a.parts + slot] = make_float2(all, total);
         }
-        f32x4 mine[kGiven];
+        f32x4 total[kGiven];
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
 #pragma unroll
             for (int c = 0; c < kGiven; c++) {
                 const int i = w * kGiven + c;
-                const f32x4 x = acc[i] * weight[i / (kSets * kDims)];
-                if (w == wave) mine[c] = x;
+                const f32x4 x = acc[i] * weight[i / kDimTiles];
+                if (w == wave) total[c] = x;
                 else lds.given[wave < w ? wave : wave - 1][i][lane] = x;
             }
         }
         __syncthreads();
 #pragma unroll
-        for (int c = 0; c < kGiven; c++)
+        for (int c = 0; c < kGiven; c++) {
 #pragma unroll
-            for (int g = 0; g < kWaves - 1; g++) mine[c] += lds.given[g][wave * kGiven + c][lane];
-        const int unit = wave * kGiven / kDims;
-        store(std::integral_constant<int, kGiven>{}, unit / kSets, unit % kSets * kSetDims + wave * kGiven % kDims, mine);
+            for (int g = 0; g < kWaves - 1; g++) total[c] += lds.given[g][wave * kGiven + c][lane];
+            store(wave * kGiven + c, total[c]);
+        }
     }
 };
 
@@ -757,14 +699,14 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     const int64_t columns = (int64_t)requests * group, each = groups > 0 ? columns / groups : 0;
     l.sets = each <= 16 ? 1 : c.head_dim > 128 ? 2 : 4;
     l.lines = columns / (kHeads * l.sets) + groups;
-    auto split = [&](int64_t rows, int64_t tokens, mfh_u32& piece, mfh_u32& parts) {
+    auto split = [&](int64_t blocks, int64_t rows, int64_t tokens, mfh_u32& piece, mfh_u32& parts) {
         const int64_t tiles = (std::min<int64_t>(std::max<int64_t>(tokens, 1), kLongest) + kTile - 1) / kTile + 1;
-        const int64_t wanted = std::max<int64_t>(1, 2 * dev->compute_units / std::max<int64_t>(rows, 1));
+        const int64_t wanted = std::max<int64_t>(1, blocks / std::max<int64_t>(rows, 1));
         piece = (mfh_u32)std::max<int64_t>(8, (tiles + wanted - 1) / wanted);
         parts = (mfh_u32)((tiles + piece - 1) / piece);
     };
-    split(std::max<int64_t>(groups, columns / (kHeads * l.sets)) * c.kv_heads, most_shared, l.shared_piece, l.shared_parts);
-    split((int64_t)requests * c.kv_heads, most_own, l.own_piece, l.own_parts);
+    split((l.sets > 1 ? 1 : 2) * dev->compute_units, std::max<int64_t>(groups, columns / (kHeads * l.sets)) * c.kv_heads, most_shared, l.shared_piece, l.shared_parts);
+    split(2 * dev->compute_units, (int64_t)requests * c.kv_heads, most_own, l.own_piece, l.own_parts);
     if (groups == 0) l.shared_parts = 0;
     l.shared_blocks = ((int64_t)c.kv_heads * l.shared_parts + 7) / 8 * 8 * l.lines;
     l.own_blocks = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads) * l.own_parts;
