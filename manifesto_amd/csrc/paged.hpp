@@ -191,6 +191,16 @@ struct PageArgs {
     }
 };
 
+// Attention of requests with one new token each to the tokens that their groups
+// share, by prefill.hip's kernels: sums and references of `parts` parts of each row
+// (request * q_heads + head) go to the first of its part_slots slots; a part that
+// saw nothing has the reference -inf and the sum 0, and no sums.
+int prefill_rows(int dim);  // of a workgroup
+int prefill_shared(const mfh_attention_shape& shape, const mfh_kv_cache& cache, const PageArgs& pages, int32_t requests,
+                   int32_t groups, const void* q, const int32_t* starts, const int32_t* shared, const int32_t* lengths,
+                   const float* slopes, mfh_u32 parts, mfh_u32 part_slots, float* part_out, float2* part_sum,
+                   hipStream_t s);
+
 MFH_DEV mfh_i64 shuffle64(mfh_i64 v, int lane)
 {
     const mfh_u32 lo = __shfl((int)(mfh_u32)v, lane), hi = __shfl((int)(v >> 32), lane);

@@ -53,6 +53,7 @@ struct PrefillArgs {
     int32_t window, kv_heads, q_heads, group, dim;
     mfh_u32 row_tiles;  // of a request and head at most
     mfh_u32 parts;      // of a row's keys
+    mfh_u32 part_slots; // of a row in part_out: `parts`, or more
     mfh_u32 step_entries, step_bytes;  // a tile's keys in whole pages, and in bytes of a page
     Divider by_group, by_kv_heads, by_row_tiles, by_parts, by_q_heads;
 };
@@ -70,7 +71,11 @@ MFH_DEV int place(int row, int piece)
 // DP: head_dim rounded up to 64, 128 or 256.  WAVES: 4 (one group) or 8.  WIDE:
 // scores have a wide cap; as a branch its code takes registers and time from calls
 // without one (heads of 256 13% slower, a prompt of 512 3%).
-template <int DT, bool FP8, int DP, int WAVES, bool WIDE>
+// SHARED: a "request" is a group of requests with one new token each, whose keys are
+// the tokens that they have in common (mfh_paged_decode_shared): starts are those of
+// the groups, `prefix` holds the shared tokens, lengths are those of the requests;
+// the pages are the first request's, and results are parts.
+template <int DT, bool FP8, int DP, int WAVES, bool WIDE, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a)
 {
     constexpr int kWaves = WAVES, kThreads = 64 * kWaves, kRows = 32 * kWaves;
@@ -106,17 +111,35 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     const mfh_u32 rows = computed * a.group, row0 = row_tile * kRows;
     if (row0 >= rows) return;
     const mfh_u64 most = min((mfh_u64)a.pages.width * a.pages.by_page.d, (mfh_u64)kLongest);
-    const int length = (int)min((mfh_u64)max(a.lengths[r], 0), most);
-    const int prefix = a.prefix ? min(max(a.prefix[r], 0), length) : 0;
+    const int length = (int)min((mfh_u64)max(SHARED ? a.prefix[r] : a.lengths[r], 0), most);
+    const int prefix = !SHARED && a.prefix ? min(max(a.prefix[r], 0), length) : 0;
     const int first_position = length - (int)fresh;  // of the request's new tokens; may be negative
+    // Where a token of the group stands in its request, -1 without one; and the least
+    // and the greatest of some.
+    auto stands = [&](mfh_u32 token) {
+        if constexpr (SHARED) return (int)min((mfh_u64)max(a.lengths[begin + token], 0), most) - 1;
+        else return first_position + (int)token;
+    };
+    auto range = [&](mfh_u32 first_row, mfh_u32 last_row, int& low, int& high) {
+        const mfh_u32 first = a.by_group.quotient(first_row), last = a.by_group.quotient(last_row);
+        if constexpr (SHARED) {
+            low = kLongest, high = -1;
+            for (mfh_u32 t = first + lane; t <= last; t += 64) low = min(low, stands(t)), high = max(high, stands(t));
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) low = min(low, __shfl_xor(low, x)), high = max(high, __shfl_xor(high, x));
+            low = (int)uniform((mfh_u32)low), high = (int)uniform((mfh_u32)high);
+        } else {
+            low = stands(first), high = stands(last);
+        }
+    };
 
-    const int32_t* table = a.pages.table + (int64_t)r * a.pages.table_stride;
+    const int32_t* table = a.pages.table + (SHARED ? begin : (int64_t)r) * a.pages.table_stride;
     const char* k_base = a.pages.k + kv * a.pages.head_bytes;
     const char* v_base = a.pages.v + kv * a.pages.head_bytes;
 
     // Positions of the workgroup's rows, and the keys any of them sees.
-    const int low_position = first_position + (int)a.by_group.quotient(row0);
-    const int high_position = first_position + (int)a.by_group.quotient(min(row0 + kRows, rows) - 1);
+    int low_position, high_position;
+    range(row0, min(row0 + kRows, rows) - 1, low_position, high_position);
     const int key_end = min(max(high_position + 1, prefix), length);
     const int window_first = a.window > 0 ? max(low_position - a.window + 1, 0) : 0;  // below: the prefix only
     // The next tile at or after `tile` that has a key for some row: between the
@@ -134,10 +157,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     const bool real = row < rows;
     const mfh_u32 token = a.by_group.quotient(min(row, rows - 1));
     const mfh_u32 head = kv * a.group + (min(row, rows - 1) - token * a.group);
-    const int position = first_position + (int)token;
-    const mfh_u32 wave_row0 = min(row0 + 32 * wave, rows - 1), wave_row1 = min(row0 + 32 * wave + 31, rows - 1);
-    const int wave_low = first_position + (int)a.by_group.quotient(wave_row0);
-    const int wave_high = first_position + (int)a.by_group.quotient(wave_row1);
+    const int position = stands(token);
+    int wave_low, wave_high;
+    range(min(row0 + 32 * wave, rows - 1), min(row0 + 32 * wave + 31, rows - 1), wave_low, wave_high);
 
     u32x4 q[kSteps];
 #pragma unroll
@@ -355,9 +377,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
         // capped: 786 us, so 858).
         float scale = a.scale, offset = 0.0f;
         if (!plain.value || optional) {
-            // past the prefix a band of positions, for a row's own is below the length: one
-            // comparison a score (a window of 512 over 4096: 119 us, so 130)
-            const bool band = clean && key_first >= prefix;
+            // past the prefix a band of positions, for a row's own is below the length (of shared
+            // tokens it may be behind): one comparison a score (a window of 512 over 4096: 119
+            // us, so 130)
+            const bool band = clean && key_first >= prefix && (!SHARED || key_behind <= length);
             const mfh_u32 width = a.window > 0 ? (mfh_u32)a.window : 1u << 31;
             mfh_u64 mask = 0;   // bit i: key i is there
             if (!plain.value && !all && !band) mask = __ballot(there(key_first + lane));
@@ -560,8 +583,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     if (out_at >= rows) return;
     const mfh_u32 out_token = a.by_group.quotient(out_at), out_head = kv * a.group + (out_at - out_token * a.group);
     const int64_t out_row = (begin + out_token) * a.q_heads + out_head;
-    if (a.parts > 1) {
-        const int64_t at_part = out_row * a.parts + part;
+    if (SHARED || a.parts > 1) {
+        const int64_t at_part = out_row * a.part_slots + part;
         if (tile0 < tile_end)
 #pragma unroll
         for (int d = 0; d < kDimTiles; d++) {
@@ -692,23 +715,46 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     return l;
 }
 
-template <int DT, bool FP8, bool WIDE>
+template <int DT, bool FP8, bool WIDE, bool SHARED>
 void launch_dims(int dim, int waves, unsigned grid, hipStream_t s, const PrefillArgs& a)
 {
-    if (dim > 128) k_prefill<DT, FP8, 256, 4, WIDE><<<grid, 256, 0, s>>>(a);
-    else if (waves == 4 && dim <= 64) k_prefill<DT, FP8, 64, 4, WIDE><<<grid, 256, 0, s>>>(a);
-    else if (waves == 4) k_prefill<DT, FP8, 128, 4, WIDE><<<grid, 256, 0, s>>>(a);
-    else if (dim <= 64) k_prefill<DT, FP8, 64, 8, WIDE><<<grid, 512, 0, s>>>(a);
-    else k_prefill<DT, FP8, 128, 8, WIDE><<<grid, 512, 0, s>>>(a);
+    if (dim > 128) k_prefill<DT, FP8, 256, 4, WIDE, SHARED><<<grid, 256, 0, s>>>(a);
+    else if (waves == 4 && dim <= 64) k_prefill<DT, FP8, 64, 4, WIDE, SHARED><<<grid, 256, 0, s>>>(a);
+    else if (waves == 4) k_prefill<DT, FP8, 128, 4, WIDE, SHARED><<<grid, 256, 0, s>>>(a);
+    else if (dim <= 64) k_prefill<DT, FP8, 64, 8, WIDE, SHARED><<<grid, 512, 0, s>>>(a);
+    else k_prefill<DT, FP8, 128, 8, WIDE, SHARED><<<grid, 512, 0, s>>>(a);
 }
 
-template <int DT>
+template <int DT, bool SHARED>
 void launch_form(bool fp8, bool wide, int dim, int waves, unsigned grid, hipStream_t s, const PrefillArgs& a)
 {
-    if (fp8 && wide) launch_dims<DT, true, true>(dim, waves, grid, s, a);
-    else if (fp8) launch_dims<DT, true, false>(dim, waves, grid, s, a);
-    else if (wide) launch_dims<DT, false, true>(dim, waves, grid, s, a);
-    else launch_dims<DT, false, false>(dim, waves, grid, s, a);
+    if (fp8 && wide) launch_dims<DT, true, true, SHARED>(dim, waves, grid, s, a);
+    else if (fp8) launch_dims<DT, true, false, SHARED>(dim, waves, grid, s, a);
+    else if (wide) launch_dims<DT, false, true, SHARED>(dim, waves, grid, s, a);
+    else launch_dims<DT, false, false, SHARED>(dim, waves, grid, s, a);
+}
+
+// What a call's shape says, and its scores' scale and cap.
+void describe(PrefillArgs& a, const mfh_attention_shape& shape, const mfh_kv_cache& cache)
+{
+    a.scale = shape.scale * cache.k_scale * kLog2e;
+    if (shape.softcap > 0.0f) {
+        a.cap_scaled = shape.softcap * kLog2e;
+        a.cap_factor = shape.softcap > kWideCap ? 1.0f / a.cap_scaled : 2.0f / shape.softcap * a.scale;
+        if (!__builtin_isfinite(a.cap_factor)) a.cap_factor = __builtin_copysignf(FLT_MAX, a.cap_factor);  // a score of 0 is capped at 0
+    }
+    a.v_scale = cache.v_scale;
+    a.window = shape.window < kLongest ? shape.window : 0, a.kv_heads = cache.kv_heads, a.q_heads = shape.q_heads;
+    a.group = shape.q_heads / cache.kv_heads;
+    a.dim = cache.head_dim;
+    const Strides qs(shape.q_token_stride, shape.q_head_stride, shape.q_heads, cache.head_dim);
+    const Strides os(shape.out_token_stride, shape.out_head_stride, shape.q_heads, cache.head_dim);
+    a.q_t = qs.token, a.q_h = qs.head, a.out_t = os.token, a.out_h = os.head;
+    const int keys = keys_of(a.dim);
+    a.step_entries = (mfh_u32)(keys / cache.page_size);
+    a.step_bytes = (mfh_u32)(keys % cache.page_size) * a.pages.token_bytes;
+    a.by_group = Divider((mfh_u32)a.group), a.by_kv_heads = Divider((mfh_u32)a.kv_heads);
+    a.by_q_heads = Divider((mfh_u32)a.q_heads);
 }
 
 template <int DT>
@@ -722,6 +768,29 @@ void launch_join(const PrefillArgs& a, int requests, hipStream_t s)
 }
 
 }  // namespace
+
+int prefill_rows(int dim) { return 32 * waves_of(dim); }
+
+int prefill_shared(const mfh_attention_shape& shape, const mfh_kv_cache& cache, const PageArgs& pages, int32_t requests,
+                   int32_t groups, const void* q, const int32_t* starts, const int32_t* shared, const int32_t* lengths,
+                   const float* slopes, mfh_u32 parts, mfh_u32 part_slots, float* part_out, float2* part_sum,
+                   hipStream_t s)
+{
+    PrefillArgs a{};
+    a.pages = pages;
+    a.q = (const char*)q, a.starts = starts, a.prefix = shared, a.lengths = lengths, a.slopes = slopes;
+    describe(a, shape, cache);
+    a.tokens = a.most_fresh = requests;
+    a.row_tiles = (mfh_u32)(((int64_t)requests * a.group + prefill_rows(a.dim) - 1) / prefill_rows(a.dim));
+    a.parts = parts, a.part_slots = part_slots, a.part_out = part_out, a.part_sum = part_sum;
+    a.by_parts = Divider(parts), a.by_row_tiles = Divider(a.row_tiles);
+    const unsigned grid = (unsigned)groups * a.row_tiles * a.kv_heads * parts;
+    const bool fp8 = cache.dtype == kF8E4M3, wide = shape.softcap > kWideCap;
+    if (shape.dtype == kBFloat16) launch_form<kBFloat16, true>(fp8, wide, a.dim, waves_of(a.dim), grid, s, a);
+    else launch_form<kFloat16, true>(fp8, wide, a.dim, waves_of(a.dim), grid, s, a);
+    return launch_status("k_prefill");
+}
+
 }  // namespace mfh
 
 using namespace mfh;
@@ -768,21 +837,8 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
     a.pages = PageArgs(*cache, k_cache, v_cache, table, table_stride, table_width);
     a.q = (const char*)q, a.out = (char*)out, a.lse = lse;
     a.starts = starts, a.lengths = lengths, a.prefix = prefix, a.slopes = slopes;
-    const Strides qs(shape->q_token_stride, shape->q_head_stride, shape->q_heads, cache->head_dim);
-    const Strides os(shape->out_token_stride, shape->out_head_stride, shape->q_heads, cache->head_dim);
-    a.q_t = qs.token, a.q_h = qs.head, a.out_t = os.token, a.out_h = os.head;
+    describe(a, *shape, *cache);
     a.tokens = tokens, a.most_fresh = std::min(most_fresh, tokens);
-    a.scale = shape->scale * cache->k_scale * kLog2e;
-    const bool wide = shape->softcap > kWideCap;
-    if (shape->softcap > 0.0f) {
-        a.cap_scaled = shape->softcap * kLog2e;
-        a.cap_factor = wide ? 1.0f / a.cap_scaled : 2.0f / shape->softcap * a.scale;
-        if (!__builtin_isfinite(a.cap_factor)) a.cap_factor = __builtin_copysignf(FLT_MAX, a.cap_factor);  // a score of 0 is capped at 0
-    }
-    a.v_scale = cache->v_scale;
-    a.window = shape->window < kLongest ? shape->window : 0, a.kv_heads = cache->kv_heads, a.q_heads = shape->q_heads;
-    a.group = shape->q_heads / cache->kv_heads;
-    a.dim = cache->head_dim;
     Layout l = layout(dev, *shape, *cache, requests, tokens, most_fresh,
                       std::min<int64_t>(longest, (int64_t)table_width * cache->page_size));
     if (l.parts > 1) {  // as many as there is room for
@@ -794,20 +850,16 @@ int mfh_paged_prefill(const mfh_attention_shape* shape, const mfh_kv_cache* cach
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %lld tokens and %d heads are too many for one call",
                     what, requests, (long long)a.most_fresh, shape->q_heads);
     a.row_tiles = (mfh_u32)l.row_tiles;
-    a.parts = l.parts, a.by_parts = Divider(l.parts), a.by_q_heads = Divider((mfh_u32)a.q_heads);
+    a.parts = a.part_slots = l.parts, a.by_parts = Divider(l.parts);
     if (l.parts > 1) {
         a.part_out = (float*)workspace;
         a.part_sum = (float2*)(a.part_out + tokens * shape->q_heads * l.parts * a.dim);
     }
-    const int keys = keys_of(a.dim);
-    a.step_entries = (mfh_u32)(keys / cache->page_size);
-    a.step_bytes = (mfh_u32)(keys % cache->page_size) * a.pages.token_bytes;
-    a.by_group = Divider((mfh_u32)a.group), a.by_kv_heads = Divider((mfh_u32)a.kv_heads);
     a.by_row_tiles = Divider(a.row_tiles);
     hipStream_t s = (hipStream_t)stream;
-    const bool fp8 = cache->dtype == kF8E4M3;
-    if (shape->dtype == kBFloat16) launch_form<kBFloat16>(fp8, wide, a.dim, l.waves, (unsigned)grid, s, a);
-    else launch_form<kFloat16>(fp8, wide, a.dim, l.waves, (unsigned)grid, s, a);
+    const bool fp8 = cache->dtype == kF8E4M3, wide = shape->softcap > kWideCap;
+    if (shape->dtype == kBFloat16) launch_form<kBFloat16, false>(fp8, wide, a.dim, l.waves, (unsigned)grid, s, a);
+    else launch_form<kFloat16, false>(fp8, wide, a.dim, l.waves, (unsigned)grid, s, a);
     MFH_TRY(launch_status("k_prefill"));
     if (l.parts > 1) {
         if (shape->dtype == kBFloat16) launch_join<kBFloat16>(a, requests, s);

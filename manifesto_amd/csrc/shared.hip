@@ -25,6 +25,7 @@ namespace {
 using namespace decode;
 
 constexpr int kMostGroups = 4096;
+constexpr int kManyColumns = 256;
 
 struct SharedArgs {
     PageArgs pages;
@@ -45,6 +46,7 @@ struct SharedArgs {
     mfh_u32 lines;                         // columns in 16, 32 or 64, of all groups, at most
     mfh_u32 shared_blocks;
     mfh_u32 shared_parts, own_parts, parts, shared_piece, own_piece;  // piece: tiles of a part
+    bool all_parts;  // every request of a group has as many shared parts as there are
     Divider by_group, by_lines, by_shared_parts, by_own_parts, by_kv_heads, by_head_groups, by_shared_piece, by_own_piece, by_q_heads;
 };
 
@@ -648,7 +650,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a)
     Seen own;
     own.length = length_of(a, r);
     own.first = max(first_of(a, own.length), group.length);
-    const mfh_u32 common = group.members > 0 ? Tiles(group, a.by_shared_piece, a.shared_parts).parts : 0;
+    const mfh_u32 common = group.members == 0 ? 0 : a.all_parts ? a.shared_parts : Tiles(group, a.by_shared_piece, a.shared_parts).parts;
     const mfh_u32 parts = common + Tiles(own, a.by_own_piece, a.own_parts).parts;
     const float2* sums = a.part_sum + (int64_t)row * a.parts;
     const int d = 128 * chunk + 2 * lane;
@@ -662,6 +664,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a)
 #pragma unroll 4
     for (mfh_u32 n = wave; n < parts; n += kJoinWaves) {
         const float2 s = sums[slot(n)];
+        if (s.x == -INFINITY && s.y == 0.0f) continue;  // it saw nothing
         const float2 w = *reinterpret_cast<const float2*>(from + (int64_t)slot(n) * a.dim);
         const float f = s.x == -INFINITY ? 0.0f : exp2_fast(s.x - top);
         all += s.x == -INFINITY ? s.y : f * s.y;  // without a reference 0, or NaN
@@ -685,6 +688,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a)
 }
 
 struct Layout {
+    bool prefill;
     int sets;
     int64_t lines, shared_blocks, own_blocks;
     mfh_u32 shared_parts, own_parts, shared_piece, own_piece;
@@ -697,7 +701,8 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     Layout l{};
     const int group = sh.q_heads / c.kv_heads;
     const int64_t columns = (int64_t)requests * group, each = groups > 0 ? columns / groups : 0;
-    l.sets = each <= 16 ? 1 : c.head_dim > 128 ? 2 : 4;
+    l.prefill = each >= kManyColumns && groups <= 16;
+    l.sets = each <= 16 || l.prefill ? 1 : c.head_dim > 128 ? 2 : 4;
     l.lines = columns / (kHeads * l.sets) + groups;
     auto split = [&](int64_t blocks, int64_t rows, int64_t tokens, mfh_u32& piece, mfh_u32& parts) {
         const int64_t tiles = (std::min<int64_t>(std::max<int64_t>(tokens, 1), kLongest) + kTile - 1) / kTile + 1;
@@ -705,10 +710,15 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
         piece = (mfh_u32)std::max<int64_t>(8, (tiles + wanted - 1) / wanted);
         parts = (mfh_u32)((tiles + piece - 1) / piece);
     };
-    split((l.sets > 1 ? 1 : 2) * dev->compute_units, std::max<int64_t>(groups, columns / (kHeads * l.sets)) * c.kv_heads, most_shared, l.shared_piece, l.shared_parts);
+    if (l.prefill) {
+        const int64_t rows = (each + prefill_rows(c.head_dim) - 1) / prefill_rows(c.head_dim) * groups * c.kv_heads;
+        const int64_t tiles = std::min<int64_t>(std::max<int64_t>(most_shared, 1), kLongest) / 256;  // of a part at least
+        l.shared_parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({dev->compute_units / rows, tiles, 64}));
+        l.shared_piece = 1;
+    } else split((l.sets > 1 ? 1 : 2) * dev->compute_units, std::max<int64_t>(groups, columns / (kHeads * l.sets)) * c.kv_heads, most_shared, l.shared_piece, l.shared_parts);
     split(2 * dev->compute_units, (int64_t)requests * c.kv_heads, most_own, l.own_piece, l.own_parts);
     if (groups == 0) l.shared_parts = 0;
-    l.shared_blocks = ((int64_t)c.kv_heads * l.shared_parts + 7) / 8 * 8 * l.lines;
+    l.shared_blocks = l.prefill ? 0 : ((int64_t)c.kv_heads * l.shared_parts + 7) / 8 * 8 * l.lines;
     l.own_blocks = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads) * l.own_parts;
     l.bytes = (size_t)requests * sh.q_heads * (l.shared_parts + l.own_parts) * (c.head_dim + 2) * sizeof(float);
     return l;
@@ -823,6 +833,10 @@ int mfh_paged_decode_shared(const mfh_attention_shape* shape, const mfh_kv_cache
                       ((uintptr_t)k_cache | (uintptr_t)v_cache | a.pages.page_bytes | a.pages.head_bytes | a.pages.token_bytes) % 4 == 0;
     const bool fp8 = cache->dtype == kF8E4M3;
     const unsigned grid = (unsigned)(l.shared_blocks + l.own_blocks);
+    a.all_parts = l.prefill;
+    if (l.prefill)
+        MFH_TRY(prefill_shared(*shape, *cache, a.pages, requests, groups, q, starts, shared, lengths, slopes, l.shared_parts, a.parts,
+                               a.part_out, a.part_sum, s));
     if (shape->dtype == kBFloat16) {
         if (fp8) launch_dims<kBFloat16, true>(fast, l.sets, grid, s, a);
         else launch_dims<kBFloat16, false>(fast, l.sets, grid, s, a);
