@@ -25,7 +25,6 @@ namespace {
 using namespace decode;
 
 constexpr int kMostGroups = 4096;
-constexpr int kManyColumns = 256;
 
 struct SharedArgs {
     PageArgs pages;
@@ -47,6 +46,7 @@ struct SharedArgs {
     mfh_u32 shared_blocks;
     mfh_u32 shared_parts, own_parts, parts, shared_piece, own_piece;  // piece: tiles of a part
     bool all_parts;  // every request of a group has as many shared parts as there are
+    bool alone;      // a wave takes a request's own part alone
     Divider by_group, by_lines, by_shared_parts, by_own_parts, by_kv_heads, by_head_groups, by_shared_piece, by_own_piece, by_q_heads;
 };
 
@@ -574,13 +574,15 @@ struct Part {
 
 // DP: head_dim rounded up to 64, 128 or 256.  SETS: of 16 columns, of the shared tokens.
 template <int DT, bool FP8, int DP, bool FAST, int SETS>
-__global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_shared(SharedArgs a)
+__global__ __launch_bounds__(kThreads, SETS > 2 || DP == 256 ? 1 : SETS > 1 || DP == 128 ? 2 : 3) void k_shared(SharedArgs a)
 {
     typedef Part<DT, FP8, DP, FAST, SETS, kWaves> Common;
     typedef Part<DT, FP8, DP, FAST, 1, kWaves> Own;
+    typedef Part<DT, FP8, DP, FAST, 1, 1> Alone;
     __shared__ union {
         typename Common::Lds common;
         typename Own::Lds own;
+        typename Alone::Lds alone;
     } lds;
     const int lane = threadIdx.x & 63;
     if (blockIdx.x < a.shared_blocks) {
@@ -614,11 +616,16 @@ __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ?
                     tiles.first + min(part * share, tiles.count), tiles.first + min((part + 1) * share, tiles.count), part);
         return;
     }
-    const mfh_u32 block = blockIdx.x - a.shared_blocks;
-    mfh_u32 rest = a.by_own_parts.quotient(block);
-    const mfh_u32 part = block - rest * a.own_parts;
-    const mfh_u32 line = a.by_head_groups.quotient(rest), head_group = rest - line * a.head_groups;
+    // A request's own tokens: a row (request, key-value head, 16 of its query heads) and
+    // part each, of a workgroup or, of many rows, of a wave.
+    mfh_u32 rest = blockIdx.x - a.shared_blocks;
+    if (a.alone) rest = rest * kWaves + uniform(threadIdx.x >> 6);
+    mfh_u32 line = a.by_own_parts.quotient(rest);
+    const mfh_u32 part = rest - line * a.own_parts;
+    rest = line, line = a.by_head_groups.quotient(rest);
+    const mfh_u32 head_group = rest - line * a.head_groups;
     const mfh_u32 r = a.by_kv_heads.quotient(line), kv = line - r * a.kv_heads;
+    if (r >= a.requests) return;
     Group group;
     group.with(a, r, lane);
     Seen own;
@@ -627,23 +634,25 @@ __global__ __launch_bounds__(kThreads, SETS > 1 ? 1 : DP == 64 ? 3 : DP == 128 ?
     const Tiles tiles(own, a.by_own_piece, a.own_parts);
     if (part >= tiles.parts) return;
     const mfh_u32 share = uniform((tiles.count + tiles.parts - 1) / tiles.parts);
-    Own::run(a, lds.own, r, 1, head_group * kHeads, kv, own, r, tiles.first + min(part * share, tiles.count),
-             tiles.first + min((part + 1) * share, tiles.count), a.shared_parts + part);
+    const mfh_u32 begin = tiles.first + min(part * share, tiles.count), end = tiles.first + min((part + 1) * share, tiles.count);
+    if (a.alone) Alone::run(a, lds.alone, r, 1, head_group * kHeads, kv, own, r, begin, end, a.shared_parts + part);
+    else Own::run(a, lds.own, r, 1, head_group * kHeads, kv, own, r, begin, end, a.shared_parts + part);
 }
 
-// Joins a row's parts, of the shared tokens and of its own.  A workgroup takes
-// 128 dims of a query head, a quarter of the parts in each wave; lanes take two
-// dims each.
+// Joins a row's parts, of the shared tokens and of its own.  A wave takes 128 dims
+// of a query head, two a lane; or, of many parts, four waves a quarter of them each.
 constexpr int kJoinWaves = 4;
 
-template <int DT>
-__global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a)
+template <int DT, int WAVES>
+__global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a, mfh_u32 units)
 {
     __shared__ float s_all[kJoinWaves];
     __shared__ float2 s_out[kJoinWaves][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int chunks = (a.dim + 127) / 128;
-    const mfh_u32 row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const mfh_u32 chunks = (a.dim + 127) / 128;
+    const mfh_u32 unit = WAVES > 1 ? blockIdx.x : blockIdx.x * kJoinWaves + wave;
+    if (WAVES == 1 && unit >= units) return;
+    const mfh_u32 row = chunks > 1 ? unit / 2 : unit, chunk = unit - row * chunks;
     const mfh_u32 r = a.by_q_heads.quotient(row), head = row - r * a.q_heads;
     Group group;
     group.with(a, r, lane);
@@ -661,25 +670,27 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a)
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
     float all = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll 4
-    for (mfh_u32 n = wave; n < parts; n += kJoinWaves) {
+#pragma unroll 8
+    for (mfh_u32 n = WAVES > 1 ? wave : 0; n < parts; n += WAVES) {
         const float2 s = sums[slot(n)];
-        if (s.x == -INFINITY && s.y == 0.0f) continue;  // it saw nothing
-        const float2 w = *reinterpret_cast<const float2*>(from + (int64_t)slot(n) * a.dim);
+        const bool seen = s.x != -INFINITY || s.y != 0.0f;  // else there is nothing
+        const float2 w = seen ? *reinterpret_cast<const float2*>(from + (int64_t)slot(n) * a.dim) : make_float2(0.0f, 0.0f);
         const float f = s.x == -INFINITY ? 0.0f : exp2_fast(s.x - top);
         all += s.x == -INFINITY ? s.y : f * s.y;  // without a reference 0, or NaN
         o0 += f * w.x;
         o1 += f * w.y;
     }
-    if (lane == 0) s_all[wave] = all;
-    s_out[wave][lane] = make_float2(o0, o1);
-    __syncthreads();
-    if (wave > 0) return;
+    if constexpr (WAVES > 1) {
+        if (lane == 0) s_all[wave] = all;
+        s_out[wave][lane] = make_float2(o0, o1);
+        __syncthreads();
+        if (wave > 0) return;
 #pragma unroll
-    for (int w = 1; w < kJoinWaves; w++) {
-        all += s_all[w];
-        o0 += s_out[w][lane].x;
-        o1 += s_out[w][lane].y;
+        for (int w = 1; w < kJoinWaves; w++) {
+            all += s_all[w];
+            o0 += s_out[w][lane].x;
+            o1 += s_out[w][lane].y;
+        }
     }
     if (d >= a.dim) return;
     const float f = all == 0.0f ? 0.0f : a.v_scale / all;
@@ -687,8 +698,33 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a)
     if (d == 0 && a.lse) a.lse[row] = all == 0.0f ? -INFINITY : top * kLn2 + logf(all);
 }
 
+template <int DT>
+void launch_join(const SharedArgs& a, hipStream_t s)
+{
+    const mfh_u32 units = a.requests * a.q_heads * ((a.dim + 127) / 128);
+    if (a.parts > 24) k_shared_join<DT, kJoinWaves><<<units, 64 * kJoinWaves, 0, s>>>(a, units);
+    else k_shared_join<DT, 1><<<(units + kJoinWaves - 1) / kJoinWaves, 64 * kJoinWaves, 0, s>>>(a, units);
+}
+
+// How a call is laid out, from what the host knows.
+//
+// Shared tokens: sets of 16 columns, as many as a group has on average, up to 64
+// columns, with which a workgroup fills a CU (24 groups of 4 to 32 columns over up
+// to 6000 e4m3 tokens: by 64 columns 94 us, by 32 48 us).  Of 256 columns on and
+// long shared tokens prefill's kernels, whose tiles serve 256 columns, are
+// faster: 256 requests of 32 heads over 8, 16384 tokens, 141 us, else 166; 64 such
+// requests over 65536 133 us, else 160; but over 8192 56 and 54, and 128 requests
+// over 2000 64 and 58.
+//
+// Parts: as many as CUs hold workgroups, one of 64 columns or of heads wider than
+// 128 (64 requests over 8192 tokens 55 us, twice as many 64; two groups of eight
+// over 131072 tokens of 256 dims 153 and 161) and two of fewer columns, and half as
+// many again where groups may differ (the 24 groups: 48 us, 42 to 50).  Eight tiles
+// at least.  Of a request's own tokens two workgroups a CU, or, where there are
+// four rows a CU and more, a wave a row: 256 requests of up to 300 own tokens 39 us,
+// by workgroups 44.
 struct Layout {
-    bool prefill;
+    bool prefill, alone;
     int sets;
     int64_t lines, shared_blocks, own_blocks;
     mfh_u32 shared_parts, own_parts, shared_piece, own_piece;
@@ -699,27 +735,31 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
               int64_t most_shared, int64_t most_own)
 {
     Layout l{};
-    const int group = sh.q_heads / c.kv_heads;
+    const int group = sh.q_heads / c.kv_heads, cus = dev->compute_units;
     const int64_t columns = (int64_t)requests * group, each = groups > 0 ? columns / groups : 0;
-    l.prefill = each >= kManyColumns && groups <= 16;
-    l.sets = each <= 16 || l.prefill ? 1 : c.head_dim > 128 ? 2 : 4;
+    const int64_t tokens = std::min<int64_t>(std::max<int64_t>(most_shared, 1), kLongest);
+    l.prefill = each >= 256 && each * tokens >= (1 << 22) && groups <= 16;
+    l.sets = each <= 16 || l.prefill ? 1 : each <= 32 || c.head_dim > 128 ? 2 : 4;
     l.lines = columns / (kHeads * l.sets) + groups;
-    auto split = [&](int64_t blocks, int64_t rows, int64_t tokens, mfh_u32& piece, mfh_u32& parts) {
-        const int64_t tiles = (std::min<int64_t>(std::max<int64_t>(tokens, 1), kLongest) + kTile - 1) / kTile + 1;
-        const int64_t wanted = std::max<int64_t>(1, blocks / std::max<int64_t>(rows, 1));
+    auto split = [](int64_t blocks, int64_t rows, int64_t tokens, mfh_u32& piece, mfh_u32& parts) {
+        const int64_t tiles = (tokens + kTile - 1) / kTile + 1, wanted = std::max<int64_t>(1, blocks / std::max<int64_t>(rows, 1));
         piece = (mfh_u32)std::max<int64_t>(8, (tiles + wanted - 1) / wanted);
         parts = (mfh_u32)((tiles + piece - 1) / piece);
     };
     if (l.prefill) {
         const int64_t rows = (each + prefill_rows(c.head_dim) - 1) / prefill_rows(c.head_dim) * groups * c.kv_heads;
-        const int64_t tiles = std::min<int64_t>(std::max<int64_t>(most_shared, 1), kLongest) / 256;  // of a part at least
-        l.shared_parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({dev->compute_units / rows, tiles, 64}));
+        l.shared_parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({cus / rows, tokens / 256, 64}));
         l.shared_piece = 1;
-    } else split((l.sets > 1 ? 1 : 2) * dev->compute_units, std::max<int64_t>(groups, columns / (kHeads * l.sets)) * c.kv_heads, most_shared, l.shared_piece, l.shared_parts);
-    split(2 * dev->compute_units, (int64_t)requests * c.kv_heads, most_own, l.own_piece, l.own_parts);
+    } else {
+        const int blocks = l.sets > 2 || c.head_dim > 128 ? cus : groups > 1 ? 3 * cus : 2 * cus;
+        split(blocks, std::max<int64_t>(groups, columns / (kHeads * l.sets)) * c.kv_heads, tokens, l.shared_piece, l.shared_parts);
+    }
+    split(2 * cus, (int64_t)requests * c.kv_heads, std::min<int64_t>(std::max<int64_t>(most_own, 1), kLongest), l.own_piece, l.own_parts);
     if (groups == 0) l.shared_parts = 0;
     l.shared_blocks = l.prefill ? 0 : ((int64_t)c.kv_heads * l.shared_parts + 7) / 8 * 8 * l.lines;
     l.own_blocks = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads) * l.own_parts;
+    l.alone = l.own_blocks >= 4 * cus;
+    if (l.alone) l.own_blocks = (l.own_blocks + kWaves - 1) / kWaves;
     l.bytes = (size_t)requests * sh.q_heads * (l.shared_parts + l.own_parts) * (c.head_dim + 2) * sizeof(float);
     return l;
 }
@@ -728,6 +768,7 @@ template <int DT, bool FP8, int DP, bool FAST>
 void launch_sets(int sets, unsigned grid, hipStream_t s, const SharedArgs& a)
 {
     if (sets == 1) k_shared<DT, FP8, DP, FAST, 1><<<grid, kThreads, 0, s>>>(a);
+    else if (sets == 2 || DP == 256) k_shared<DT, FP8, DP, FAST, 2><<<grid, kThreads, 0, s>>>(a);
     else k_shared<DT, FP8, DP, FAST, DP == 256 ? 2 : 4><<<grid, kThreads, 0, s>>>(a);
 }
 
@@ -833,7 +874,7 @@ int mfh_paged_decode_shared(const mfh_attention_shape* shape, const mfh_kv_cache
                       ((uintptr_t)k_cache | (uintptr_t)v_cache | a.pages.page_bytes | a.pages.head_bytes | a.pages.token_bytes) % 4 == 0;
     const bool fp8 = cache->dtype == kF8E4M3;
     const unsigned grid = (unsigned)(l.shared_blocks + l.own_blocks);
-    a.all_parts = l.prefill;
+    a.all_parts = l.prefill, a.alone = l.alone;
     if (l.prefill)
         MFH_TRY(prefill_shared(*shape, *cache, a.pages, requests, groups, q, starts, shared, lengths, slopes, l.shared_parts, a.parts,
                                a.part_out, a.part_sum, s));
@@ -845,9 +886,8 @@ int mfh_paged_decode_shared(const mfh_attention_shape* shape, const mfh_kv_cache
         else launch_dims<kFloat16, false>(fast, l.sets, grid, s, a);
     }
     MFH_TRY(launch_status("k_shared"));
-    const unsigned joins = (unsigned)((int64_t)requests * a.q_heads * ((a.dim + 127) / 128));
-    if (shape->dtype == kBFloat16) k_shared_join<kBFloat16><<<joins, 64 * kJoinWaves, 0, s>>>(a);
-    else k_shared_join<kFloat16><<<joins, 64 * kJoinWaves, 0, s>>>(a);
+    if (shape->dtype == kBFloat16) launch_join<kBFloat16>(a, s);
+    else launch_join<kFloat16>(a, s);
     return launch_status("k_shared_join");
 }
 
