@@ -317,6 +317,15 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
     const mfh_u32 row0 = group * a.beams;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
+    // A thread's first candidates are on their way during the logarithms.
+    const mfh_u32 lists = a.beams * a.pieces;
+    const mfh_u64* keys = a.best + (int64_t)row0 * a.pieces * a.picks;
+    mfh_u64 first[2];
+#pragma unroll
+    for (mfh_u32 i = 0; i < 2; i++) {
+        const mfh_u32 n = threadIdx.x + i * kThreads;
+        first[i] = n < lists * a.picks ? keys[n] : 0;
+    }
     // the logarithm of each beam's sum, a wave each
     for (mfh_u32 b = wave; b < a.beams; b += kWaves) {
         const mfh_u32 row = row0 + b;
@@ -326,11 +335,16 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
         float top = -INFINITY;
         double sum = 0.0;
         if (!ended) {
-            for (mfh_u32 n = lane; n < a.pieces; n += 64) top = fmaxf(top, tops[n]);
+            const bool some = (mfh_u32)lane < a.pieces;
+            const float mine = some ? tops[lane] : -INFINITY;
+            const double its = some ? sums[lane] : 0.0;
+            top = mine;
+            for (mfh_u32 n = lane + 64; n < a.pieces; n += 64) top = fmaxf(top, tops[n]);
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-            for (mfh_u32 n = lane; n < a.pieces; n += 64)
-                sum += tops[n] == -INFINITY ? sums[n] : exp((double)tops[n] - (double)top) * sums[n];
+            auto add = [&](float t, double s) { sum += t == -INFINITY ? s : exp((double)t - (double)top) * s; };
+            add(mine, its);
+            for (mfh_u32 n = lane + 64; n < a.pieces; n += 64) add(tops[n], sums[n]);
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
         }
@@ -342,18 +356,15 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
     }
     __syncthreads();
 
-    const mfh_u32 lists = a.beams * a.pieces;
-    auto candidate = [&](mfh_u32 n) {
+    auto candidate = [&](mfh_u32 n, mfh_u64 key) {
         const mfh_u32 list = a.by_picks.quotient(n), i = n - list * a.picks;
         const mfh_u32 b = a.by_pieces.quotient(list), piece = list - b * a.pieces;
-        mfh_u64 key;
         double score;
         if (s_ended[b]) {
             if (piece > 0 || i > 0) return Key::none();
             key = (mfh_u64)0xffffffffu << 32 | (mfh_u32)~a.end_token;
             score = s_score[b];
         } else {
-            key = a.best[((int64_t)row0 * a.pieces + list) * a.picks + i];
             if (key == 0) return Key::none();
             score = s_score[b] + ((double)unordered((mfh_u32)(key >> 32)) - s_norm[b]);
         }
@@ -362,10 +373,16 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
         return Key{ordered(score), low};
     };
     auto each = [&](const Key&, auto f) {
-        for (mfh_u32 n = threadIdx.x; n < lists * a.picks; n += kThreads) {
-            const Key k = candidate(n);
+        auto one = [&](mfh_u32 n, mfh_u64 key) {
+            const Key k = candidate(n, key);
             if (k.some()) f(k);
+        };
+#pragma unroll
+        for (mfh_u32 i = 0; i < 2; i++) {
+            const mfh_u32 n = threadIdx.x + i * kThreads;
+            if (n < lists * a.picks) one(n, first[i]);
         }
+        for (mfh_u32 n = threadIdx.x + 2 * kThreads; n < lists * a.picks; n += kThreads) one(n, keys[n]);
     };
     Key top = Key::none();
     each(Key::none(), [&](Key k) { top = k > top ? k : top; });

@@ -710,7 +710,9 @@ void launch_join(const SharedArgs& a, hipStream_t s)
 //
 // Shared tokens: sets of 16 columns, as many as a group has on average, up to 64
 // columns, with which a workgroup fills a CU (24 groups of 4 to 32 columns over up
-// to 6000 e4m3 tokens: by 64 columns 94 us, by 32 48 us).  Of 256 columns on and
+// to 6000 e4m3 tokens: by 64 columns 94 us, by 32 48 us), and to 32 where there is
+// less to share than each request has for itself, whose workgroups a CU then holds
+// two of.  Of 256 columns on and
 // long shared tokens prefill's kernels, whose tiles serve 256 columns, are
 // faster: 256 requests of 32 heads over 8, 16384 tokens, 141 us, else 166; 64 such
 // requests over 65536 133 us, else 160; but over 8192 56 and 54, and 128 requests
@@ -739,7 +741,7 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     const int64_t columns = (int64_t)requests * group, each = groups > 0 ? columns / groups : 0;
     const int64_t tokens = std::min<int64_t>(std::max<int64_t>(most_shared, 1), kLongest);
     l.prefill = each >= 256 && each * tokens >= (1 << 22) && groups <= 16;
-    l.sets = each <= 16 || l.prefill ? 1 : each <= 32 || c.head_dim > 128 ? 2 : 4;
+    l.sets = each <= 16 || l.prefill ? 1 : each <= 32 || c.head_dim > 128 || tokens < most_own ? 2 : 4;
     l.lines = columns / (kHeads * l.sets) + groups;
     auto split = [](int64_t blocks, int64_t rows, int64_t tokens, mfh_u32& piece, mfh_u32& parts) {
         const int64_t tiles = (tokens + kTile - 1) / kTile + 1, wanted = std::max<int64_t>(1, blocks / std::max<int64_t>(rows, 1));
