@@ -83,6 +83,8 @@ struct Key {
     MFH_DEV bool operator>(const Key& o) const { return high > o.high || (high == o.high && low > o.low); }
     MFH_DEV bool operator>=(const Key& o) const { return !(o > *this); }
     MFH_DEV bool some() const { return low != 0; }
+    // (member by member: a choice between two keys as such goes through memory)
+    static MFH_DEV Key choose(bool first, const Key& a, const Key& b) { return Key{first ? a.high : b.high, first ? a.low : b.low}; }
     static MFH_DEV Key none() { return Key{0, 0}; }
     static MFH_DEV Key all() { return Key{~(mfh_u64)0, ~(mfh_u64)0}; }
     MFH_DEV Key from_lane(int mask) const
@@ -307,6 +309,8 @@ __global__ __launch_bounds__(kThreads, 8) void k_beam_rows(BeamArgs a)
     }
 }
 
+// FLAT: a group's candidates are two a thread at most.
+template <bool FLAT>
 __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
 {
     __shared__ Selection<Key> s;
@@ -317,14 +321,19 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
     const mfh_u32 row0 = group * a.beams;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
-    // A thread's first candidates are on their way during the logarithms.
+    // Up to two candidates a thread are taken at once.  Of more the heads come first: a
+    // piece's list is in order, and its head says whether the rest matters (2 groups of 8
+    // beams, 16 picks from 42 pieces each: 8.4 us, all at once 22; 3 groups of 16
+    // beams, 32 picks from one piece: 11 us, by the heads 35).  The first ones are
+    // on their way during the logarithms.
     const mfh_u32 lists = a.beams * a.pieces;
     const mfh_u64* keys = a.best + (int64_t)row0 * a.pieces * a.picks;
+    const mfh_u32 firsts = FLAT ? lists * a.picks : lists;
     mfh_u64 first[2];
 #pragma unroll
     for (mfh_u32 i = 0; i < 2; i++) {
         const mfh_u32 n = threadIdx.x + i * kThreads;
-        first[i] = n < lists * a.picks ? keys[n] : 0;
+        first[i] = n < firsts ? keys[FLAT ? n : (int64_t)n * a.picks] : 0;
     }
     // the logarithm of each beam's sum, a wave each
     for (mfh_u32 b = wave; b < a.beams; b += kWaves) {
@@ -356,8 +365,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
     }
     __syncthreads();
 
-    auto candidate = [&](mfh_u32 n, mfh_u64 key) {
-        const mfh_u32 list = a.by_picks.quotient(n), i = n - list * a.picks;
+    auto candidate = [&](mfh_u32 list, mfh_u32 i, mfh_u64 key) {
         const mfh_u32 b = a.by_pieces.quotient(list), piece = list - b * a.pieces;
         double score;
         if (s_ended[b]) {
@@ -372,20 +380,36 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
         const mfh_u64 low = (mfh_u64)(kMostBeams - 1 - b) << 56 | (key >> 32) << kTokenBits | (key & ((1u << kTokenBits) - 1));
         return Key{ordered(score), low};
     };
-    auto each = [&](const Key&, auto f) {
-        auto one = [&](mfh_u32 n, mfh_u64 key) {
-            const Key k = candidate(n, key);
-            if (k.some()) f(k);
-        };
+    Key mine[2], top = Key::none();
 #pragma unroll
-        for (mfh_u32 i = 0; i < 2; i++) {
-            const mfh_u32 n = threadIdx.x + i * kThreads;
-            if (n < lists * a.picks) one(n, first[i]);
+    for (mfh_u32 i = 0; i < 2; i++) {
+        const mfh_u32 n = threadIdx.x + i * kThreads, list = FLAT ? a.by_picks.quotient(n) : n;
+        mine[i] = Key::none();
+        if (n < firsts) mine[i] = candidate(list, FLAT ? n - list * a.picks : 0, first[i]);
+        top = Key::choose(mine[i] > top, mine[i], top);
+    }
+    if constexpr (!FLAT)
+        for (mfh_u32 list = threadIdx.x + 2 * kThreads; list < lists; list += kThreads) {
+            const Key k = candidate(list, 0, keys[(int64_t)list * a.picks]);
+            top = Key::choose(k > top, k, top);
         }
-        for (mfh_u32 n = threadIdx.x + 2 * kThreads; n < lists * a.picks; n += kThreads) one(n, keys[n]);
+    auto each = [&](const Key& least, auto f) {
+        if constexpr (FLAT) {
+#pragma unroll
+            for (mfh_u32 i = 0; i < 2; i++)
+                if (mine[i].some()) f(mine[i]);
+        } else {
+            for (mfh_u32 list = threadIdx.x; list < lists; list += kThreads) {
+                Key k = Key::choose(list < kThreads, mine[0], mine[1]);
+                if (list >= 2 * kThreads) k = candidate(list, 0, keys[(int64_t)list * a.picks]);
+                for (mfh_u32 i = 1; k.some() && !(least > k); i++) {
+                    f(k);
+                    if (i == a.picks) break;
+                    k = candidate(list, i, keys[(int64_t)list * a.picks + i]);
+                }
+            }
+        }
     };
-    Key top = Key::none();
-    each(Key::none(), [&](Key k) { top = k > top ? k : top; });
     s.run(a.picks, top, s_best, each);
     __syncthreads();
 
@@ -532,7 +556,9 @@ int mfh_beam_select(const mfh_beam_shape* shape, int32_t groups, const void* log
     else if (shape->dtype == kFloat16) launch_rows<kFloat16>(l, (unsigned)cells, s, a);
     else launch_rows<kBFloat16>(l, (unsigned)cells, s, a);
     MFH_TRY(launch_status("k_beam_rows"));
-    k_beam_merge<<<(unsigned)groups * a.slices, kThreads, 0, s>>>(a);
+    const unsigned grid = (unsigned)groups * a.slices;
+    if (a.beams * a.pieces * a.picks <= 2 * kThreads) k_beam_merge<true><<<grid, kThreads, 0, s>>>(a);
+    else k_beam_merge<false><<<grid, kThreads, 0, s>>>(a);
     return launch_status("k_beam_merge");
 }
 
