@@ -56,13 +56,13 @@ typedef struct {
  *
  * history, if not NULL, holds the tokens of each row so far, known[g] of
  * them in group g ([rows][history_stride]); history_out ([groups * picks]
- * [history_stride], another buffer) gets the parent's with the new token
- * behind them.  Tokens that do not fit the stride are not written, nor is the
+ * [history_stride]) gets the parent's with the new token behind them.  Tokens that do not fit the stride are not written, nor is the
  * row of a result without parent; what stands behind stays as it is.
  *
- * The workspace (any 16-byte aligned device memory, free for other use once
- * the call's work is done) has to be as large as mfh_beam_select_workspace
- * says. */
+ * scores_out, ended_out and history_out are other buffers than scores, ended
+ * and history.  The workspace (any 16-byte aligned device memory, free for
+ * other use once the call's work is done) has to be as large as
+ * mfh_beam_select_workspace says. */
 int mfh_beam_select(const mfh_beam_shape* shape, int32_t groups, const void* logits, const float* scores,
                     const uint8_t* ended, float* scores_out, int32_t* tokens, int32_t* parents, uint8_t* ended_out,
                     const int32_t* history, const int32_t* known, int32_t* history_out, void* workspace,

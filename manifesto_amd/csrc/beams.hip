@@ -532,8 +532,16 @@ int mfh_beam_select(const mfh_beam_shape* shape, int32_t groups, const void* log
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: NULL buffer", what);
     if (ended && shape->end_token < 0)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: beams that have ended, and no end token", what);
-    if (history && history == history_out)
-        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: history_out is history, which is still read", what);
+    const int64_t rows = (int64_t)groups * shape->beams, results = (int64_t)groups * shape->picks;
+    auto overlap = [](const void* p, int64_t p_bytes, const void* q, int64_t q_bytes) {
+        return (uintptr_t)p < (uintptr_t)q + q_bytes && (uintptr_t)q < (uintptr_t)p + p_bytes;
+    };
+    if (overlap(scores, rows * 4, scores_out, results * 4))
+        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: scores_out overlaps scores, which other workgroups still read", what);
+    if (ended && ended_out && overlap(ended, rows, ended_out, results))
+        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: ended_out overlaps ended, which other workgroups still read", what);
+    if (history && overlap(history, rows * shape->history_stride * 4, history_out, results * shape->history_stride * 4))
+        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: history_out overlaps history, which other workgroups still read", what);
     if (workspace_bytes < l.bytes || !workspace || (uintptr_t)workspace % 16)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: a workspace of %zu bytes is NULL, not 16-byte aligned or less than %zu",
                     what, workspace_bytes, l.bytes);

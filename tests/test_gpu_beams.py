@@ -271,7 +271,7 @@ def test_refused_arguments():
     p = ptr(t)
 
     def call(shape=None, **args):
-        base = dict(groups=1, logits=p, scores=p, ended=0, scores_out=p, tokens=p, parents=p, ended_out=0, history=0, known=0, history_out=0,
+        base = dict(groups=1, logits=p, scores=p, ended=0, scores_out=p + 1024, tokens=p, parents=p, ended_out=0, history=0, known=0, history_out=0,
                     workspace=p, workspace_bytes=1 << 16)
         B.beam_select(B.Beams(**{"dtype": F32, "beams": 2, "picks": 2, "vocab": 10, **(shape or {})}), **{**base, **args})
 
@@ -281,7 +281,8 @@ def test_refused_arguments():
                          (dict(shape=dict(end_token=-2)), "end token"), (dict(shape=dict(logits_stride=9)), "overlap"),
                          (dict(shape=dict(history_stride=-1)), "history"), (dict(groups=-1), "groups"), (dict(groups=2 ** 31 - 1), "too many"),
                          (dict(logits=0), "NULL"), (dict(scores=0), "NULL"), (dict(parents=0), "NULL"), (dict(history=p), "NULL"),
-                         (dict(history=p, known=p, history_out=p), "history_out"), (dict(ended=p), "end token"), (dict(workspace=0), "workspace"),
+                         (dict(shape=dict(history_stride=4), history=p, known=p, history_out=p + 16), "history_out"),
+                         (dict(scores_out=p + 4), "scores_out"), (dict(shape=dict(end_token=1), ended=p, ended_out=p + 1), "ended_out"), (dict(ended=p), "end token"), (dict(workspace=0), "workspace"),
                          (dict(workspace=p + 8), "workspace"), (dict(workspace_bytes=40), "workspace")):
         with pytest.raises(M.MFHError, match=message):
             call(**bad)

@@ -309,6 +309,66 @@ def test_another_stream_and_a_captured_step():
         s.kv = whole
 
 
+# Of 256 columns of a group on, and long shared tokens (of which only the bound is long here), prefill's kernels compute them.
+MANY = [(200, [201, 330, 200, 0, 260]), (64, [65, 64, 130, 20]), (1, [2] * 6), (0, [7, 0, 1, 40]), (257, [300, 258, 259, 9])]
+
+
+@pytest.mark.parametrize("dtype, cache", [(BF16, BF16), (F16, F16), (BF16, FP8), (F16, FP8)])
+@pytest.mark.parametrize("hq, hk, dim, page, order", [(64, 1, 64, 16, "head"), (130, 2, 128, 7, "token"), (64, 1, 80, 100, "head"), (64, 1, 256, 48, "token"),
+                                                      (192, 2, 192, 1, "token")])
+def test_many_columns_against_f64(dtype, cache, hq, hk, dim, page, order):
+    s = Shared(dtype, cache, MANY, hq, hk, dim, page, order, seed=dim + page, q_std=2.0, outside=((5, 0), (33,)))
+    out, lse = s.run(most_shared=1 << 24)
+    s.check(out, lse)
+    first = s.run(most_shared=1 << 24)
+    assert torch.equal(first[0], out) and torch.equal(first[1], lse)
+
+
+@pytest.mark.parametrize("option", [dict(window=1), dict(window=33), dict(window=130), dict(window=10 ** 9), dict(softcap=20.0), dict(slopes=True),
+                                    dict(slopes=True, softcap=5.0, window=90), dict(scale=-0.3), dict(scale=0.0), dict(softcap=1e5)])
+@pytest.mark.parametrize("page, dim", [(16, 64), (10, 128)])
+def test_many_columns_with_window_cap_and_bias(option, page, dim):
+    s = Shared(BF16, BF16, MANY, 64, 1, dim, page, seed=5, q_std=3.0, **dict(option))
+    s.check(*s.run(most_shared=1 << 24))
+
+
+def test_many_columns_over_several_parts():
+    s = Shared(BF16, BF16, [(3000, [3001, 3100, 2990, 3000, 3600])], 64, 1, 64, 16, seed=6)
+    s.check(*s.run(most_shared=1 << 16))
+    s.table[0, 100] = -1  # a page of the shared tokens is none of the cache's
+    out, lse = s.run(most_shared=1 << 16)
+    keep = torch.cat([torch.arange(1600), torch.arange(1616, 3000)])
+    for r in (0, 2):
+        k = torch.cat([keep, torch.arange(3000, s.lengths[r])]) if s.lengths[r] > 3000 else keep[: s.lengths[r] - 16]
+        want = attention_oracle(s.q[r: r + 1].double(), s.kv[r][0][k], s.kv[r][1][k], [10 ** 6], s.scale)
+        check_attention(out[r: r + 1], lse[r: r + 1], want, BF16, 64)
+
+
+@pytest.mark.parametrize("cache", [BF16, FP8])
+def test_many_columns_and_values_that_are_not_finite(cache):
+    s = Shared(BF16, cache, [(100, [101, 130, 140, 60])], 64, 1, 64, 16, seed=12, window=50)
+    want = s.oracle()
+    value = math.nan if cache == FP8 else math.inf
+    for t, dim, what in ((70, 5, value), (20, 6, value), (99, 7, math.nan)):
+        s.cache.views[1][int(s.table[0, t // 16]), t % 16, 0, dim] = 127 if cache == FP8 else what
+    out, lse = s.run(most_shared=1 << 24)
+    got, exact = out.double().cpu(), want[0]
+    assert torch.isfinite(got[:, :, 8:]).all() and torch.isfinite(lse).all()
+    for dim, rows in {5: [0], 6: [3], 7: [0, 1, 2]}.items():
+        for r in range(4):
+            if r in rows:
+                assert (torch.isnan(got[r, :, dim]) if dim == 7 or cache == FP8 else got[r, :, dim] == math.inf).all(), (dim, r)
+            else:
+                assert ((got[r, :, dim] - exact[r, :, dim]).abs() < 0.05).all(), (dim, r)
+
+
+def test_many_requests_with_few_tokens_of_their_own():
+    # four rows a CU and more: a wave a row
+    lengths = [(40, [40 + (7 * g + i) % 50 for i in range(4)]) for g in range(70)]
+    s = Shared(F16, F16, lengths, 16, 8, 64, 16, seed=21, outside=((3,), ()))
+    s.check(*s.run())
+
+
 def test_no_requests_and_no_groups():
     s = Shared(F16, F16, [], 4, 2, 64, 16, seed=4, outside=((30, 0, 77), ()))
     s.check(*s.run())
