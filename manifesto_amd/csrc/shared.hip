@@ -9,12 +9,15 @@
 // them.  A request's own tokens are a group of one request.  Both kinds of
 // parts run in one launch, the shared ones first, and a second one joins them.
 //
-// A wave takes tiles of 32 tokens on its own, from memory straight into the
-// matrix operands (decode.hpp); V is turned once for all columns.  Columns see
+// A wave takes tiles of 32 tokens on its own: whole rows of K and V into registers
+// while the tile before is worked on, from there to its part of LDS, and out of it
+// as matrix operands, V turned on the way, once for all columns.  Columns see
 // different tokens (a window, a request shorter than its group's shared
 // tokens), so that a value that is not finite may be seen by some only: it is
 // cut to zero in the product and added to those columns by itself.
 #include "decode.hpp"
+
+#include <numeric>
 
 namespace mfh {
 
@@ -42,12 +45,11 @@ struct SharedArgs {
     int cap;
     int32_t window, kv_heads, q_heads, group, head_groups, dim;
     mfh_u32 requests, groups, group_step;  // group_step: groups between two that are looked at first
-    mfh_u32 lines;                         // columns in 16, 32 or 64, of all groups, at most
     mfh_u32 shared_blocks;
     mfh_u32 shared_parts, own_parts, parts, shared_piece, own_piece;  // piece: tiles of a part
     bool all_parts;  // every request of a group has as many shared parts as there are
     bool alone;      // a wave takes a request's own part alone
-    Divider by_group, by_lines, by_shared_parts, by_own_parts, by_kv_heads, by_head_groups, by_shared_piece, by_own_piece, by_q_heads;
+    Divider by_group, by_kv_parts, by_shared_parts, by_own_parts, by_kv_heads, by_head_groups, by_shared_piece, by_own_piece, by_q_heads;
 };
 
 MFH_DEV mfh_u32 limited(const SharedArgs& a, int32_t tokens)
@@ -587,9 +589,10 @@ __global__ __launch_bounds__(kThreads, SETS > 2 || DP == 256 ? 1 : SETS > 1 || D
     const int lane = threadIdx.x & 63;
     if (blockIdx.x < a.shared_blocks) {
         // Workgroups of one head and part, which read the same keys if they are of
-        // one group, are on one XCD (every eighth is), one after the other.
-        const mfh_u32 eighth = blockIdx.x >> 3, high = a.by_lines.quotient(eighth), line = eighth - high * a.lines;
-        const mfh_u32 kv_part = high * 8 + (blockIdx.x & 7);
+        // one group, are on one XCD (every eighth is).  Lines that no group has come
+        // last: workgroups go to an XCD's shader engines in turn, and with every fourth
+        // an empty one 240 others took two rounds on 256 CUs, 100 us for 67.
+        const mfh_u32 line = a.by_kv_parts.quotient(blockIdx.x), kv_part = blockIdx.x - line * a.by_kv_parts.d;
         const mfh_u32 kv = a.by_shared_parts.quotient(kv_part), part = kv_part - kv * a.shared_parts;
         if (kv >= (mfh_u32)a.kv_heads) return;
         constexpr mfh_u32 kColumns = kHeads * SETS;
@@ -710,25 +713,26 @@ void launch_join(const SharedArgs& a, hipStream_t s)
 //
 // Shared tokens: sets of 16 columns, as many as a group has on average, up to 64
 // columns, with which a workgroup fills a CU (24 groups of 4 to 32 columns over up
-// to 6000 e4m3 tokens: by 64 columns 94 us, by 32 48 us), and to 32 where there is
-// less to share than each request has for itself, whose workgroups a CU then holds
-// two of.  Of 256 columns on and
-// long shared tokens prefill's kernels, whose tiles serve 256 columns, are
-// faster: 256 requests of 32 heads over 8, 16384 tokens, 141 us, else 166; 64 such
-// requests over 65536 133 us, else 160; but over 8192 56 and 54, and 128 requests
-// over 2000 64 and 58.
+// to 6000 e4m3 tokens: by 64 columns 94 us, by 32 48), and to 32 where there is less
+// to share than each request has for itself, whose workgroups a CU then holds two
+// of.  Of 256 columns on and long shared tokens prefill's kernels, whose tiles serve
+// 256 columns, are faster: 256 requests of 32 heads over 8, 16384 tokens, 120 us,
+// else 145; 64 such requests over 65536 122, else 146; but over 8192 47 and 43.
 //
-// Parts: as many as CUs hold workgroups, one of 64 columns or of heads wider than
-// 128 (64 requests over 8192 tokens 55 us, twice as many 64; two groups of eight
-// over 131072 tokens of 256 dims 153 and 161) and two of fewer columns, and half as
-// many again where groups may differ (the 24 groups: 48 us, 42 to 50).  Eight tiles
-// at least.  Of a request's own tokens two workgroups a CU, or, where there are
-// four rows a CU and more, a wave a row: 256 requests of up to 300 own tokens 39 us,
-// by workgroups 44.
+// Parts: as many as fill half of the card, so that the requests' own parts run beside
+// them on the other half; where the shared tokens take the waves many rounds (`rounds`,
+// against those of the own tokens), as many as fill the card, and the own parts come
+// after them.  Half: 64 requests over 8192 tokens and 512 of their own 42 us, a full
+// card 54; 32 over 4000 and 500 in four groups 55 and 64.  A full card: 48 requests
+// over 30000 and 30 67, half of it 92.  Two parts at least where groups may differ
+// (those 24: 50 us, with one 63), eight tiles at least.  Of a request's own tokens two
+// workgroups a CU, or, where there are four rows a CU and more, a wave a row: 256
+// requests of up to 300 own tokens 39 us, by workgroups 44.
 struct Layout {
     bool prefill, alone;
     int sets;
-    int64_t lines, shared_blocks, own_blocks;
+    int64_t shared_blocks, own_blocks;
+    mfh_u32 kv_parts;  // key-value heads times shared parts, in eights
     mfh_u32 shared_parts, own_parts, shared_piece, own_piece;
     size_t bytes;
 };
@@ -740,9 +744,13 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     const int group = sh.q_heads / c.kv_heads, cus = dev->compute_units;
     const int64_t columns = (int64_t)requests * group, each = groups > 0 ? columns / groups : 0;
     const int64_t tokens = std::min<int64_t>(std::max<int64_t>(most_shared, 1), kLongest);
+    const int64_t own = std::min<int64_t>(std::max<int64_t>(most_own, 1), kLongest);
     l.prefill = each >= 256 && each * tokens >= (1 << 22) && groups <= 16;
     l.sets = each <= 16 || l.prefill ? 1 : each <= 32 || c.head_dim > 128 || tokens < most_own ? 2 : 4;
-    l.lines = columns / (kHeads * l.sets) + groups;
+    // Columns in 16, 32 or 64, of all groups, at most: a group's number of columns is a
+    // multiple of `step`, so that its last line leaves at most that much less than a line.
+    const int64_t wide = kHeads * l.sets, step = std::gcd((int64_t)group, wide);
+    const int64_t lines = (columns + std::min<int64_t>(groups, requests) * (wide - step)) / wide;
     auto split = [](int64_t blocks, int64_t rows, int64_t tokens, mfh_u32& piece, mfh_u32& parts) {
         const int64_t tiles = (tokens + kTile - 1) / kTile + 1, wanted = std::max<int64_t>(1, blocks / std::max<int64_t>(rows, 1));
         piece = (mfh_u32)std::max<int64_t>(8, (tiles + wanted - 1) / wanted);
@@ -753,12 +761,19 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
         l.shared_parts = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>({cus / rows, tokens / 256, 64}));
         l.shared_piece = 1;
     } else {
-        const int blocks = l.sets > 2 || c.head_dim > 128 ? cus : groups > 1 ? 3 * cus : 2 * cus;
-        split(blocks, std::max<int64_t>(groups, columns / (kHeads * l.sets)) * c.kv_heads, tokens, l.shared_piece, l.shared_parts);
+        // Rounds of tiles that the waves take if shared parts have all workgroups that
+        // the card holds, and those of the own parts after them.
+        const int64_t held = l.sets > 2 || c.head_dim > 128 ? cus : 2 * cus, waves = held * kWaves;
+        const int64_t rows = std::max<int64_t>(groups, columns / wide) * c.kv_heads;
+        const int64_t heads = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads);
+        const int64_t rounds = rows * (tokens / kTile) / waves, after = heads * (own / kTile + 1) / waves;
+        const int64_t blocks = rounds > 8 + 2 * after ? held : held / 2;
+        split(groups > 1 ? std::max(blocks, 2 * rows) : blocks, rows, tokens, l.shared_piece, l.shared_parts);
     }
-    split(2 * cus, (int64_t)requests * c.kv_heads, std::min<int64_t>(std::max<int64_t>(most_own, 1), kLongest), l.own_piece, l.own_parts);
+    split(2 * cus, (int64_t)requests * c.kv_heads, own, l.own_piece, l.own_parts);
     if (groups == 0) l.shared_parts = 0;
-    l.shared_blocks = l.prefill ? 0 : ((int64_t)c.kv_heads * l.shared_parts + 7) / 8 * 8 * l.lines;
+    l.kv_parts = (mfh_u32)(((int64_t)c.kv_heads * l.shared_parts + 7) / 8 * 8);
+    l.shared_blocks = l.prefill ? 0 : l.kv_parts * lines;
     l.own_blocks = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads) * l.own_parts;
     l.alone = l.own_blocks >= 4 * cus;
     if (l.alone) l.own_blocks = (l.own_blocks + kWaves - 1) / kWaves;
@@ -862,11 +877,11 @@ int mfh_paged_decode_shared(const mfh_attention_shape* shape, const mfh_kv_cache
     a.head_groups = (a.group + kHeads - 1) / kHeads;
     a.dim = cache->head_dim;
     a.requests = (mfh_u32)requests, a.groups = (mfh_u32)groups, a.group_step = (mfh_u32)(groups + 63) / 64;
-    a.lines = (mfh_u32)l.lines, a.shared_blocks = (mfh_u32)l.shared_blocks;
+    a.shared_blocks = (mfh_u32)l.shared_blocks;
     a.shared_parts = l.shared_parts, a.own_parts = l.own_parts, a.parts = l.shared_parts + l.own_parts;
     a.part_out = (float*)workspace;
     a.part_sum = (float2*)(a.part_out + (int64_t)requests * a.q_heads * a.parts * a.dim);
-    a.by_group = Divider((mfh_u32)a.group), a.by_lines = Divider(std::max(a.lines, 1u));
+    a.by_group = Divider((mfh_u32)a.group), a.by_kv_parts = Divider(std::max(l.kv_parts, 1u));
     a.by_shared_parts = Divider(std::max(a.shared_parts, 1u)), a.by_own_parts = Divider(a.own_parts);
     a.by_kv_heads = Divider((mfh_u32)a.kv_heads), a.by_head_groups = Divider((mfh_u32)a.head_groups);
     a.by_shared_piece = Divider(l.shared_piece), a.by_own_piece = Divider(l.own_piece), a.by_q_heads = Divider((mfh_u32)a.q_heads);
