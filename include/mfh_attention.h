@@ -133,7 +133,7 @@ int mfh_page_plan(const int32_t* before, const int32_t* after, int32_t requests,
  *
  * The workspace (mfh_page_fork_workspace bytes, any 16-byte aligned device
  * memory, free for other use once the call's work is done) has to be as large
- * as it says, which may be 0. */
+ * as it says. */
 int mfh_page_fork(const int32_t* parents, const int32_t* before, const int32_t* keep, int32_t requests,
                   int32_t page_size, const int32_t* table, int32_t* table_out, int64_t table_stride,
                   int32_t table_width, const int32_t* shares, int32_t* shares_out, int64_t pages, int32_t* ring,

@@ -56,8 +56,9 @@ typedef struct {
  *
  * history, if not NULL, holds the tokens of each row so far, known[g] of
  * them in group g ([rows][history_stride]); history_out ([groups * picks]
- * [history_stride]) gets the parent's with the new token behind them.  Tokens that do not fit the stride are not written, nor is the
- * row of a result without parent; what stands behind stays as it is.
+ * [history_stride]) gets the parent's with the new token behind them.  Tokens
+ * that do not fit the stride are not written, nor is the row of a result
+ * without parent; what stands behind stays as it is.
  *
  * scores_out, ended_out and history_out are other buffers than scores, ended
  * and history.  The workspace (any 16-byte aligned device memory, free for

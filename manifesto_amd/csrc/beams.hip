@@ -22,6 +22,10 @@
 // rounding, 2^-25 of |l - max| log2(e), which the sum averages to about 1e-8.
 // The histories' rows are cut over several workgroups, each of which merges
 // again: that costs less than one more launch.
+//
+// A step of few rows is two launches' latency: 4 rows of 32003 f32 6.2 and 5.7 us.
+// 256 rows of 131072 bf16 (67 MB, 13 us at a copy's rate) take 19.7 and 7.4: beside
+// the loads stand the exponentials, and two barriers and the list of each piece.
 #include "common.hpp"
 #include "launch.hpp"
 #include "paged.hpp"
@@ -440,6 +444,8 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
 
 // Packets of a thread: as many as leave every CU two workgroups, for what a
 // workgroup does once (the bound, the list) costs the same whatever its piece.
+// 256 rows of 131072 bf16: by 8 packets 27 us, by 1 47; 35 rows of 50001 f16: by 1
+// 12.8 us, by 8 16; 64 rows of 32003 f32: by 2 as here 14.5, by 4 13.8, by 8 15.5.
 struct Layout {
     int packets;
     int64_t pieces;

@@ -14,9 +14,11 @@
 // places are a running sum over the pages' counts.
 //
 // Where pages and requests are few one workgroup does all of it, with the counts in
-// LDS: latency bounds it.  Else there are four launches: what concerns each
+// LDS: latency bounds it, 9 us.  Else there are four launches: what concerns each
 // request once (one workgroup) beside the counts' copy, the tables, the number of
-// pages that go back in each piece of the counts, and those pages.  (Numbers
+// pages that go back in each piece of the counts, and those pages.  For 1021
+// requests of up to 512 pages they take 5, 9, 3 and 4 us: the chain of loads, the
+// atomics, and the starts of launches bound them, not the 3 MB that move.  (Numbers
 // kept by the second launch, as pages fall below zero, are a launch less, but
 // atomics on a few words: 1021 requests that return 28800 pages, 58 us.)
 #include "common.hpp"
@@ -29,7 +31,9 @@ namespace {
 constexpr int kThreads = 1024;  // of a workgroup that plans
 constexpr int kWaves = kThreads / 64;
 constexpr mfh_u32 kMostRequests = 8192;
-constexpr mfh_u32 kFewRequests = 1024, kFewPages = 32768;  // of the form in one workgroup
+// The form in one workgroup: 9 us for 64 requests of up to 125 pages, in four launches
+// 17; from some 14000 table entries on those are faster (25000: 26 and 17 us).
+constexpr mfh_u32 kFewRequests = 1024, kFewPages = 16384, kFewEntries = 12288;
 constexpr mfh_u32 kChunk = 4 * kThreads;                   // pages of a workgroup that returns them
 constexpr mfh_u32 kNone = 0xffffffffu;
 
@@ -358,6 +362,8 @@ size_t fork_workspace(int32_t requests, int64_t pages)
 
 // A page's rows (one token of one head) in pieces of 16 bytes, in the order in
 // which they stand in memory; a workgroup takes kPieces * kCopyThreads of them.
+// Memory bounds it: 1000 pages of 64 tokens, 8 heads of 128 e4m3 (262 MB read and
+// written) take 52 us, 5.0 TB/s, what a large copy reaches; a step's 64 pages 3.5 us.
 constexpr int kCopyThreads = 256;
 constexpr int kPieces = 4;
 
@@ -465,7 +471,7 @@ int mfh_page_fork(const int32_t* parents, const int32_t* before, const int32_t* 
     a.rows = (u32x4*)workspace, a.freed = (mfh_u32*)(a.rows + requests);
     a.by_page = Divider((mfh_u32)page_size), a.by_width = Divider((mfh_u32)std::max(table_width, 1));
     hipStream_t s = (hipStream_t)stream;
-    if (requests <= (int32_t)kFewRequests && pages <= (int64_t)kFewPages && (int64_t)requests * table_width <= 65536) {
+    if (requests <= (int32_t)kFewRequests && pages <= (int64_t)kFewPages && (int64_t)requests * table_width <= kFewEntries) {
         k_fork_few<<<1, kThreads, 0, s>>>(a);
         return launch_status("k_fork_few");
     }

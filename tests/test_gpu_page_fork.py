@@ -145,11 +145,11 @@ def test_forks_match_the_loop(n, page, keep):
     same(fork(*args, in_place=True), want)
 
 
-@pytest.mark.parametrize("pages", [32768, 32769, 100_001])
-def test_many_pages(pages):
-    # the count in LDS ends at 32768 pages; pages that go back stand in many chunks
+@pytest.mark.parametrize("n, pages", [(100, 16384), (102, 16384), (103, 16384), (100, 16385), (300, 32769), (300, 100_001)])
+def test_many_pages(n, pages):
+    # the count in LDS ends at 16384 pages and 12288 entries; pages that go back stand in many chunks
     rng = np.random.default_rng(pages)
-    n, page, width = 300, 4, 120
+    page, width = 4, 120
     before, table, shares, ring, head, tail = state(rng, n, page, width, 400, spare=400)
     more = pages - len(shares)
     assert more > 0
