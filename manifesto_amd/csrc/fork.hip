@@ -176,7 +176,7 @@ MFH_DEV mfh_u32 plan(const ForkArgs& a, mfh_u32* s_first, mfh_u32* s_heir, mfh_u
 // Row r's new entry c, and what of the old one nobody takes over: page numbers
 // are asked for in `load`, for several entries at a time, and dealt with in `finish`.
 struct Entry {
-    mfh_u32 r, c, cover, copied, heir_cover, heir_copied;
+    mfh_u32 r, c;
     bool write, drop, adds;
     int32_t from, old, fresh;
     // row: of r; heir: of r's heir, if it has one; first: whether r is its parent's heir
