@@ -247,7 +247,8 @@ int mfh_paged_decode_workspace(const mfh_attention_shape* shape, const mfh_kv_ca
  * and most_own are the caller's upper bounds of the shared tokens and of a
  * request's own ones: they decide how both are split over workgroups, and with
  * it the order of the sums, nothing else.  The workspace has to be as large as
- * mfh_paged_decode_shared_workspace says for these sizes. */
+ * mfh_paged_decode_shared_workspace says for these sizes; what it says for sizes
+ * that are nowhere smaller (requests, groups and both bounds) does too. */
 int mfh_paged_decode_shared(const mfh_attention_shape* shape, const mfh_kv_cache* cache, int32_t requests,
                             int32_t groups, const void* q, const void* k_cache, const void* v_cache,
                             const int32_t* table, int64_t table_stride, int32_t table_width, const int32_t* starts,

@@ -740,6 +740,26 @@ struct Layout {
     size_t bytes;
 };
 
+bool prefill_pays(int64_t columns, int64_t tokens) { return columns >= 256 && columns * tokens >= (1 << 22); }
+
+// Rows of parts (requests * q_heads, times the parts of each) at most, of these sizes
+// and of all smaller ones: fewer rows, or fewer own tokens, may have more parts each.
+// A row has as many parts as tokens give, a part for eight tiles, and a call:
+//   own parts     2 * cus / (requests * kv_heads) a row, so 2 * cus * group, or one each;
+//   shared parts  held / (max(1, columns / wide) * kv_heads) a row, of columns * kv_heads
+//                 rows: less than 2 * wide * held, which is 128 * cus; or two each;
+//   prefill's     cus / (each / P * kv_heads * groups) a row, P its workgroup's rows, of less
+//                 than (each + 1) * groups * kv_heads rows, where `each` is at least 256:
+//                 less than 257 * cus for its 256 rows.
+int64_t part_rows(int64_t cus, int64_t requests, int64_t groups, int64_t group, int64_t kv_heads, int64_t tokens, int64_t own)
+{
+    const int64_t rows = requests * group * kv_heads, columns = requests * group;
+    auto by_tokens = [&](int64_t t) { return rows * (((t + kTile - 1) / kTile + 1 + 7) / 8); };
+    const int64_t card = (prefill_pays(columns, tokens) ? 257 : 128) * cus;
+    const int64_t own_rows = std::min(by_tokens(own), std::max(rows, 2 * cus * group));
+    return own_rows + (groups > 0 ? std::min(by_tokens(tokens), std::max(2 * rows, card)) : 0);
+}
+
 Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cache& c, int32_t requests, int32_t groups,
               int64_t most_shared, int64_t most_own)
 {
@@ -748,7 +768,7 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     const int64_t columns = (int64_t)requests * group, each = groups > 0 ? columns / groups : 0;
     const int64_t tokens = std::min<int64_t>(std::max<int64_t>(most_shared, 1), kLongest);
     const int64_t own = std::min<int64_t>(std::max<int64_t>(most_own, 1), kLongest);
-    l.prefill = each >= 256 && each * tokens >= (1 << 22) && groups <= 16;
+    l.prefill = prefill_pays(each, tokens) && groups <= 16;
     l.sets = each <= 16 || l.prefill ? 1 : each <= 32 || c.head_dim > 128 || tokens < most_own ? 2 : 4;
     // Columns in 16, 32 or 64, of all groups, at most: a group's number of columns is a
     // multiple of `step`, so that its last line leaves at most that much less than a line.
@@ -780,7 +800,7 @@ Layout layout(const Device* dev, const mfh_attention_shape& sh, const mfh_kv_cac
     l.own_blocks = (int64_t)requests * c.kv_heads * ((group + kHeads - 1) / kHeads) * l.own_parts;
     l.alone = l.own_blocks >= 4 * cus;
     if (l.alone) l.own_blocks = (l.own_blocks + kWaves - 1) / kWaves;
-    l.bytes = (size_t)requests * sh.q_heads * (l.shared_parts + l.own_parts) * (c.head_dim + 2) * sizeof(float);
+    l.bytes = (size_t)part_rows(cus, requests, groups, group, c.kv_heads, tokens, own) * (c.head_dim + 2) * sizeof(float);
     return l;
 }
 
@@ -813,8 +833,12 @@ int check_shared(const Device* dev, const mfh_attention_shape* shape, const mfh_
     if (requests < 0) return fail(MFH_ERR_INVALID_ARGUMENT, "%s: negative number of requests %d", what, requests);
     if (groups < 0 || groups > kMostGroups)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d groups are not within 0..%d", what, groups, kMostGroups);
-    *l = layout(dev, *shape, *cache, requests, groups, most_shared, most_own);
-    if ((int64_t)requests * shape->q_heads > (1 << 22) || l->shared_blocks + l->own_blocks >= (int64_t(1) << 32) / kThreads)
+    bool many = (int64_t)requests * shape->q_heads > (1 << 22);
+    if (!many) {
+        *l = layout(dev, *shape, *cache, requests, groups, most_shared, most_own);
+        many = l->shared_blocks + l->own_blocks >= (int64_t(1) << 32) / kThreads;
+    }
+    if (many)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %d requests of %d heads are too many for one call", what, requests,
                     shape->q_heads);
     return MFH_OK;
