@@ -60,7 +60,7 @@ class BeamSearch(_paged.PagedAttention):
         self.select_space = torch.empty(B.beam_select_workspace(self.shape, requests), dtype=torch.uint8, device="cuda")
         # the shared attention's: beams of a request, and the whole pages of its prompt
         self.group_starts = torch.arange(0, rows + 1, beams, dtype=torch.int32, device="cuda")
-        self.shared, self.most_shared = ints(requests), longest
+        self.shared, self.most_shared, self.most_own = ints(requests), longest, longest
         need = A.paged_decode_shared_workspace(self.attention, self.cache, rows, requests, longest, longest)
         self.shared_space = torch.empty(need, dtype=torch.uint8, device="cuda")
 
@@ -98,6 +98,8 @@ class BeamSearch(_paged.PagedAttention):
         self.known.copy_(torch.tensor([len(x) for x in prompts], dtype=torch.int32))
         self.shared.copy_(self.known // self.page_size * self.page_size)
         self.most_shared = int(self.shared.max())
+        # what does not fill a page of the prompt, and the steps that the longest prompt leaves
+        self.most_own = min(self.page_size - 1 + self.longest - max(len(x) for x in prompts), self.longest)
         # of each request only the first beam is there yet
         self.scores.fill_(float("-inf"))
         self.scores[:: self.beams] = 0.0
@@ -123,7 +125,7 @@ class BeamSearch(_paged.PagedAttention):
         A.rotary_append(self.rotary, self.cache, n, p(qkv), p(q), p(qkv) + at_k, p(qkv) + at_k + self.kv_heads * self.head_dim * 2,
                         p(positions), p(slots), p(self.frequencies), p(self.keys), p(self.values), stream=stream)
         A.paged_decode_shared(self.attention, self.cache, n, self.groups, p(q), p(self.keys), p(self.values), p(self.table), self.width,
-                              p(self.group_starts), p(self.shared), self.most_shared, p(self.lengths), self.longest - self.most_shared, 0,
+                              p(self.group_starts), p(self.shared), self.most_shared, p(self.lengths), self.most_own, 0,
                               p(out), 0, p(self.shared_space), self.shared_space.numel(), stream=stream)
         return out, q
 
