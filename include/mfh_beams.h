@@ -63,7 +63,8 @@ typedef struct {
  * scores_out, ended_out and history_out are other buffers than scores, ended
  * and history.  The workspace (any 16-byte aligned device memory, free for
  * other use once the call's work is done) has to be as large as
- * mfh_beam_select_workspace says. */
+ * mfh_beam_select_workspace says; what it says for more groups, beams, picks or
+ * tokens does too. */
 int mfh_beam_select(const mfh_beam_shape* shape, int32_t groups, const void* logits, const float* scores,
                     const uint8_t* ended, float* scores_out, int32_t* tokens, int32_t* parents, uint8_t* ended_out,
                     const int32_t* history, const int32_t* known, int32_t* history_out, void* workspace,

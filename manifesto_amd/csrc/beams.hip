@@ -456,13 +456,17 @@ Layout layout(const Device* dev, const mfh_beam_shape& sh, int32_t groups)
 {
     Layout l{};
     const int64_t rows = (int64_t)groups * sh.beams;
-    auto with_packets = [&](int packets) {
+    auto pieces_by = [&](int packets) {
         const int64_t piece = (int64_t)kThreads * packets * (sh.dtype == kFloat32 ? 4 : 8);
-        l.packets = packets, l.pieces = (sh.vocab + piece - 1) / piece;
+        return (sh.vocab + piece - 1) / piece;
     };
-    with_packets(8);
-    while (l.packets > 1 && rows * l.pieces < 2 * dev->compute_units) with_packets(l.packets / 2);
-    l.bytes = (size_t)(rows * l.pieces) * (sh.picks * sizeof(mfh_u64) + sizeof(double) + sizeof(float));
+    l.packets = 8;
+    while (l.packets > 1 && rows * pieces_by(l.packets) < 2 * dev->compute_units) l.packets /= 2;
+    l.pieces = pieces_by(l.packets);
+    // Room for all smaller calls too, whose rows may be in more pieces: less than 2 * cus
+    // of twice the packets are less than 4 * cus.
+    const int64_t most = std::min(rows * pieces_by(1), std::max<int64_t>(rows * pieces_by(8), 4 * dev->compute_units));
+    l.bytes = (size_t)most * (sh.picks * sizeof(mfh_u64) + sizeof(double) + sizeof(float));
     return l;
 }
 
