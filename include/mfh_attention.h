@@ -127,9 +127,9 @@ int mfh_page_plan(const int32_t* before, const int32_t* after, int32_t requests,
  * table and table_out are different buffers [requests][table_stride]; entries
  * behind a request's pages keep what table_out held.  shares and shares_out
  * have `pages` entries and may be one buffer, ring and its states are
- * mfh_page_plan's, lengths is another buffer than before.  requests <= 8192,
- * pages <= ring_size.  Negative shares count as 0; page numbers outside the
- * cache are handed on, and not counted.
+ * mfh_page_plan's; lengths, status and the list of copies are other buffers than
+ * before and table.  requests <= 8192, pages <= ring_size.  Negative shares count
+ * as 0; page numbers outside the cache are handed on, and not counted.
  *
  * The workspace (mfh_page_fork_workspace bytes, any 16-byte aligned device
  * memory, free for other use once the call's work is done) has to be as large

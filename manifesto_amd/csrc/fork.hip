@@ -447,18 +447,25 @@ int mfh_page_fork(const int32_t* parents, const int32_t* before, const int32_t* 
         (requests > 0 && (!parents || !before || !lengths || !status || !copy_from || !copy_to || !copy_tokens ||
                           (table_width > 0 && (!table || !table_out)))))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: NULL buffer", what);
-    if (ring_state == ring_state_out)
-        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: ring_state_out is ring_state, which other workgroups still read",
-                    what);
-    auto overlap = [](const void* p, const void* q, int64_t entries) {
-        return (uintptr_t)p < (uintptr_t)q + entries * 4 && (uintptr_t)q < (uintptr_t)p + entries * 4;
+    auto overlap = [](const void* p, int64_t p_bytes, const void* q, int64_t q_bytes) {
+        return (uintptr_t)p < (uintptr_t)q + q_bytes && (uintptr_t)q < (uintptr_t)p + p_bytes;
     };
-    if (requests > 0 && table_width > 0 &&
-        overlap(table, table_out, (int64_t)(requests - 1) * table_stride + table_width))
+    if (overlap(ring_state, 16, ring_state_out, 16))
+        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: ring_state_out overlaps ring_state, which other workgroups still read",
+                    what);
+    const int64_t row_bytes = (int64_t)requests * 4;
+    const int64_t table_bytes = requests > 0 && table_width > 0 ? ((requests - 1) * table_stride + table_width) * 4 : 0;
+    if (table_bytes && overlap(table, table_bytes, table_out, table_bytes))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: table_out overlaps table, which is still read", what);
-    if (requests > 0 && overlap(lengths, before, requests))
-        return fail(MFH_ERR_INVALID_ARGUMENT, "%s: lengths overlaps before, which is still read", what);
-    if (shares != shares_out && overlap(shares, shares_out, pages))
+    const struct { const char* name; const int32_t* at; } results[] = {
+        {"lengths", lengths}, {"status", status}, {"copy_from", copy_from}, {"copy_to", copy_to}, {"copy_tokens", copy_tokens}};
+    for (const auto& r : results) {
+        if (requests > 0 && overlap(r.at, row_bytes, before, row_bytes))
+            return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %s overlaps before, which is still read", what, r.name);
+        if (table_bytes && overlap(r.at, row_bytes, table, table_bytes))
+            return fail(MFH_ERR_INVALID_ARGUMENT, "%s: %s overlaps table, which is still read", what, r.name);
+    }
+    if (shares != shares_out && overlap(shares, pages * 4, shares_out, pages * 4))
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: shares_out overlaps shares without being it", what);
     if (workspace_bytes < need || !workspace || (uintptr_t)workspace % 16)
         return fail(MFH_ERR_INVALID_ARGUMENT, "%s: a workspace of %zu bytes is NULL, not 16-byte aligned or less than %zu",
