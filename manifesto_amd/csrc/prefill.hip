@@ -115,7 +115,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     const int prefix = !SHARED && a.prefix ? min(max(a.prefix[r], 0), length) : 0;
     const int first_position = length - (int)fresh;  // of the request's new tokens; may be negative
     // Where a token of the group stands in its request, -1 without one; and the least
-    // and the greatest of some.
+    // and the greatest of some.  Returns the least of those that there are.
     auto stands = [&](mfh_u32 token) {
         if constexpr (SHARED) return (int)min((mfh_u64)max(a.lengths[begin + token], 0), most) - 1;
         else return first_position + (int)token;
@@ -123,13 +123,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
     auto range = [&](mfh_u32 first_row, mfh_u32 last_row, int& low, int& high) {
         const mfh_u32 first = a.by_group.quotient(first_row), last = a.by_group.quotient(last_row);
         if constexpr (SHARED) {
-            low = kLongest, high = -1;
-            for (mfh_u32 t = first + lane; t <= last; t += 64) low = min(low, stands(t)), high = max(high, stands(t));
+            mfh_u32 least = kLongest;  // (-1 is the greatest number)
+            high = -1;
+            bool ended = false;
+            for (mfh_u32 t = first + lane; t <= last; t += 64) {
+                const int at = stands(t);
+                least = min(least, (mfh_u32)at), high = max(high, at), ended |= at < 0;
+            }
 #pragma unroll
-            for (int x = 1; x < 64; x <<= 1) low = min(low, __shfl_xor(low, x)), high = max(high, __shfl_xor(high, x));
-            low = (int)uniform((mfh_u32)low), high = (int)uniform((mfh_u32)high);
+            for (int x = 1; x < 64; x <<= 1) least = min(least, (mfh_u32)__shfl_xor((int)least, x)), high = max(high, __shfl_xor(high, x));
+            high = (int)uniform((mfh_u32)high);
+            low = __any(ended) ? -1 : (int)uniform(least);
+            return (int)uniform(least);
         } else {
             low = stands(first), high = stands(last);
+            return low;
         }
     };
 
@@ -139,9 +147,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void k_prefill(PrefillArgs a
 
     // Positions of the workgroup's rows, and the keys any of them sees.
     int low_position, high_position;
-    range(row0, min(row0 + kRows, rows) - 1, low_position, high_position);
+    const int least_position = range(row0, min(row0 + kRows, rows) - 1, low_position, high_position);
     const int key_end = min(max(high_position + 1, prefix), length);
-    const int window_first = a.window > 0 ? max(low_position - a.window + 1, 0) : 0;  // below: the prefix only
+    const int window_first = a.window > 0 ? max(least_position - a.window + 1, 0) : 0;  // below: the prefix only
     // The next tile at or after `tile` that has a key for some row: between the
     // prefix and the window there is none.
     auto next_tile = [&](int tile) {
