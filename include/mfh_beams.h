@@ -43,7 +43,8 @@ typedef struct {
  * row number of the beam each continues).  Continuations of equal score come
  * in the order of their beams, and those of one beam in the order of their
  * logits and then of their tokens.  Scores are compared before they are
- * rounded to f32.
+ * rounded to f32; one below its range becomes -inf there, and keeps its token
+ * and parent.
  *
  * A continuation whose score is -inf or NaN is none, nor are those of a beam
  * one of whose logits, or whose score, is NaN or +inf.  Where a group has
