@@ -248,7 +248,10 @@ int mfh_paged_decode_workspace(const mfh_attention_shape* shape, const mfh_kv_ca
  * request's own ones: they decide how both are split over workgroups, and with
  * it the order of the sums, nothing else.  The workspace has to be as large as
  * mfh_paged_decode_shared_workspace says for these sizes; what it says for sizes
- * that are nowhere smaller (requests, groups and both bounds) does too. */
+ * that are nowhere smaller (requests, groups and both bounds) does too.
+ *
+ * Own tokens are split alike for all requests: a batch in which few have many
+ * times the others' is faster by mfh_paged_decode, which splits by lengths. */
 int mfh_paged_decode_shared(const mfh_attention_shape* shape, const mfh_kv_cache* cache, int32_t requests,
                             int32_t groups, const void* q, const void* k_cache, const void* v_cache,
                             const int32_t* table, int64_t table_stride, int32_t table_width, const int32_t* starts,

@@ -24,8 +24,10 @@
 // again: that costs less than one more launch.
 //
 // A step of few rows is two launches' latency: 4 rows of 32003 f32 6.2 and 5.7 us.
-// 256 rows of 131072 bf16 (67 MB, 13 us at a copy's rate) take 19.7 and 7.4: beside
-// the loads stand the exponentials, and two barriers and the list of each piece.
+// 256 rows of 131072 bf16 (67 MB, 13 us at a copy's rate) take 20.4 and 7.1: their
+// 1024 workgroups are what the card holds at once, all of which load and then all
+// compute the exponentials, the bound and the list.  With a quarter of the beams
+// ended (50 MB) they take 20.0 and 7.2, for the others' pieces are no faster.
 #include "common.hpp"
 #include "launch.hpp"
 #include "paged.hpp"
@@ -247,7 +249,6 @@ __global__ __launch_bounds__(kThreads, 8) void k_beam_rows(BeamArgs a)
 #pragma unroll
         for (int e = 1; e < P; e++) most = fmaxf(most, logit_of<DT>(packet[i], e));
         if (most > top) top = most, at = i;
-        
     }
     // (unpacked anew for each of its uses: kept unpacked, a workgroup's registers would
     // leave room for no other one)
@@ -266,7 +267,6 @@ __global__ __launch_bounds__(kThreads, 8) void k_beam_rows(BeamArgs a)
     for (int i = 0; i < PACKETS; i++) {
 #pragma unroll
         for (int e = 0; e < P; e++) part[e % 4] += exp2_fast((logit_of<DT>(packet[i], e) - base) * kLog2e);
-        
     }
     packed();
     double sum = (double)(part[0] + part[1]) + (double)(part[2] + part[3]);
@@ -444,8 +444,9 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
 
 // Packets of a thread: as many as leave every CU two workgroups, for what a
 // workgroup does once (the bound, the list) costs the same whatever its piece.
-// 256 rows of 131072 bf16: by 8 packets 27 us, by 1 47; 35 rows of 50001 f16: by 1
-// 12.8 us, by 8 16; 64 rows of 32003 f32: by 2 as here 14.5, by 4 13.8, by 8 15.5.
+// 256 rows of 131072 bf16: by 8 packets 27 us, by 1 47; 256 of 32000: by 4 as here
+// 18.0, by 8 18.7, by 2 18.5; 35 rows of 50001 f16: by 1 12.8 us, by 8 16.  In between
+// one more doubling can be 5% faster: 64 rows of 32003 f32 by 2 as here 14.2, by 4 13.6.
 struct Layout {
     int packets;
     int64_t pieces;

@@ -7,7 +7,9 @@
 // group's requests, and a workgroup takes 16, 32 or 64 of them.  Below some 64
 // columns bytes bound it, above the matrix units and the exponentials beside
 // them.  A request's own tokens are a group of one request.  Both kinds of
-// parts run in one launch, the shared ones first, and a second one joins them.
+// parts run in one launch, the shared ones first, and a second one joins them; where
+// a group has so many columns that prefill's kernels compute the shared parts, these
+// are a launch of their own in front.
 //
 // A wave takes tiles of 32 tokens on its own: whole rows of K and V into registers
 // while the tile before is worked on, from there to its part of LDS, and out of it
@@ -703,7 +705,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_shared_join(SharedArgs a, m
 
 // A wave a row; four of them where there are many parts, or too few rows to fill the
 // card (`few`): 16 requests of 32 heads and 17 parts 43.7 us in all, by a wave a row
-// 44.6; 190 of them and 4 parts 51.3 us, by a wave a row 48.9.
+// 44.6; 190 of them and 4 parts 51.3 us, by a wave a row 48.9.  Many: 1200 rows of 52
+// parts 56.3 us, by a wave a row 58.7; 2000 of 33 63.2 and 63.1; 4000 of 17 88.9 and 84.5.
 template <int DT>
 void launch_join(const SharedArgs& a, mfh_u32 few, hipStream_t s)
 {
@@ -718,9 +721,19 @@ void launch_join(const SharedArgs& a, mfh_u32 few, hipStream_t s)
 // columns, with which a workgroup fills a CU (24 groups of 4 to 32 columns over up
 // to 6000 e4m3 tokens: by 64 columns 94 us, by 32 48), and to 32 where there is less
 // to share than each request has for itself, whose workgroups a CU then holds two
-// of.  Of 256 columns on and long shared tokens prefill's kernels, whose tiles serve
-// 256 columns, are faster: 256 requests of 32 heads over 8, 16384 tokens, 120 us,
-// else 145; 64 such requests over 65536 122, else 146; but over 8192 47 and 43.
+// of: 24 groups of up to 96 columns over up to 500 e4m3 tokens, 1000 of their own,
+// 112 us, by 64 columns 143; one group is as fast by either, 64 requests of 32 heads
+// over 8 behind 400 bf16 tokens, 1000 of their own, 44 and 43.
+//
+// Of 256 columns on and long shared tokens prefill's kernels, whose tiles serve 256
+// columns, are faster.  32 heads over 8, bf16, by them and by 64 columns:
+//   256 requests over 16384 tokens    120 us  145      64 over 65536    122 us  146
+//   over 8192                         100     120      over 16384        62      68
+//   over 4096                          84      73      over 8192         52      43
+// The rule changes over at 2^22 columns times tokens: the third line left, the second
+// right.
+// Up to 16 groups, from which on 64 columns fill the card too: groups of 64 such
+// requests over 16384, 8 of them 242 us and 301, 16 560 and 555, 24 1428 and 814.
 //
 // Parts: as many as fill half of the card, so that the requests' own parts run beside
 // them on the other half; where the shared tokens take the waves many rounds (`rounds`,
