@@ -60,7 +60,7 @@ struct BeamArgs {
     int64_t row_bytes, history_stride;
     mfh_u32 beams, picks, vocab, pieces, slices;
     int32_t end_token;
-    Divider by_pieces, by_picks, by_slices;
+    Divider by_pieces, by_picks, by_slices, by_piece;  // by_piece: tokens of a piece
 };
 
 // A float as a whole number of the same order; -0 is 0.
@@ -112,7 +112,9 @@ struct Logit {
 
 // The `picks` largest of a workgroup's elements, in order, into `best` behind a
 // barrier.  each(least, f) calls f for every element of the thread, but may leave out
-// lower ones than `least`; top is the largest.
+// lower ones than `least`, and all others once f has returned false; top is the
+// largest.  `attempt` is false, with nothing done, where no bound is found or
+// more than the list holds reach it.
 template <typename K>
 struct Selection {
     K by_wave[kWaves][64];
@@ -123,7 +125,7 @@ struct Selection {
     mfh_u32 count;
 
     template <typename Each>
-    MFH_DEV void run(mfh_u32 picks, K top, K* best, Each each)
+    MFH_DEV bool attempt(mfh_u32 picks, K top, K* best, Each each, bool needs_bound = true)
     {
         const mfh_u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         by_wave[wave][lane] = top;
@@ -148,29 +150,38 @@ struct Selection {
         if (wave == 0 && rank[lane] == picks - 1) bound = mine;  // with fewer columns than picks none: everything is listed
         __syncthreads();
         const K least = bound;
+        if (needs_bound && !least.some()) return false;
         if (top.some() && top >= least)
             each(least, [&](K k) {
-                if (k.some() && k >= least) {
-                    const mfh_u32 at = atomicAdd(&count, 1u);
-                    if (at < kList) list[at] = k;
-                }
+                if (!k.some() || !(k >= least)) return true;
+                const mfh_u32 at = atomicAdd(&count, 1u);
+                if (at < kList) list[at] = k;
+                return at < kList;
             });
         __syncthreads();
         const mfh_u32 n = count;
-        if (n <= kList) {
-            for (mfh_u32 i = tid; i < n; i += kThreads) {
-                const K k = list[i];
-                mfh_u32 before = 0;
-                for (mfh_u32 j = 0; j < n; j++) before += list[j] > k;
-                if (before < picks) best[before] = k;
-            }
-            return;
+        if (n > kList) return false;
+        for (mfh_u32 i = tid; i < n; i += kThreads) {
+            const K k = list[i];
+            mfh_u32 before = 0;
+            for (mfh_u32 j = 0; j < n; j++) before += list[j] > k;
+            if (before < picks) best[before] = k;
         }
+        return true;
+    }
+
+    // One after the other where the attempt fails.
+    template <typename Each>
+    MFH_DEV void run(mfh_u32 picks, K top, K* best, Each each)
+    {
+        if (attempt(picks, top, best, each, false)) return;
+        const mfh_u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         K last = K::all();
         for (mfh_u32 i = 0; i < picks; i++) {
             K most = K::none();
             each(K::none(), [&](K k) {
                 if (last > k && k > most) most = k;
+                return true;
             });
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1) {
@@ -392,29 +403,76 @@ __global__ __launch_bounds__(kThreads) void k_beam_merge(BeamArgs a)
         if (n < firsts) mine[i] = candidate(list, FLAT ? n - list * a.picks : 0, first[i]);
         top = Key::choose(mine[i] > top, mine[i], top);
     }
-    if constexpr (!FLAT)
+    if constexpr (FLAT) {
+        s.run(a.picks, top, s_best, [&](const Key&, auto f) {
+#pragma unroll
+            for (mfh_u32 i = 0; i < 2; i++)
+                if (mine[i].some()) f(mine[i]);
+        });
+    } else {
         for (mfh_u32 list = threadIdx.x + 2 * kThreads; list < lists; list += kThreads) {
             const Key k = candidate(list, 0, keys[(int64_t)list * a.picks]);
             top = Key::choose(k > top, k, top);
         }
-    auto each = [&](const Key& least, auto f) {
-        if constexpr (FLAT) {
-#pragma unroll
-            for (mfh_u32 i = 0; i < 2; i++)
-                if (mine[i].some()) f(mine[i]);
-        } else {
+        // From the heads on, each list as far as the bound goes.
+        const bool done = s.attempt(a.picks, top, s_best, [&](const Key& least, auto f) {
             for (mfh_u32 list = threadIdx.x; list < lists; list += kThreads) {
                 Key k = Key::choose(list < kThreads, mine[0], mine[1]);
                 if (list >= 2 * kThreads) k = candidate(list, 0, keys[(int64_t)list * a.picks]);
                 for (mfh_u32 i = 1; k.some() && !(least > k); i++) {
-                    f(k);
+                    if (!f(k)) return;
                     if (i == a.picks) break;
                     k = candidate(list, i, keys[(int64_t)list * a.picks + i]);
                 }
             }
+        });
+        if (!done) {
+            // Fewer lists than picks, or heads far apart, give no bound that leaves few.  Then
+            // the best heads, and of what is behind them what can be among the best: entry i
+            // behind the j-th head has i + j others before it (3 groups of 31 beams, 62 picks
+            // of 68 tokens: 27 us, one pick after the other 1030; 256 beams, 64 picks of 32000
+            // f16: 114 and 960; asked first of every call, 4 us more where the heads suffice).
+            __syncthreads();
+            s.run(a.picks, top, s_best, [&](const Key&, auto f) {
+                for (mfh_u32 list = threadIdx.x; list < lists; list += kThreads) {
+                    Key k = Key::choose(list < kThreads, mine[0], mine[1]);
+                    if (list >= 2 * kThreads) k = candidate(list, 0, keys[(int64_t)list * a.picks]);
+                    f(k);
+                }
+            });
+            __syncthreads();
+            // (another i in a lane for each head: a column of threads has some of every rank)
+            constexpr int kEach = kMostPicks / kWaves;
+            auto place = [&](int e) { return (mfh_u32)(lane - 29 * (wave + e * kWaves)) & (kMostPicks - 1); };
+            mfh_u64 entry[kEach];
+            mfh_u32 from[kEach];
+            Key some[kEach];
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                const mfh_u32 j = wave + e * kWaves, i = place(e);
+                some[e] = Key::none(), entry[e] = 0, from[e] = 0;
+                if (i + j >= a.picks) continue;
+                const Key head = s_best[j];
+                if (i == 0) some[e] = head;
+                const mfh_u32 b = kMostBeams - 1 - (mfh_u32)(head.low >> 56);
+                if (i == 0 || !head.some() || s_ended[b]) continue;
+                from[e] = b * a.pieces + a.by_piece.quotient(~(mfh_u32)head.low & ((1u << kTokenBits) - 1));
+                entry[e] = keys[(int64_t)from[e] * a.picks + i];
+            }
+            top = Key::none();
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                if (entry[e] != 0) some[e] = candidate(from[e], place(e), entry[e]);
+                top = Key::choose(some[e] > top, some[e], top);
+            }
+            __syncthreads();
+            s.run(a.picks, top, s_best, [&](const Key&, auto f) {
+#pragma unroll
+                for (int e = 0; e < kEach; e++)
+                    if (some[e].some()) f(some[e]);
+            });
         }
-    };
-    s.run(a.picks, top, s_best, each);
+    }
     __syncthreads();
 
     auto token_of = [](const Key& k) { return k.some() ? (int32_t)(~k.low & ((1u << kTokenBits) - 1)) : -1; };
@@ -570,6 +628,7 @@ int mfh_beam_select(const mfh_beam_shape* shape, int32_t groups, const void* log
     const int64_t history_bytes = history ? shape->history_stride * shape->picks * 4 : 0;
     a.slices = (mfh_u32)std::max<int64_t>(1, std::min<int64_t>(history_bytes >> 14, dev->compute_units / groups));
     a.by_pieces = Divider(a.pieces), a.by_picks = Divider(a.picks), a.by_slices = Divider(a.slices);
+    a.by_piece = Divider((mfh_u32)(kThreads * l.packets * (16 / bytes)));
     hipStream_t s = (hipStream_t)stream;
     if (shape->dtype == kFloat32) launch_rows<kFloat32>(l, (unsigned)cells, s, a);
     else if (shape->dtype == kFloat16) launch_rows<kFloat16>(l, (unsigned)cells, s, a);
